@@ -27,6 +27,12 @@ class SpmdmConfig(C.Structure):
     ]
 
 
+class PagedCache(C.Structure):
+    """struct fbgemm_amd_paged_cache."""
+    _fields_ = [("row_ty", _I32), ("block_size", _I32), ("heads", _I32), ("dim", _I32), ("blocks", _I64),
+                ("key_strides", _I64 * 3), ("value_strides", _I64 * 3)]
+
+
 SYMBOLS = {
     "fbgemm_amd_last_error": (C.c_char_p, []),
     "fbgemm_amd_version": (C.c_char_p, []),
@@ -72,6 +78,11 @@ SYMBOLS = {
     "fbgemm_amd_pruned_array_lookup": (C.c_int, [_P, _P, _I32, _I64, _P, _I32, _P, _I32, _P, _P]),
     "fbgemm_amd_tbe_inplace_update": (C.c_int, [_P, _P, _P, _P, _I64, _P, _P, _I32, _P, _I64, _P, _P]),
     "fbgemm_amd_pruned_array_lookup_from_row_idx": (C.c_int, [_P, _I32, _P, _I64, _P, _I32, _P, _I32, _P, _P]),
+    "fbgemm_amd_kv_block_tables": (C.c_int, [_P, _P, _I32, _I64, _P, _I64, _I64, _P, _I64, _P, _I32, _I64, _P, _P, _P, _P, _P, _P, _P]),
+    "fbgemm_amd_kv_cache_append": (C.c_int, [C.POINTER(PagedCache), _P, _P, _I32, _I64, C.POINTER(_I64), C.POINTER(_I64), _P, _P, _P, _P, _P]),
+    "fbgemm_amd_paged_attention_workspace": (_I64, [C.POINTER(PagedCache), _I64, _I32, _I64]),
+    "fbgemm_amd_paged_attention": (C.c_int, [C.POINTER(PagedCache), _P, _I32, _I64, _I32, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I32, C.c_float, _I64, C.c_float, _P, _P, _P, _I64, _P]),
+    "fbgemm_amd_penalize_logits": (C.c_int, [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P, _I32, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _I64, _P]),
     "fbgemm_amd_unpadded_row_size_in_bytes": (_I32, [_I32, _I32, _I32]),
     "fbgemm_amd_padded_row_size_in_bytes": (_I32, [_I32, _I32, _I32, _I32]),
 }

@@ -18,8 +18,10 @@ SOURCES = ["lookup_both_i64_checked.hip", "lookup_both_i32_checked.hip", "lookup
            "lookup_lean_i64_exact_q8.hip", "lookup_lean_i64_fast_q8.hip", "lookup_lean_i32_exact_q8.hip", "lookup_lean_i32_fast_q8.hip",
            "lookup_matrix_i64.hip", "lookup_matrix_i32.hip", "lookup_burst_i64.hip", "lookup_burst_i32.hip", "lookup_i64.hip", "lookup_i32.hip", "lookup_i64_checked.hip", "lookup_i32_checked.hip", "lookup_i64_general.hip", "lookup_i32_general.hip",
            "lookup_kernels.hip", "index_ops_kernels.hip", "quantize_kernels.hip", "sequence_kernels.hip", "sequence_stream.hip",
-           "prune_kernels.hip", "remap_rank_kernels.hip", "split_bag_kernels.hip", "update_kernels.hip", "c_api.cpp"]
-HEADERS = ["cache_policy.h", "launchers.h", "lookup_both.h", "lookup_burst.h", "lookup_common.h", "lookup_device.h", "lookup_general.h", "lookup_lean.h", "lookup_matrix.h", os.path.join("..", "..", "include", "fbgemm_amd.h"),
+           "prune_kernels.hip", "remap_rank_kernels.hip", "split_bag_kernels.hip", "update_kernels.hip",
+           "paged_attention_bf16.hip", "paged_attention_fp16.hip", "paged_attention_bf16_rows8.hip", "paged_attention_fp16_rows8.hip",
+           "kv_append.hip", "kv_block_tables.hip", "penalize_logits.hip", "decode_api.cpp", "c_api.cpp"]
+HEADERS = ["api_error.h", "cache_policy.h", "decode.h", "launchers.h", "lookup_both.h", "lookup_burst.h", "lookup_common.h", "lookup_device.h", "lookup_general.h", "lookup_lean.h", "lookup_matrix.h", "paged_attention.h", "rowwise_code.h", os.path.join("..", "..", "include", "fbgemm_amd.h"),
            os.path.join("..", "..", "include", "fbgemm_amd_bench.h")]
 
 # -ffp-contract=off: the kernels spell out every fma; nothing else may be fused,
@@ -110,7 +112,7 @@ def build_torch_op(verbose=False):
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch.compiled_with_cxx11_abi()),
            f"-I{tdir}/include", f"-I{tdir}/include/torch/csrc/api/include", "-I/opt/rocm/include",
-           "-o", TORCH_OP_OUT, os.path.join(CSRC, "torch_op.cpp"),
+           "-o", TORCH_OP_OUT, os.path.join(CSRC, "torch_op.cpp"), os.path.join(CSRC, "torch_op_decode.cpp"),
            f"-L{os.path.dirname(OUT)}", "-lfbgemm_amd", f"-L{tdir}/lib", "-ltorch_cpu", "-lc10", "-lc10_hip",
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tdir}/lib"]
     _run(cmd, verbose)

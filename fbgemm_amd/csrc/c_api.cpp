@@ -16,6 +16,7 @@
 
 #include "../../include/fbgemm_amd.h"
 #include "../../include/fbgemm_amd_bench.h"
+#include "api_error.h"
 #include "cache_policy.h"
 #include "lookup_common.h"
 
@@ -23,11 +24,9 @@
 
 using namespace fbgemm_amd;
 
-namespace {
+static thread_local char g_err[512] = "";
 
-thread_local char g_err[512] = "";
-
-int fail(int code, const char* fmt, ...) {
+int fbgemm_amd::fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
@@ -35,11 +34,7 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-#define HIP_TRY(expr)                                                                   \
-  do {                                                                                  \
-    hipError_t e_ = (expr);                                                             \
-    if (e_ != hipSuccess) return fail(FBGEMM_AMD_E_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
-  } while (0)
+namespace {
 
 int type_bits(int ty) {
   switch (ty) {

@@ -1,0 +1,151 @@
+// New key and value rows into their slots of a paged cache: cache[slot / S][head][slot % S] = row,
+// as they are, or as the framework's 8-bit rows (fp16 scale and bias in front, then the bytes).
+//
+// Bound by memory: every byte is read once and written once (8-bit rows: half of it written). A
+// thread takes a piece of 16 bytes (less where strides or addresses ask for it) of one row of both
+// keys and values, so that two loads are in flight and the slot is looked up once for the two.
+#include "decode.h"
+#include "rowwise_code.h"
+
+namespace fbgemm_amd {
+
+namespace {
+
+constexpr int THREADS = 256;
+typedef __attribute__((ext_vector_type(4))) uint32_t piece16;
+typedef __attribute__((ext_vector_type(2))) uint32_t piece8;
+
+// Where a slot's rows begin, without the head; -1: the token has none
+struct Place {
+  int64_t block, in_block;
+};
+__device__ __forceinline__ bool place_of(const AppendArgs& a, int64_t token, bool report, Place& p) {
+  const int64_t slot = a.slots[token];
+  if (slot < 0 || slot >= a.total_slots) {
+    if (report && slot != -1 && a.status) status_index(a.status, token); // -1: a token of no request
+    return false;
+  }
+  if (a.total_slots <= 0x7fffffff) { // the same for every thread
+    p.block = divide((uint32_t)slot, a.block);
+    p.in_block = (uint32_t)slot - (uint32_t)p.block * a.block.d;
+  } else {
+    p.block = slot / a.block.d;
+    p.in_block = slot - p.block * a.block.d;
+  }
+  return true;
+}
+
+template <typename piece_t>
+__global__ __launch_bounds__(THREADS) void kv_append_kernel(const AppendArgs a) {
+  const uint32_t pieces = a.per_row.d * (uint32_t)a.heads; // of a token
+  const int64_t n = a.tokens * pieces;
+  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * THREADS) {
+    const int64_t token = n <= 0xffffffffll ? (uint32_t)i / pieces : i / pieces;
+    const uint32_t in_token = (uint32_t)(i - token * pieces);
+    const uint32_t head = divide(in_token, a.per_row), piece = in_token - head * a.per_row.d;
+    Place p;
+    if (!place_of(a, token, in_token == 0, p)) continue;
+    piece_t v[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      v[k] = *reinterpret_cast<const piece_t*>(a.in[k] + token * a.token_stride[k] + head * a.head_stride[k] + (int64_t)piece * sizeof(piece_t));
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const CacheRows& c = a.cache[k];
+      *reinterpret_cast<piece_t*>(c.base + p.block * c.block_stride + head * c.head_stride + p.in_block * c.slot_stride +
+                                  (int64_t)piece * sizeof(piece_t)) = v[k];
+    }
+  }
+}
+
+struct F32 {
+  static constexpr int BYTES = 4;
+  static __device__ __forceinline__ float at(const char* p) { return *reinterpret_cast<const float*>(p); }
+};
+struct F16 {
+  static constexpr int BYTES = 2;
+  static __device__ __forceinline__ float at(const char* p) { return half_bits_to_float(*reinterpret_cast<const uint16_t*>(p)); }
+};
+struct B16 {
+  static constexpr int BYTES = 2;
+  static __device__ __forceinline__ float at(const char* p) { return q_bits_to_float((uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16); }
+};
+
+// One row per group of `lanes` lanes (a power of two), RUN elements a lane and step; a row's elements
+// stay in registers between the search for its extremes and the rounding while they are one step's.
+// The format holds fp16 numbers: elements beyond fp16's largest count as that, NaN as zero.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void kv_append_rows8_kernel(const AppendArgs a, const int lanes) {
+  constexpr int RUN = 8;
+  const int sub = threadIdx.x & (lanes - 1);
+  const int64_t rows = a.tokens * a.heads;
+  const int64_t groups = (int64_t)gridDim.x * (THREADS / lanes);
+  for (int64_t row = (int64_t)blockIdx.x * (THREADS / lanes) + threadIdx.x / lanes; row < rows; row += groups) {
+    const int64_t token = rows <= 0xffffffffll ? (uint32_t)row / (uint32_t)a.heads : row / a.heads;
+    const int64_t head = row - token * a.heads;
+    Place p;
+    if (!place_of(a, token, head == 0 && sub == 0, p)) continue; // the whole group
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const char* in = a.in[k] + token * a.token_stride[k] + head * a.head_stride[k];
+      const CacheRows& c = a.cache[k];
+      char* out = c.base + p.block * c.block_stride + head * c.head_stride + p.in_block * c.slot_stride;
+      const auto element = [&](int j) {
+        const float x = T::at(in + (int64_t)j * T::BYTES);
+        return x != x ? 0.0f : __builtin_fminf(__builtin_fmaxf(x, -65504.0f), 65504.0f);
+      };
+      float lo = __builtin_inff(), hi = -__builtin_inff();
+      for (int j = sub * RUN; j < a.dim; j += lanes * RUN)
+#pragma unroll
+        for (int e = 0; e < RUN; ++e)
+          if (j + e < a.dim) {
+            const float x = element(j + e);
+            lo = __builtin_fminf(lo, x);
+            hi = __builtin_fmaxf(hi, x);
+          }
+      for (int m = 1; m < lanes; m <<= 1) {
+        lo = __builtin_fminf(lo, __shfl_xor(lo, m, 64));
+        hi = __builtin_fmaxf(hi, __shfl_xor(hi, m, 64));
+      }
+      const RowCode code = row_code<8>(lo, hi, 0, 1);
+      if (sub == 0) *reinterpret_cast<uint32_t*>(out) = (code.sb0 & 0xffffu) | (code.sb1 << 16);
+      for (int j = sub * RUN; j < a.dim; j += lanes * RUN)
+#pragma unroll
+        for (int e = 0; e < RUN; ++e)
+          if (j + e < a.dim) {
+            const float r = __builtin_rintf((element(j + e) - code.minimum) * code.inverse_scale);
+            out[4 + j + e] = (char)(uint8_t)__builtin_fminf(__builtin_fmaxf(r, 0.0f), 255.0f);
+          }
+    }
+  }
+}
+
+int grid_for(int64_t items, int per_block) {
+  const int64_t want = (items + per_block - 1) / per_block;
+  return (int)(want > 8192 ? 8192 : want);
+}
+
+} // namespace
+
+hipError_t launch_kv_append(const AppendArgs& a, int piece_bytes, hipStream_t stream) {
+  const int grid = grid_for(a.tokens * a.heads * a.per_row.d, THREADS);
+  switch (piece_bytes) {
+    case 16: kv_append_kernel<piece16><<<grid, THREADS, 0, stream>>>(a); break;
+    case 8: kv_append_kernel<piece8><<<grid, THREADS, 0, stream>>>(a); break;
+    case 4: kv_append_kernel<uint32_t><<<grid, THREADS, 0, stream>>>(a); break;
+    default: kv_append_kernel<uint16_t><<<grid, THREADS, 0, stream>>>(a); break;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_append_rows8(const AppendArgs& a, int32_t input_ty, hipStream_t stream) {
+  int lanes = 1;
+  while (lanes < 64 && lanes * 8 < a.dim) lanes <<= 1;
+  const int grid = grid_for(a.tokens * a.heads, THREADS / lanes);
+  if (input_ty == ST_FP32) kv_append_rows8_kernel<F32><<<grid, THREADS, 0, stream>>>(a, lanes);
+  else if (input_ty == ST_FP16) kv_append_rows8_kernel<F16><<<grid, THREADS, 0, stream>>>(a, lanes);
+  else kv_append_rows8_kernel<B16><<<grid, THREADS, 0, stream>>>(a, lanes);
+  return hipGetLastError();
+}
+
+} // namespace fbgemm_amd

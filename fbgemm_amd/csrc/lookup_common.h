@@ -23,6 +23,7 @@ enum : int32_t {
   ERR_BAG_OVERRUN = 2,        // a bag ends past index_size / past the index array
   ERR_LENGTH_MISMATCH = 4,    // sum of bag lengths != index_size
   ERR_NEGATIVE_LENGTH = 8,    // offsets decrease (the reference's result is then undefined)
+  ERR_OUT_OF_BLOCKS = 16,     // a free list has no page left for a token
 };
 
 // Device status block: word 0 = OR of ERR_* bits, words 2..3 = the smallest

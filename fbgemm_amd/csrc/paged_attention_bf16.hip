@@ -1,0 +1,6 @@
+// One instance of the attention kernels (paged_attention.h): bf16 queries, rows of the same type.
+#include "paged_attention.h"
+
+namespace fbgemm_amd {
+hipError_t launch_paged_attention_bf16(const AttentionArgs& a, hipStream_t stream) { return attention::launch_any<true, false>(a, stream); }
+} // namespace fbgemm_amd

@@ -50,7 +50,8 @@ enum {
   FBGEMM_AMD_ERR_INDEX_OUT_OF_RANGE = 1,
   FBGEMM_AMD_ERR_BAG_OVERRUN = 2,
   FBGEMM_AMD_ERR_LENGTH_MISMATCH = 4,
-  FBGEMM_AMD_ERR_NEGATIVE_LENGTH = 8
+  FBGEMM_AMD_ERR_NEGATIVE_LENGTH = 8,
+  FBGEMM_AMD_ERR_OUT_OF_BLOCKS = 16 /* fbgemm_amd_kv_block_tables only */
 };
 
 #define FBGEMM_AMD_STATUS_BYTES 16
@@ -567,6 +568,102 @@ int fbgemm_amd_rowwise_prune_map(const float* d_indicator, int64_t rows, double 
                                  void* stream);
 int fbgemm_amd_rowwise_prune_gather(const void* d_weights, int64_t rows, int64_t row_bytes, const void* d_remap,
                                     int32_t index_bits, void* d_output, int64_t output_rows, void* stream);
+
+/* ---- a decoding step over a paged key-value cache ---------------------------- *
+ *
+ * Operators of language-model serving that have no counterpart in the reference's
+ * quantized-embedding path. A cache is an array of blocks (pages) of block_size
+ * tokens; a request's tokens are those of the blocks its table lists, in order.
+ * Asynchronous, capture-safe; nothing is allocated and nothing waits. Lengths and
+ * lists live on the device, so a step needs no copy to the host.
+ *
+ * fbgemm_amd_kv_block_tables: pages, slots and positions for the tokens a step adds.
+ * Request r holds d_lengths[r] tokens and gets d_new_tokens[r] (both int32 or int64).
+ * Its table (table_width entries, table_stride apart; those of the tokens it holds
+ * are read, the entries behind them written) gets the next blocks of d_free_blocks,
+ * requests in order, from *d_free_start on; *d_free_next is the place behind the last
+ * block taken (beyond free_numel: that many are missing). New token k of request r is
+ * number d_offsets[r] + k of the step, its position is d_lengths[r] + k, its slot
+ * table[position / block_size] * block_size + position % block_size, or -1 where
+ * there is no block for it (table too narrow, free list exhausted, a negative entry).
+ * d_slots and d_positions hold num_tokens entries: those behind the last token are -1
+ * and 0; tokens beyond num_tokens get none. d_total_lengths = lengths + new tokens.
+ * Called again with the same inputs it writes the same. d_status (may be NULL: then
+ * the entries say it all): NEGATIVE_LENGTH (counted as 0), BAG_OVERRUN (a table too
+ * narrow), OUT_OF_BLOCKS, LENGTH_MISMATCH (the new tokens' sum is not num_tokens).
+ * d_free_next must not be d_free_start, nor d_total_lengths d_lengths. */
+int fbgemm_amd_kv_block_tables(
+    const void* d_lengths, const void* d_new_tokens, int32_t index_bits, int64_t requests, int32_t* d_block_tables,
+    int64_t table_stride, int64_t table_width, const int32_t* d_free_blocks, int64_t free_numel, const int32_t* d_free_start,
+    int32_t block_size, int64_t num_tokens, int64_t* d_slots, int64_t* d_positions, int32_t* d_offsets, void* d_total_lengths,
+    int32_t* d_free_next, void* d_status, void* stream);
+
+/* Keys and values are two arrays [blocks][heads][block_size][row]; strides (blocks,
+ * heads, slots) in elements of storage (INT8: bytes), a row's elements next to each
+ * other. INT8 rows are the table-batched operator's: fp16 scale, fp16 bias, dim bytes
+ * (dim + 4 bytes, on 4-byte boundaries). */
+typedef struct fbgemm_amd_paged_cache {
+  int32_t row_ty;     /* FBGEMM_AMD_FP32/FP16/BF16/INT8 */
+  int32_t block_size; /* tokens of a block */
+  int32_t heads, dim; /* of keys and values */
+  int64_t blocks;
+  int64_t key_strides[3], value_strides[3];
+} fbgemm_amd_paged_cache;
+
+/* New rows into their slots: cache[slot / block_size][head][slot % block_size] = row.
+ * d_key and d_value are [tokens][heads][dim] with the strides (tokens, heads) given in
+ * elements. A cache of FP32 / FP16 / BF16 rows takes rows of its own type as they are;
+ * an INT8 cache takes any of the three and stores what fbgemm_amd_quantize_rowwise
+ * (bit_rate 8, sb_float 0, FBGEMM_AMD_QLAYOUT_TBE) makes of them, with elements beyond
+ * fp16's range at its end and NaN as 0 (a zero bias may have either sign). Slot -1 is
+ * skipped; another slot outside the cache too, and is recorded in d_status (may be
+ * NULL) as INDEX_OUT_OF_RANGE with the token's number. Of several tokens with one slot
+ * any one is stored. */
+int fbgemm_amd_kv_cache_append(
+    const fbgemm_amd_paged_cache* cache, const void* d_key, const void* d_value, int32_t input_ty, int64_t tokens,
+    const int64_t* key_strides, const int64_t* value_strides, const int64_t* d_slots, void* d_key_cache, void* d_value_cache,
+    void* d_status, void* stream);
+
+/* Attention of one new token per request. d_query [requests][query_heads][dim] (FP16
+ * or BF16; strides in elements, rows on 16-byte boundaries), query head h reads key
+ * head h / (query_heads / heads). Of request r's d_lengths[r] tokens (the new one
+ * among them; more than its table has room for count as that many) all are read, or
+ * with window > 0 the last `window`:
+ *   s_t = scale * q . k_t, with softcap > 0 softcap * tanh(s_t / softcap),
+ *   d_output [requests][query_heads][dim] (the queries' type, dense) = softmax(s) v,
+ *   d_lse [requests][query_heads] = log(sum_t exp(s_t)).
+ * Tokens of a block outside [0, blocks) are left out; where no token is left the output
+ * is 0 and d_lse -inf. What the cache holds where no token is may be anything; a
+ * token's key or value that is not finite makes its queries' outputs not finite. A
+ * cache of FP16 / BF16 rows must have the queries' type and rows on 16-byte boundaries,
+ * one of INT8 rows goes with either. dim: a multiple of 8, at most 256. Scores, weights
+ * and sums are fp32 (weights go to the matrix cores as two 16-bit numbers); results do
+ * not depend on the order in which workgroups run. d_workspace: scratch of
+ * fbgemm_amd_paged_attention_workspace bytes that no other call uses at the same time. */
+int64_t fbgemm_amd_paged_attention_workspace(const fbgemm_amd_paged_cache* cache, int64_t requests, int32_t query_heads, int64_t table_width);
+int fbgemm_amd_paged_attention(
+    const fbgemm_amd_paged_cache* cache, const void* d_query, int32_t query_ty, int64_t requests, int32_t query_heads,
+    int64_t query_request_stride, int64_t query_head_stride, const void* d_key_cache, const void* d_value_cache,
+    const int32_t* d_block_tables, int64_t table_stride, int64_t table_width, const void* d_lengths, int32_t index_bits,
+    float scale, int64_t window, float softcap, void* d_output, float* d_lse, void* d_workspace, int64_t workspace_bytes, void* stream);
+
+/* Logits [rows][vocab] (FP32, FP16 or BF16) made ready to sample from. A row's tokens
+ * are d_tokens[d_offsets[row] .. d_offsets[row + 1] - 1], the first
+ * d_prompt_lengths[row] (NULL: none) of them its prompt; tokens outside the vocabulary
+ * are passed over. In fp32, in this order, rounded once at the end:
+ *   a token of the list:              x = x > 0 ? x / repetition : x * repetition
+ *   n > 0 times behind the prompt:    x = x - frequency * n, then x = x - presence
+ *   a bias for it (the last one):     x = x + bias
+ *   its bit of the mask is 0:         x = -inf, whatever x was
+ * The three penalties are one fp32 number per row (NULL: 1, 0, 0), biases a list of
+ * (id, value) per row like the tokens' (all lists have index_bits), the mask one bit
+ * per token, bit v % 32 of word v / 32 of a row (mask_stride words apart). d_output may
+ * be d_logits (with the same stride). */
+int fbgemm_amd_penalize_logits(
+    const void* d_logits, int32_t logits_ty, int64_t rows, int64_t vocab, int64_t logits_stride, const void* d_tokens,
+    int64_t tokens_numel, const void* d_offsets, const void* d_prompt_lengths, int32_t index_bits, const float* d_repetition,
+    const float* d_frequency, const float* d_presence, const void* d_bias_ids, const float* d_bias_values, int64_t bias_numel,
+    const void* d_bias_offsets, const int32_t* d_mask, int64_t mask_stride, void* d_output, int64_t output_stride, void* stream);
 
 /* Wait for everything enqueued on `stream` (hipStreamSynchronize), for callers
  * of the asynchronous entry points that hold no HIP headers. */
