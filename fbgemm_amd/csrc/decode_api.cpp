@@ -98,6 +98,10 @@ int check_attention(const fbgemm_amd_paged_cache* cache, int64_t requests, int32
   if (query_heads <= 0 || query_heads > (1 << 20) || query_heads % cache->heads)
     return fail(FBGEMM_AMD_E_ARG, "query heads must be a multiple of the cache's heads");
   if (table_width < 0) return fail(FBGEMM_AMD_E_ARG, "table_width must not be negative");
+  const int64_t sets = (int64_t)cache->heads * ((query_heads / cache->heads + ATTENTION_ROWS - 1) / ATTENTION_ROWS);
+  const int64_t units = attention_max_tokens(*cache, table_width) / ATTENTION_CHUNK + 2;
+  if (requests > 0 && units > MOST / (requests * sets)) // requests * sets < 2^45
+    return fail(FBGEMM_AMD_E_UNSUPPORTED, "tables for fewer than 2^31 times %d tokens, over all requests and heads, are supported", ATTENTION_CHUNK);
   return 0;
 }
 
@@ -227,6 +231,7 @@ int fbgemm_amd_paged_attention(
   a.value = rows_of(const_cast<void*>(d_value_cache), cache->value_strides, cache->row_ty);
   const int64_t row_align = rows8 ? 4 : 16;
   bool aligned = divides(16, {a.query_request_stride, a.query_head_stride}) && (uintptr_t)d_query % 16 == 0;
+  if (a.key.slot_stride >= (1 << 26) || a.value.slot_stride >= (1 << 26)) return fail(FBGEMM_AMD_E_UNSUPPORTED, "tokens of a block must be less than 64 MiB apart");
   for (const CacheRows* r : {&a.key, &a.value})
     aligned = aligned && divides(row_align, {r->block_stride, r->head_stride, r->slot_stride}) && (uintptr_t)r->base % row_align == 0;
   if (!aligned) return fail(FBGEMM_AMD_E_ARG, "queries and 16-bit rows must begin on 16-byte boundaries, 8-bit rows on 4-byte ones");

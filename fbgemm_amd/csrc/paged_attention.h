@@ -25,8 +25,8 @@
 // 8-bit rows (fp16 scale a_t and bias b_t in front): s_t = a_t (q . k8_t) + b_t sum(q), and weights
 // p_t a_t for the bytes, p_t b_t for the bias: 0 .. 255 are exact in bf16 and fp16.
 //
-// Work: units of CHUNK tokens of a (request, key head, 16 queries), numbered in that order; worker w
-// of W (at most U) takes units w U / W .. (w + 1) U / W - 1, whatever requests they are of, so that all workers
+// Work: units of CHUNK tokens of a (request, key head, 16 queries), numbered in that order; each
+// of W workers (at most U) takes U / W of them in a row, whatever requests they are of, so that all workers
 // end together however long the requests are. A worker's four waves take 32 tokens each in turn and
 // are joined in LDS; what a worker has whole it writes out, of what it shares with its neighbours (its
 // first and its last pair) it leaves the sums, which a second launch joins in order.
@@ -114,12 +114,47 @@ __device__ __forceinline__ uint4 widen(uint32_t a, uint32_t b) {
 __device__ __forceinline__ float half_at(uint32_t pair, int i) { return (float)__builtin_bit_cast(f16x2, pair)[i]; }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// n tokens of a request from `lo` on, in units of CHUNK from `base` on
+// Tables and lengths are written by nobody while a kernel runs: where an address is the same for the
+// wave, the scalar unit reads them, apart from the rows' loads and what waits for these.
+template <typename T>
+using constant = const __attribute__((address_space(4))) T*;
+template <typename T>
+__device__ __forceinline__ constant<T> as_constant(const void* p) {
+  return (constant<T>)reinterpret_cast<uintptr_t>(p);
+}
+
+// A tile's rows as a buffer: its address sits in scalar registers, a lane adds 32 bits, a row the scalar offset. Every
+// load is inside the tile by the lanes' own offsets; the size is there to be given.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const char* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, 0x7fffffff, 0x00027000);
+}
+template <int N>
+__device__ __forceinline__ void fetch(uint32_t (&to)[N], __amdgpu_buffer_rsrc_t rows, uint32_t lane, uint32_t row, uint32_t piece) {
+  if constexpr (N == 4) {
+    const auto w = __builtin_amdgcn_raw_buffer_load_b128(rows, lane + piece, row, 0);
+    to[0] = w[0], to[1] = w[1], to[2] = w[2], to[3] = w[3];
+  } else if constexpr (N == 2) {
+    const auto w = __builtin_amdgcn_raw_buffer_load_b64(rows, lane + piece, row, 0);
+    to[0] = w[0], to[1] = w[1];
+  } else {
+    to[0] = __builtin_amdgcn_raw_buffer_load_b32(rows, lane + piece, row, 0);
+  }
+}
+
+// the largest over the four lanes n, 16 + n, 32 + n, 48 + n
+__device__ __forceinline__ float group_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  x = __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
+
+// A request's tokens that count, lo <= t < end, in units of CHUNK from `base` on
 struct Span {
   int32_t base, lo, end, units;
 };
-__device__ __forceinline__ Span span_of(const AttentionArgs& a, int64_t request) {
-  int64_t len = a.idx64 ? reinterpret_cast<const int64_t*>(a.lengths)[request] : (int64_t) reinterpret_cast<const int32_t*>(a.lengths)[request];
+__device__ __forceinline__ Span span_of(const AttentionArgs& a, int32_t request) {
+  int64_t len = a.idx64 ? as_constant<int64_t>(a.lengths)[request] : (int64_t)as_constant<int32_t>(a.lengths)[request];
   len = len < 0 ? 0 : len > a.max_tokens ? a.max_tokens : len;
   Span s;
   s.end = (int32_t)len;
@@ -130,97 +165,189 @@ __device__ __forceinline__ Span span_of(const AttentionArgs& a, int64_t request)
   return s;
 }
 
-__device__ __forceinline__ int64_t wave_sum(int64_t v) {
+// U units over W workers: the first U % W have one more
+struct Shares {
+  uint32_t each, more;
+  __device__ __forceinline__ Shares(uint32_t units, uint32_t workers) : each(units / workers), more(units - each * workers) {}
+  __device__ __forceinline__ uint32_t begin(uint32_t worker) const { return worker * each + (worker < more ? worker : more); }
+  __device__ __forceinline__ uint32_t worker_of(uint32_t unit) const {
+    const uint32_t longer = more * (each + 1);
+    return unit < longer ? unit / (each + 1) : more + (unit - longer) / each;
+  }
+};
+
+__device__ __forceinline__ uint32_t inclusive_sum(uint32_t v, int lane) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t lo = __shfl_xor((uint32_t)v, d, 64), hi = __shfl_xor((uint32_t)((uint64_t)v >> 32), d, 64);
-    v += (int64_t)(((uint64_t)hi << 32) | lo);
+    const uint32_t o = __shfl_up(v, d, 64);
+    v += lane >= d ? o : 0;
   }
   return v;
 }
 
-// ROWS8: rows of the 8-bit format. DP: columns the code is laid out for (dim <= DP). PAGE16: pages are
-// whole 16-token tiles, whose addresses are then the same for the wave.
-template <bool BF16, bool ROWS8, int DP, bool PAGE16>
-__global__ __launch_bounds__(64 * ATT_WAVES, DP > 128 ? 1 : 2) void paged_attention_kernel(const AttentionArgs a) {
-  constexpr int KP = DP / 32;                   // products of a key tile
-  constexpr int VP = DP / 16;                   // columns of a lane in the value products
-  constexpr int HALVES = VP > 8 ? 2 : 1;        // pieces of at most 8 columns
-  constexpr int VC = VP / HALVES;               // columns of a piece: 8, or 4 of DP = 64
-  constexpr int EL = ROWS8 ? 1 : 2;             // bytes of an element
-  constexpr int HEAD = ROWS8 ? 4 : 0;           // of a row, in front of its elements
-  constexpr bool PBF16 = ROWS8 ? true : BF16;   // type of the weights: scales go into them, so 8-bit rows take bf16's range
-  constexpr float SHIFT = PBF16 ? 0.0f : 14.0f; // weights are 2^SHIFT times larger
-  constexpr int VREGS = ROWS8 ? (VC + 3) / 4 : VC / 2; // registers of a piece
-  __shared__ float s_acc[ATT_WAVES][ATTENTION_ROWS][DP + 4];
-  __shared__ float s_ml[ATT_WAVES][ATTENTION_ROWS][2];
-  __shared__ int64_t s_scan[64 * ATT_WAVES];
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int worker = blockIdx.x;
+// ROWS8: rows of the 8-bit format. DP: columns the code is laid out for; FULL: dim is DP, else less: lanes that would have the
+// columns behind read the row's first ones in their place, which meet zeros in the queries or make outputs that nobody wants.
+// PAGE16: pages are whole 16-token tiles, whose addresses are then the same for the wave.
+template <bool BF16, bool ROWS8, int DP, bool FULL, bool PAGE16>
+struct Attention {
+  static constexpr int KP = DP / 32;                   // products of a key tile
+  static constexpr int HALVES = DP > 128 ? 2 : 1;      // pieces of a value row that a lane holds
+  static constexpr int VC = DP / 16 / HALVES;          // columns of a piece: 8, or 4 of DP = 64
+  static constexpr int EL = ROWS8 ? 1 : 2;             // bytes of an element
+  static constexpr int HEAD = ROWS8 ? 4 : 0;           // of a row, in front of its elements
+  static constexpr bool PBF16 = ROWS8 ? true : BF16;   // type of the weights: scales go into them, so 8-bit rows take bf16's range
+  static constexpr float SHIFT = PBF16 ? 0.0f : 14.0f; // weights are 2^SHIFT times larger
+  static constexpr int VREGS = ROWS8 ? (VC + 3) / 4 : VC / 2; // registers of a value piece
+  static constexpr int KREGS = ROWS8 ? 2 : 4;          // registers of a key piece
 
-  // ---- the worker's units ----
-  const int64_t sets = (int64_t)a.kv_heads * a.q_tiles;
-  int64_t total = 0;
-  for (int64_t b = tid; b < a.requests; b += 64 * ATT_WAVES) total += span_of(a, b).units;
-  total = wave_sum(total);
-  if (lane == 0) s_scan[wave] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < ATT_WAVES; ++w) total += s_scan[w];
-  __syncthreads();
-  const int64_t U = total * sets;
-  const int64_t W = U < a.workers ? U : a.workers; // each has a unit at least
-  if (tid == 0) a.joins[worker] = make_int4(-1, 0, 0, 0);
-  if (worker >= W) return;
-  int64_t unit = (int64_t)worker * U / W;
-  const int64_t unit_end = (int64_t)(worker + 1) * U / W;
-  // the request that holds the first one: the last whose sum of units before it is not above unit / sets
-  int64_t request = 0, before = 0; // units (without sets) of the requests before it
-  for (int64_t b0 = 0;; b0 += 64 * ATT_WAVES) {
-    const int64_t b = b0 + tid;
-    int64_t sum = b < a.requests ? span_of(a, b).units : 0;
-    s_scan[tid] = sum;
-    __syncthreads();
-    for (int d = 1; d < 64 * ATT_WAVES; d <<= 1) {
-      const int64_t other = tid >= d ? s_scan[tid - d] : 0;
-      __syncthreads();
-      sum += other;
-      s_scan[tid] = sum;
-      __syncthreads();
-    }
-    const int64_t want = unit / sets - before;
-    if (want < s_scan[64 * ATT_WAVES - 1]) {
-      int lo = 0, hi = 64 * ATT_WAVES - 1; // the first whose inclusive sum is above
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s_scan[mid] > want) hi = mid;
-        else lo = mid + 1;
-      }
-      request = b0 + lo;
-      before += lo ? s_scan[lo - 1] : 0;
-      break;
-    }
-    before += s_scan[64 * ATT_WAVES - 1];
-    __syncthreads();
+  // what a wave has loaded of 32 tokens
+  struct Tile {
+    uint32_t k[2][KP][KREGS];
+    uint32_t v[HALVES][8][VREGS];
+    uint32_t k_pair[ROWS8 ? 8 : 1], v_pair[ROWS8 ? 8 : 1];
+    uint32_t seen; // bit j: this lane's token j counts
+    bool partial;  // some token of the tile does not (the same for the wave)
+  };
+  // where its pages are: PAGE16 of the two 16-token halves, else of token `lane & 31`
+  struct Pages {
+    int block[2];
+  };
+
+  const AttentionArgs& a;
+  const int lane, n, g;
+  uint32_t key_lane, value_lane; // bytes from a row's beginning to the lane's first piece
+  uint32_t key_rows, value_rows; // PAGE16: from a tile's, of rows n and 4 g
+  const char *key_base, *value_base;
+  const int32_t* table;
+  Span span;
+  int last_column;
+
+  __device__ __forceinline__ Attention(const AttentionArgs& args, int lane_) : a(args), lane(lane_), n(lane_ & 15), g(lane_ >> 4) {
+    key_lane = HEAD + 8 * g * EL;
+    value_lane = HEAD + (FULL || n * VC < a.dim ? n * VC * EL : 0);
+    key_rows = n * (uint32_t)a.key.slot_stride + key_lane;
+    value_rows = 4 * g * (uint32_t)a.value.slot_stride + value_lane;
   }
-  request = __builtin_amdgcn_readfirstlane((int)request);
 
-  // ---- segment after segment: units of one (request, key head, tile of queries) ----
-  while (unit < unit_end) {
-    const Span span = span_of(a, request);
-    const int64_t in_request = unit - before * sets;
-    const int set = (int)(in_request / span.units);
-    const int c0 = (int)(in_request - (int64_t)set * span.units);
-    const int64_t left = unit_end - unit;
-    const int c1 = left < span.units - c0 ? c0 + (int)left : span.units;
-    const int head = set / a.q_tiles, q0 = (set - head * a.q_tiles) * ATTENTION_ROWS;
-    const int rows = a.group - q0 < ATTENTION_ROWS ? a.group - q0 : ATTENTION_ROWS;
+  // bytes from the lane's first piece to the next ones
+  __device__ __forceinline__ uint32_t key_piece(int i) const { return FULL || 32 * i + 8 * g < a.dim ? 32 * i * EL : 0u - 8 * g * EL; }
+  __device__ __forceinline__ uint32_t value_piece(int h) const { return FULL || h == 0 || 128 * h + n * VC < a.dim ? 128 * h * EL : 0u; }
 
-    // queries: lane (n, g) holds columns 32 c + 8 g .. + 7 of query n
-    uint4 q[KP];
-    float q_sum = 0.0f;
+  __device__ __forceinline__ int token_of(int j) const { return (j >> 2) * 16 + 4 * g + (j & 3); } // of this lane's values and scores, in the tile
+
+  __device__ __forceinline__ Pages pages(int t0) const {
+    Pages p;
+    if (PAGE16) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int column = (int)divide((uint32_t)(t0 + 16 * h), a.block);
+        p.block[h] = as_constant<int32_t>(table)[column < last_column ? column : last_column]; // a half behind the end reads rows of the last page
+      }
+    } else {
+      int t = t0 + (lane & 31);
+      t = t < span.lo ? span.lo : t >= span.end ? span.end - 1 : t;
+      p.block[0] = table[divide((uint32_t)t, a.block)];
+      p.block[1] = 0;
+    }
+    return p;
+  }
+
+  __device__ __forceinline__ void load(Tile& x, int t0, const Pages& pages) const {
+    typedef __attribute__((ext_vector_type(KREGS))) uint32_t key_t;
+    typedef __attribute__((ext_vector_type(VREGS))) uint32_t value_t;
+    typedef key_t __attribute__((aligned(ROWS8 ? 4 : 16))) stored_key; // 8-bit rows begin on 4 bytes
+    typedef value_t __attribute__((aligned(ROWS8 ? 4 : 2 * VC))) stored_value;
+    x.partial = t0 < span.lo || t0 + ATT_TILE > span.end;
+    x.seen = 0xff;
+    const auto key = [&](int h, int i, const char* p) {
+      const key_t w = *reinterpret_cast<const stored_key*>(p);
+#pragma unroll
+      for (int r = 0; r < KREGS; ++r) x.k[h][i][r] = w[r];
+    };
+    const auto value = [&](int h, int j, const char* p) {
+      const value_t w = *reinterpret_cast<const stored_value*>(p);
+#pragma unroll
+      for (int r = 0; r < VREGS; ++r) x.v[h][j][r] = w[r];
+    };
+    if constexpr (PAGE16) {
+      // addresses are the page's, the same for the wave, and 32 bits that do not change from tile to tile
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int t = t0 + 16 * h;
+        const int in_block = t - (int)divide((uint32_t)t, a.block) * a.block_size;
+        int block = pages.block[h];
+        if ((uint32_t)block >= (uint32_t)a.blocks) {
+          block = 0;
+          x.partial = true;
+          x.seen &= h ? 0x0f : 0xf0;
+        }
+        const auto kb = rows_at(key_base + (block * a.key.block_stride + in_block * a.key.slot_stride));
+        const auto vb = rows_at(value_base + (block * a.value.block_stride + in_block * a.value.slot_stride));
+        const uint32_t ks = (uint32_t)a.key.slot_stride, vs = (uint32_t)a.value.slot_stride;
+#pragma unroll
+        for (int i = 0; i < KP; ++i) fetch<KREGS>(x.k[h][i], kb, key_rows + (FULL ? 0 : key_piece(i)), 0, FULL ? 32 * i * EL : 0);
+        if (ROWS8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x.k_pair[4 * h + j] = __builtin_amdgcn_raw_buffer_load_b32(kb, 4 * g * ks, j * ks, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int c = 0; c < HALVES; ++c) fetch<VREGS>(x.v[c][4 * h + j], vb, value_rows + (FULL ? 0 : value_piece(c)), j * vs, FULL ? 128 * c * EL : 0);
+          if (ROWS8) x.v_pair[4 * h + j] = __builtin_amdgcn_raw_buffer_load_b32(vb, 4 * g * vs, j * vs, 0);
+        }
+      }
+    } else {
+      // lane i finds where the row of token i is, and lanes fetch it from there
+      int t = t0 + (lane & 31);
+      t = t < span.lo ? span.lo : t >= span.end ? span.end - 1 : t;
+      const int in_block = t - (int)divide((uint32_t)t, a.block) * a.block_size;
+      int block = pages.block[0];
+      const bool bad = (uint32_t)block >= (uint32_t)a.blocks;
+      if (bad) block = 0;
+      const uint32_t bads = (uint32_t)__builtin_amdgcn_ballot_w64(bad);
+      if (bads) x.partial = true;
+      const uint64_t kt = (uint64_t)(key_base + (block * a.key.block_stride + in_block * a.key.slot_stride));
+      const uint64_t vt = (uint64_t)(value_base + (block * a.value.block_stride + in_block * a.value.slot_stride));
+      const auto row = [&](uint64_t v, int src) {
+        return reinterpret_cast<const char*>((uint64_t)__shfl((uint32_t)v, src, 64) | ((uint64_t)__shfl((uint32_t)(v >> 32), src, 64) << 32));
+      };
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const char* p = row(kt, 16 * h + n) + key_lane;
+#pragma unroll
+        for (int i = 0; i < KP; ++i) key(h, i, p + (int32_t)key_piece(i));
+      }
+      if (ROWS8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x.k_pair[j] = *reinterpret_cast<const uint32_t*>(row(kt, token_of(j)));
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const char* p = row(vt, token_of(j));
+        if ((bads >> token_of(j)) & 1) x.seen &= ~(1u << j);
+#pragma unroll
+        for (int c = 0; c < HALVES; ++c) value(c, j, p + value_lane + value_piece(c));
+        if (ROWS8) x.v_pair[j] = *reinterpret_cast<const uint32_t*>(p);
+      }
+    }
+    if (x.partial) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int t = t0 + token_of(j);
+        if (t < span.lo || t >= span.end) x.seen &= ~(1u << j);
+      }
+    }
+  }
+
+  // the running sums of 16 queries: query n is this lane's
+  uint4 q[KP];
+  float q_sum;
+  f32x4 acc[HALVES][VC];
+  float m, l, bias;
+
+  __device__ __forceinline__ void begin(int32_t request, int head, int q0, int rows) {
+    q_sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < KP; ++c) {
       q[c] = make_uint4(0, 0, 0, 0);
@@ -237,269 +364,240 @@ __global__ __launch_bounds__(64 * ATT_WAVES, DP > 128 ? 1 : 2) void paged_attent
       q_sum += __shfl_xor(q_sum, 16, 64);
       q_sum += __shfl_xor(q_sum, 32, 64);
     }
-    f32x4 acc[HALVES][VC];
 #pragma unroll
     for (int h = 0; h < HALVES; ++h)
 #pragma unroll
       for (int i = 0; i < VC; ++i) acc[h][i] = f32x4{0, 0, 0, 0};
-    float m = -__builtin_inff(), l = 0.0f, bias = 0.0f;
+    m = -__builtin_inff();
+    l = bias = 0.0f;
+  }
 
-    const char* key_base = a.key.base + head * a.key.head_stride;
-    const char* value_base = a.value.base + head * a.value.head_stride;
-    const int32_t* table = a.tables + request * a.table_stride;
-    const int last_column = span.end > 0 ? (int)divide((uint32_t)(span.end - 1), a.block) : 0;
-
-    for (int c = c0; c < c1; ++c) {
-      const int t0 = span.base + c * ATT_CHUNK + wave * ATT_TILE;
-      if (t0 >= span.end) continue;
-      bool partial = t0 < span.lo || t0 + ATT_TILE > span.end;
-      // ---- addresses: of keys, tokens n and 16 + n; of values, tokens 4g .. 4g+3 and 16+4g .. ----
-      const char *kp[2], *vp[8];
-      uint32_t seen = 0xff; // of this lane's 8 tokens
-      if (PAGE16) {
+  __device__ __forceinline__ void add(Tile& x) {
+    // ---- scores ----
+    float s[8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int t = t0 + 16 * h;
-          int column = (int)divide((uint32_t)t, a.block);
-          const int in_block = t - column * a.block_size;
-          column = column < last_column ? column : last_column; // a tile behind the end reads rows of the last page
-          int block = table[column];
-          if ((uint32_t)block >= (uint32_t)a.blocks) {
-            block = 0;
-            partial = true;
-            seen &= h ? 0x0f : 0xf0;
-          }
-          const char* kt = key_base + block * a.key.block_stride + in_block * a.key.slot_stride;
-          const char* vt = value_base + block * a.value.block_stride + in_block * a.value.slot_stride;
-          kp[h] = kt + n * a.key.slot_stride;
+    for (int h = 0; h < 2; ++h) {
+      f32x4 r = {0, 0, 0, 0};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) vp[4 * h + j] = vt + (4 * g + j) * a.value.slot_stride;
-        }
-      } else {
-        // lane i (and i + 32) finds token i's page
-        int t = t0 + (lane & 31);
-        t = t < span.lo ? span.lo : t >= span.end ? span.end - 1 : t;
-        const int column = (int)divide((uint32_t)t, a.block);
-        const int in_block = t - column * a.block_size;
-        int block = table[column];
-        const bool bad = (uint32_t)block >= (uint32_t)a.blocks;
-        if (bad) block = 0;
-        const uint32_t bads = (uint32_t)__builtin_amdgcn_ballot_w64(bad);
-        if (bads) partial = true;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int src = 16 * h + n;
-          kp[h] = key_base + (int64_t)__shfl(block, src, 64) * a.key.block_stride + (int64_t)__shfl(in_block, src, 64) * a.key.slot_stride;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int sv = 16 * h + 4 * g + j;
-            vp[4 * h + j] = value_base + (int64_t)__shfl(block, sv, 64) * a.value.block_stride + (int64_t)__shfl(in_block, sv, 64) * a.value.slot_stride;
-            if ((bads >> sv) & 1) seen &= ~(1u << (4 * h + j));
-          }
-        }
+      for (int i = 0; i < KP; ++i) {
+        const auto& k = x.k[h][i];
+        if constexpr (ROWS8) r = product<BF16>(widen<BF16>(k[0], k[1]), q[i], r);
+        else r = product<BF16>(make_uint4(k[0], k[1], k[2], k[3]), q[i], r);
       }
-      if (partial) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int t = t0 + (j >> 2) * 16 + 4 * g + (j & 3);
-          if (t < span.lo || t >= span.end) seen &= ~(1u << j);
-        }
+      for (int j = 0; j < 4; ++j) {
+        float y = r[j];
+        if (ROWS8) y = __builtin_fmaf(half_at(x.k_pair[4 * h + j], 0), y, half_at(x.k_pair[4 * h + j], 1) * q_sum);
+        s[4 * h + j] = y * a.scale;
       }
-      // ---- loads ----
-      uint4 k[2][KP];
+    }
+    if (a.softcap > 0.0f) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < KP; ++i) {
-          const int d = 32 * i + 8 * g;
-          k[h][i] = make_uint4(0, 0, 0, 0);
-          if (d < a.dim) {
-            if (ROWS8) {
-              const uint32_t* p = reinterpret_cast<const uint32_t*>(kp[h] + HEAD + d);
-              k[h][i] = make_uint4(p[0], p[1], 0, 0);
-            } else {
-              k[h][i] = *reinterpret_cast<const uint4*>(kp[h] + d * 2);
-            }
-          }
-        }
-      uint32_t v[HALVES][8][VREGS];
-#pragma unroll
-      for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int d = h * 128 + n * VC;
-#pragma unroll
-          for (int r = 0; r < VREGS; ++r) v[h][j][r] = 0;
-          if (d < a.dim) {
-            typedef __attribute__((ext_vector_type(VREGS))) uint32_t piece_t;
-            typedef piece_t __attribute__((aligned(4))) loose_t; // 8-bit rows begin on 4 bytes
-            const piece_t w = ROWS8 ? *reinterpret_cast<const loose_t*>(vp[j] + HEAD + d * EL) : *reinterpret_cast<const piece_t*>(vp[j] + d * EL);
-#pragma unroll
-            for (int r = 0; r < VREGS; ++r) v[h][j][r] = w[r];
-          }
-        }
-      uint32_t k_pair[8], v_pair[8];
-      if (ROWS8) {
-        const char* kt[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (PAGE16) kt[h] = kp[h] + (4 * g - n) * a.key.slot_stride;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (PAGE16) {
-              k_pair[4 * h + j] = *reinterpret_cast<const uint32_t*>(kt[h] + j * a.key.slot_stride);
-            } else { // lane 4g + j holds the row of token 4g + j
-              const uint64_t at = reinterpret_cast<uint64_t>(kp[h]);
-              const uint32_t lo = __shfl((uint32_t)at, 4 * g + j, 64), hi = __shfl((uint32_t)(at >> 32), 4 * g + j, 64);
-              k_pair[4 * h + j] = *reinterpret_cast<const uint32_t*>(((uint64_t)hi << 32) | lo);
-            }
-            v_pair[4 * h + j] = *reinterpret_cast<const uint32_t*>(vp[4 * h + j]);
-          }
-        }
-      }
-      // ---- scores ----
-      float s[8];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        f32x4 r = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < KP; ++i) r = product<BF16>(ROWS8 ? widen<BF16>(k[h][i].x, k[h][i].y) : k[h][i], q[i], r);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float x = r[j];
-          if (ROWS8) x = __builtin_fmaf(half_at(k_pair[4 * h + j], 0), x, half_at(k_pair[4 * h + j], 1) * q_sum);
-          x *= a.scale;
-          if (a.softcap > 0.0f) x = a.softcap * ATT_LOG2E * tanhf(x);
-          s[4 * h + j] = x;
-        }
-      }
-      if (partial) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (!((seen >> j) & 1)) {
-            s[j] = -__builtin_inff();
-            if (!ROWS8) { // what a row without a token holds may be anything: its weight of 0 would not hide it
-#pragma unroll
-              for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-                for (int r = 0; r < VREGS; ++r) v[h][j][r] = 0;
-            }
-          }
-        }
-      }
-      // ---- running maximum and sum ----
-      float most = s[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) most = __builtin_fmaxf(most, s[j]);
-      most = __builtin_fmaxf(most, __shfl_xor(most, 16, 64));
-      most = __builtin_fmaxf(most, __shfl_xor(most, 32, 64));
-      if (__builtin_amdgcn_ballot_w64(most > m)) {
-        const float now = __builtin_fmaxf(m, most);
-        const float f = m == now ? 1.0f : exp2_fast(m - now); // m = -inf: 0
-        m = now;
-        l *= f;
-        bias *= f;
-#pragma unroll
-        for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-          for (int i = 0; i < VC; ++i) acc[h][i] *= f;
-      }
-      const float ref = m == -__builtin_inff() ? 0.0f : m - SHIFT; // nothing seen yet: all weights 0
-      float p[8];
+      for (int j = 0; j < 8; ++j) s[j] = a.softcap * ATT_LOG2E * tanhf(s[j]);
+    }
+    if (x.partial) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        p[j] = exp2_fast(s[j] - ref);
-        l += p[j];
-      }
-      if (ROWS8) {
+        const uint32_t keep = (uint32_t)((int32_t)(x.seen << (31 - j)) >> 31); // all bits or none
+        s[j] = keep ? s[j] : -__builtin_inff();
+        // what a row without a token holds may be anything: its weight of 0 would not hide it
+        if (ROWS8) {
+          x.v_pair[j] &= keep;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool live = !partial || ((seen >> j) & 1);
-          bias += live ? p[j] * half_at(v_pair[j], 1) : 0.0f;
-          p[j] = live ? p[j] * half_at(v_pair[j], 0) : 0.0f;
+          for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (int r = 0; r < VREGS; ++r) x.v[h][j][r] &= keep;
         }
       }
-      uint4 hi, lo;
-      split<PBF16>(p, hi, lo);
-      // ---- values ----
+    }
+    // ---- running maximum and sum ----
+    float most = s[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) most = __builtin_fmaxf(most, s[j]);
+    most = group_max(most);
+    if (__builtin_amdgcn_ballot_w64(most > m)) {
+      const float now = __builtin_fmaxf(m, most);
+      const float f = m == now ? 1.0f : exp2_fast(m - now); // m = -inf: 0
+      m = now;
+      l *= f;
+      bias *= f;
 #pragma unroll
       for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-        for (int i = 0; i < VC; ++i) {
-          uint32_t t[4]; // column i of tokens 2 j, 2 j + 1
+        for (int i = 0; i < VC; ++i) acc[h][i] *= f;
+    }
+    const float ref = m == -__builtin_inff() ? 0.0f : m - SHIFT; // nothing seen yet: all weights 0
+    float p[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (ROWS8) {
-              const float x = (float)((v[h][2 * j][i / 4] >> (i % 4 * 8)) & 0xffu), y = (float)((v[h][2 * j + 1][i / 4] >> (i % 4 * 8)) & 0xffu);
-              t[j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u);
-            } else {
-              t[j] = __builtin_amdgcn_perm(v[h][2 * j + 1][i / 2], v[h][2 * j][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
-            }
-          }
-          const uint4 col = make_uint4(t[0], t[1], t[2], t[3]);
-          acc[h][i] = product<PBF16>(col, hi, acc[h][i]);
-          acc[h][i] = product<PBF16>(col, lo, acc[h][i]);
-        }
+    for (int j = 0; j < 8; ++j) {
+      p[j] = exp2_fast(s[j] - ref);
+      l += p[j];
     }
-
-    // ---- the four waves' sums, joined ----
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
     if (ROWS8) {
-      bias += __shfl_xor(bias, 16, 64);
-      bias += __shfl_xor(bias, 32, 64);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        bias = __builtin_fmaf(p[j], half_at(x.v_pair[j], 1), bias);
+        p[j] *= half_at(x.v_pair[j], 0);
+      }
     }
-    if (g == 0) {
-      s_ml[wave][n][0] = m;
-      s_ml[wave][n][1] = l;
-    }
+    uint4 hi, lo;
+    split<PBF16>(p, hi, lo);
+    // ---- values ----
 #pragma unroll
     for (int h = 0; h < HALVES; ++h)
 #pragma unroll
+      for (int i = 0; i < VC; ++i) {
+        uint32_t t[4]; // column i of tokens 2 j, 2 j + 1
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (ROWS8) {
+            const float y0 = (float)((x.v[h][2 * j][i / 4] >> (i % 4 * 8)) & 0xffu), y1 = (float)((x.v[h][2 * j + 1][i / 4] >> (i % 4 * 8)) & 0xffu);
+            t[j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y1), __builtin_bit_cast(uint32_t, y0), 0x07060302u);
+          } else {
+            t[j] = __builtin_amdgcn_perm(x.v[h][2 * j + 1][i / 2], x.v[h][2 * j][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+          }
+        }
+        const uint4 col = make_uint4(t[0], t[1], t[2], t[3]);
+        acc[h][i] = product<PBF16>(col, hi, acc[h][i]);
+        acc[h][i] = product<PBF16>(col, lo, acc[h][i]);
+      }
+  }
+
+  // tiles t0, t0 + CHUNK, ... below `end`: the next tile's rows are on their way while one is added, and the pages of the one
+  // behind it are being looked up
+  __device__ __forceinline__ void run(int t0, int end) {
+    if (t0 >= end) return;
+    Tile x, y;
+    // Behind the last tile it is loaded again, out of the caches: with a branch around the loads the compiler would wait for
+    // the rows of both tiles where the two ways meet, and the loads ahead would be none
+    const int last = t0 + (end - 1 - t0) / ATT_CHUNK * ATT_CHUNK;
+    const auto clamped = [&](int t) { return t < last ? t : last; };
+    load(x, t0, pages(t0));
+    Pages p = pages(clamped(t0 + ATT_CHUNK));
+    for (int t = t0;;) {
+      Pages after = pages(clamped(t + 2 * ATT_CHUNK)); // in front of the rows' loads: waiting for it is not waiting for them
+      load(y, clamped(t + ATT_CHUNK), p);
+      add(x);
+      t += ATT_CHUNK;
+      if (t > last) return;
+      p = pages(clamped(t + 2 * ATT_CHUNK));
+      load(x, clamped(t + ATT_CHUNK), after);
+      add(y);
+      t += ATT_CHUNK;
+      if (t > last) return;
+    }
+  }
+};
+
+template <bool BF16, bool ROWS8, int DP, bool FULL, bool PAGE16>
+__global__ __launch_bounds__(64 * ATT_WAVES, DP > 128 ? 1 : 2) void paged_attention_kernel(const AttentionArgs a) {
+  using A = Attention<BF16, ROWS8, DP, FULL, PAGE16>;
+  __shared__ float s_acc[ATT_WAVES][ATTENTION_ROWS][DP + 4];
+  __shared__ float s_ml[ATT_WAVES][ATTENTION_ROWS][2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t worker = blockIdx.x;
+
+  // ---- the worker's units (every wave finds them by itself: lengths come out of L2) ----
+  const uint32_t sets = (uint32_t)(a.kv_heads * a.q_tiles);
+  uint32_t total = 0;
+  for (int32_t b = lane; b < a.requests; b += 64) total += (uint32_t)span_of(a, b).units;
+  total = __builtin_amdgcn_readlane(inclusive_sum(total, lane), 63);
+  const uint32_t U = total * sets;
+  const uint32_t W = U < (uint32_t)a.workers ? U : (uint32_t)a.workers; // each has a unit at least
+  if (tid == 0) a.joins[worker] = make_int4(-1, 0, 0, 0);
+  if (worker >= W) return;
+  const Shares shares(U, W);
+  uint32_t unit = shares.begin(worker);
+  const uint32_t unit_end = shares.begin(worker + 1);
+  // the request that holds the first one: the first whose inclusive sum is above unit / sets
+  int32_t request = 0;
+  uint32_t before = 0; // units (without sets) of the requests before it
+  for (const uint32_t want = unit / sets;; request += 64) {
+    const uint32_t sum = inclusive_sum(request + lane < a.requests ? (uint32_t)span_of(a, request + lane).units : 0u, lane);
+    const uint64_t above = __builtin_amdgcn_ballot_w64(before + sum > want);
+    if (above) {
+      const int i = __builtin_ctzll(above);
+      if (i > 0) before += __builtin_amdgcn_readlane(sum, i - 1);
+      request += i;
+      break;
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+  }
+
+  A x(a, lane);
+  // ---- segment after segment: units of one (request, key head, tile of queries) ----
+  while (unit < unit_end) {
+    x.span = span_of(a, request);
+    const uint32_t in_request = unit - before * sets, units = (uint32_t)x.span.units;
+    const uint32_t set = in_request / units, c0 = in_request - set * units;
+    const uint32_t c1 = unit_end - unit < units - c0 ? c0 + (unit_end - unit) : units;
+    const int head = (int)(set / (uint32_t)a.q_tiles), q0 = ((int)set - head * a.q_tiles) * ATTENTION_ROWS;
+    const int rows = a.group - q0 < ATTENTION_ROWS ? a.group - q0 : ATTENTION_ROWS;
+    x.key_base = a.key.base + head * a.key.head_stride;
+    x.value_base = a.value.base + head * a.value.head_stride;
+    x.table = a.tables + request * a.table_stride;
+    x.last_column = x.span.end > 0 ? (int)divide((uint32_t)(x.span.end - 1), a.block) : 0;
+    x.begin(request, head, q0, rows);
+    const int64_t stop = x.span.base + (int64_t)c1 * ATT_CHUNK;
+    x.run(x.span.base + (int)c0 * ATT_CHUNK + wave * ATT_TILE, stop < x.span.end ? (int)stop : x.span.end);
+
+    // ---- the four waves' sums, joined ----
+    const int n = x.n, g = x.g;
+    x.l += __shfl_xor(x.l, 16, 64);
+    x.l += __shfl_xor(x.l, 32, 64);
+    if (ROWS8) {
+      x.bias += __shfl_xor(x.bias, 16, 64);
+      x.bias += __shfl_xor(x.bias, 32, 64);
+    }
+    if (g == 0) {
+      s_ml[wave][n][0] = x.m;
+      s_ml[wave][n][1] = x.l;
+    }
+#pragma unroll
+    for (int h = 0; h < A::HALVES; ++h)
+#pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < VC; ++i) s_acc[wave][n][h * 128 + (4 * g + r) * VC + i] = acc[h][i][r] + bias;
+        for (int i = 0; i < A::VC; ++i) s_acc[wave][n][h * 128 + (4 * g + r) * A::VC + i] = x.acc[h][i][r] + x.bias;
     __syncthreads();
-    const bool whole = c0 == 0 && c1 == span.units;
+    const bool whole = c0 == 0 && c1 == units;
     const int slot = c0 == 0 ? 1 : 0;
     for (int i = tid; i < rows * DP; i += 64 * ATT_WAVES) {
       const int row = i / DP, d = i - row * DP;
       float M = s_ml[0][row][0];
 #pragma unroll
       for (int w = 1; w < ATT_WAVES; ++w) M = __builtin_fmaxf(M, s_ml[w][row][0]);
-      float L = 0.0f, x = 0.0f;
+      float L = 0.0f, y = 0.0f;
 #pragma unroll
       for (int w = 0; w < ATT_WAVES; ++w) {
         const float mw = s_ml[w][row][0];
         const float f = mw == -__builtin_inff() ? 0.0f : exp2_fast(mw - M);
         L += f * s_ml[w][row][1];
-        x += f * s_acc[w][row][d];
+        y += f * s_acc[w][row][d];
       }
       if (d >= a.dim) continue;
       const int64_t at = request * (int64_t)(a.kv_heads * a.group) + head * a.group + q0 + row;
       if (whole) {
-        const float y = L == 0.0f ? 0.0f : x / L;
-        char* o = a.out + (at * a.dim + d) * 2;
-        *reinterpret_cast<uint16_t*>(o) = (uint16_t)pack16<BF16>(y, y);
-        if (d == 0) a.lse[at] = L == 0.0f ? -__builtin_inff() : (M - SHIFT + __builtin_amdgcn_logf(L)) * (1.0f / ATT_LOG2E);
+        y = L == 0.0f ? 0.0f : y / L;
+        *reinterpret_cast<uint16_t*>(a.out + (at * a.dim + d) * 2) = (uint16_t)pack16<BF16>(y, y);
+        if (d == 0) a.lse[at] = L == 0.0f ? -__builtin_inff() : (M - A::SHIFT + __builtin_amdgcn_logf(L)) * (1.0f / ATT_LOG2E);
       } else {
         const int64_t part = ((int64_t)worker * 2 + slot) * ATTENTION_ROWS + row;
-        a.partial[part * a.dim + d] = x;
+        a.partial[part * a.dim + d] = y;
         if (d == 0) {
           a.partial_ml[part * 2] = M;
           a.partial_ml[part * 2 + 1] = L;
         }
       }
     }
-    if (c0 == 0 && c1 < span.units && tid == 0) {
-      // the pair goes on with the next workers; its last unit's is the last worker whose first unit is not behind it
-      const int64_t last = unit + span.units - 1;
-      a.joins[worker] = make_int4((int)request, set, (int)(((last + 1) * W + U - 1) / U - 1), 0);
-    }
+    // the pair goes on with the next workers, up to the one that has its last unit
+    if (c0 == 0 && c1 < units && tid == 0) a.joins[worker] = make_int4(request, (int)set, (int)shares.worker_of(unit + units - 1), 0);
     __syncthreads();
     unit += c1 - c0;
-    if (c1 == span.units && set == (int)sets - 1) {
-      before += span.units;
+    if (c1 == units && set == sets - 1) {
+      before += units;
       ++request;
     }
   }
@@ -507,9 +605,9 @@ __global__ __launch_bounds__(64 * ATT_WAVES, DP > 128 ? 1 : 2) void paged_attent
 
 // One workgroup per (worker, query): where a pair of requests and heads begins with this worker and goes on
 // with others, its sums are added up in the workers' order.
-template <bool BF16>
+template <bool BF16, int COLUMNS>
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(const AttentionArgs a, const int rows_max, const float shift) {
-  __shared__ float s_acc[4][256];
+  __shared__ float s_acc[4][64 * COLUMNS];
   __shared__ float s_l[4];
   const int worker = blockIdx.x / rows_max, row = blockIdx.x - worker * rows_max;
   const int4 join = a.joins[worker];
@@ -523,18 +621,38 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const Attenti
   for (int i = lane; i < parts; i += 64) M = __builtin_fmaxf(M, a.partial_ml[place(i) * 2]);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) M = __builtin_fmaxf(M, __shfl_xor(M, d, 64));
-  float x[4] = {0, 0, 0, 0}, L = 0.0f;
-  for (int i = wave; i < parts; i += 4) {
-    const int64_t at = place(i);
-    const float mw = a.partial_ml[at * 2];
-    const float f = mw == -__builtin_inff() ? 0.0f : exp2_fast(mw - M);
-    L += f * a.partial_ml[at * 2 + 1];
+  // a wave takes every fourth part, 64 of these at a time: lane i has the weight of the i-th
+  float x[COLUMNS] = {}, L = 0.0f;
+  for (int i0 = wave; i0 < parts; i0 += 4 * 64) {
+    const int mine = i0 + 4 * lane;
+    float f = 0.0f, lf = 0.0f;
+    if (mine < parts) {
+      const float mw = a.partial_ml[place(mine) * 2];
+      f = mw == -__builtin_inff() ? 0.0f : exp2_fast(mw - M);
+      lf = f * a.partial_ml[place(mine) * 2 + 1];
+    }
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (lane + 64 * c < a.dim) x[c] += f * a.partial[at * a.dim + lane + 64 * c];
+    for (int d = 1; d < 64; d <<= 1) lf += __shfl_xor(lf, d, 64);
+    L += lf;
+    const int count = (parts - i0 + 3) / 4 < 64 ? (parts - i0 + 3) / 4 : 64;
+    for (int k0 = 0; k0 < count; k0 += 8) {
+      float v[8][COLUMNS];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + 4 * (k0 + k < count ? k0 + k : count - 1);
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c) v[k][c] = lane + 64 * c < a.dim ? a.partial[place(i) * a.dim + lane + 64 * c] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float fk = k0 + k < count ? __shfl(f, k0 + k, 64) : 0.0f;
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c) x[c] += fk * v[k][c];
+      }
+    }
   }
 #pragma unroll
-  for (int c = 0; c < 4; ++c) s_acc[wave][lane + 64 * c] = x[c];
+  for (int c = 0; c < COLUMNS; ++c) s_acc[wave][lane + 64 * c] = x[c];
   if (lane == 0) s_l[wave] = L;
   __syncthreads();
   const int d = threadIdx.x;
@@ -547,14 +665,20 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const Attenti
   if (d == 0) a.lse[at] = L == 0.0f ? -__builtin_inff() : (M - shift + __builtin_amdgcn_logf(L)) * (1.0f / ATT_LOG2E);
 }
 
+template <bool BF16, bool ROWS8, int DP, bool FULL>
+void launch_kernel(const AttentionArgs& a, hipStream_t stream) {
+  if (a.block_size % 16 == 0) paged_attention_kernel<BF16, ROWS8, DP, FULL, true><<<a.workers, 64 * ATT_WAVES, 0, stream>>>(a);
+  else paged_attention_kernel<BF16, ROWS8, DP, FULL, false><<<a.workers, 64 * ATT_WAVES, 0, stream>>>(a);
+}
+
 template <bool BF16, bool ROWS8, int DP>
 hipError_t launch_dp(const AttentionArgs& a, hipStream_t stream) {
-  if (a.block_size % 16 == 0) paged_attention_kernel<BF16, ROWS8, DP, true><<<a.workers, 64 * ATT_WAVES, 0, stream>>>(a);
-  else paged_attention_kernel<BF16, ROWS8, DP, false><<<a.workers, 64 * ATT_WAVES, 0, stream>>>(a);
+  if (a.dim == DP) launch_kernel<BF16, ROWS8, DP, true>(a, stream);
+  else launch_kernel<BF16, ROWS8, DP, false>(a, stream);
   if (hipError_t e = hipGetLastError()) return e;
   if (a.max_tokens <= ATT_CHUNK - 15) return hipSuccess; // every request is one unit
   const int rows = a.group < ATTENTION_ROWS ? a.group : ATTENTION_ROWS;
-  paged_attention_join_kernel<BF16><<<a.workers * rows, 256, 0, stream>>>(a, rows, ROWS8 || BF16 ? 0.0f : 14.0f);
+  paged_attention_join_kernel<BF16, DP / 64><<<a.workers * rows, 256, 0, stream>>>(a, rows, ROWS8 || BF16 ? 0.0f : 14.0f);
   return hipGetLastError();
 }
 

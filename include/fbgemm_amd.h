@@ -636,7 +636,8 @@ int fbgemm_amd_kv_cache_append(
  * is 0 and d_lse -inf. What the cache holds where no token is may be anything; a
  * token's key or value that is not finite makes its queries' outputs not finite. A
  * cache of FP16 / BF16 rows must have the queries' type and rows on 16-byte boundaries,
- * one of INT8 rows goes with either. dim: a multiple of 8, at most 256. Scores, weights
+ * one of INT8 rows goes with either. dim: a multiple of 8, at most 256;
+ * requests * heads * table_width * block_size below some 2^38. Scores, weights
  * and sums are fp32 (weights go to the matrix cores as two 16-bit numbers); results do
  * not depend on the order in which workgroups run. d_workspace: scratch of
  * fbgemm_amd_paged_attention_workspace bytes that no other call uses at the same time. */
