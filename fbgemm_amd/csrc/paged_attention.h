@@ -25,11 +25,13 @@
 // 8-bit rows (fp16 scale a_t and bias b_t in front): s_t = a_t (q . k8_t) + b_t sum(q), and weights
 // p_t a_t for the bytes, p_t b_t for the bias: 0 .. 255 are exact in bf16 and fp16.
 //
-// Work: units of CHUNK tokens of a (request, key head, 16 queries), numbered in that order; each
-// of W workers (at most U) takes U / W of them in a row, whatever requests they are of, so that all workers
-// end together however long the requests are. A worker's four waves take 32 tokens each in turn and
-// are joined in LDS; what a worker has whole it writes out, of what it shares with its neighbours (its
-// first and its last pair) it leaves the sums, which a second launch joins in order.
+// Work: steps of 128 tokens of a (request, key head, 16 queries), 32 for each of a worker's (workgroup's) four waves, numbered in
+// that order. Each of W workers takes a W-th of them in a row, whatever requests they are of, so that all end together
+// however long the requests are; a pair of request and head weighs one more than its steps, or a worker that meets
+// many short ones would be late. The waves' sums of a pair are joined in LDS. A pair that a worker has whole it writes
+// out; of one that it shares with its neighbours (its first and its last, at
+// most) it leaves the sums, and the last of eight workers to leave some adds theirs up in the workers' order, the last of
+// eight such groups these, and so on: one launch, few loads in a row, and results that depend on no order.
 #pragma once
 #include "decode.h"
 
@@ -37,8 +39,9 @@ namespace fbgemm_amd {
 
 constexpr int ATT_WAVES = 4;
 constexpr int ATT_TILE = 32; // tokens of a wave's step
-constexpr int ATT_CHUNK = ATT_WAVES * ATT_TILE;
-static_assert(ATT_CHUNK == ATTENTION_CHUNK, "");
+constexpr int ATT_STEP = ATT_WAVES * ATT_TILE; // of all waves'
+static_assert(ATT_STEP == ATTENTION_STEP, "");
+constexpr uint32_t ATT_JOIN = 8;               // workers whose sums are added up at once
 constexpr float ATT_LOG2E = 1.4426950408889634f;
 
 #if defined(__HIPCC__)
@@ -113,6 +116,11 @@ __device__ __forceinline__ uint4 widen(uint32_t a, uint32_t b) {
 
 __device__ __forceinline__ float half_at(uint32_t pair, int i) { return (float)__builtin_bit_cast(f16x2, pair)[i]; }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// (1 - t) / (1 + t), t = exp(-2 |x|): off by some 2^-23 of 1
+__device__ __forceinline__ float tanh_fast(float x) {
+  const float t = exp2_fast(-2.0f * ATT_LOG2E * __builtin_fabsf(x));
+  return __builtin_copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
+}
 
 // Tables and lengths are written by nobody while a kernel runs: where an address is the same for the
 // wave, the scalar unit reads them, apart from the rows' loads and what waits for these.
@@ -124,9 +132,10 @@ __device__ __forceinline__ constant<T> as_constant(const void* p) {
 }
 
 // A tile's rows as a buffer: its address sits in scalar registers, a lane adds 32 bits, a row the scalar offset. Every
-// load is inside the tile by the lanes' own offsets; the size is there to be given.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const char* p) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, 0x7fffffff, 0x00027000);
+// load is inside the tile by the lanes' own offsets; the size is there to be none, for a tile that is not there: its
+// loads touch no memory.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const char* p, bool any) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, any ? 0x7fffffff : 0, 0x00027000);
 }
 template <int N>
 __device__ __forceinline__ void fetch(uint32_t (&to)[N], __amdgpu_buffer_rsrc_t rows, uint32_t lane, uint32_t row, uint32_t piece) {
@@ -149,9 +158,9 @@ __device__ __forceinline__ float group_max(float x) {
   return __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
 }
 
-// A request's tokens that count, lo <= t < end, in units of CHUNK from `base` on
+// A request's tokens that count, lo <= t < end, in `steps` from `base` on
 struct Span {
-  int32_t base, lo, end, units;
+  int32_t base, lo, end, steps;
 };
 __device__ __forceinline__ Span span_of(const AttentionArgs& a, int32_t request) {
   int64_t len = a.idx64 ? as_constant<int64_t>(a.lengths)[request] : (int64_t)as_constant<int32_t>(a.lengths)[request];
@@ -160,8 +169,8 @@ __device__ __forceinline__ Span span_of(const AttentionArgs& a, int32_t request)
   s.end = (int32_t)len;
   s.lo = a.window > 0 && len > a.window ? (int32_t)(len - a.window) : 0;
   s.base = s.lo & ~15;
-  const int32_t n = (s.end - s.base + ATT_CHUNK - 1) / ATT_CHUNK;
-  s.units = n > 0 ? n : 1; // an empty one is somebody's too: its result is zeros
+  const int32_t n = (s.end - s.base + ATT_STEP - 1) / ATT_STEP;
+  s.steps = n > 0 ? n : 1; // an empty one is somebody's too: its result is zeros
   return s;
 }
 
@@ -220,7 +229,7 @@ struct Attention {
   const char *key_base, *value_base;
   const int32_t* table;
   Span span;
-  int last_column;
+  int first_column, last_column; // of the tokens that count
 
   __device__ __forceinline__ Attention(const AttentionArgs& args, int lane_) : a(args), lane(lane_), n(lane_ & 15), g(lane_ >> 4) {
     key_lane = HEAD + 8 * g * EL;
@@ -244,30 +253,30 @@ struct Attention {
         p.block[h] = as_constant<int32_t>(table)[column < last_column ? column : last_column]; // a half behind the end reads rows of the last page
       }
     } else {
-      int t = t0 + (lane & 31);
-      t = t < span.lo ? span.lo : t >= span.end ? span.end - 1 : t;
-      p.block[0] = table[divide((uint32_t)t, a.block)];
+      const int column = (int)divide((uint32_t)(t0 + (lane & 31)), a.block); // of a token that counts, or the nearest one that does
+      p.block[0] = table[column < first_column ? first_column : column > last_column ? last_column : column];
       p.block[1] = 0;
     }
     return p;
   }
 
-  __device__ __forceinline__ void load(Tile& x, int t0, const Pages& pages) const {
+  // `any`: false: PAGE16 loads nothing, else the tile as well (it is there)
+  __device__ __forceinline__ void load(Tile& tile, int t0, const Pages& pages, bool any) const {
     typedef __attribute__((ext_vector_type(KREGS))) uint32_t key_t;
     typedef __attribute__((ext_vector_type(VREGS))) uint32_t value_t;
     typedef key_t __attribute__((aligned(ROWS8 ? 4 : 16))) stored_key; // 8-bit rows begin on 4 bytes
     typedef value_t __attribute__((aligned(ROWS8 ? 4 : 2 * VC))) stored_value;
-    x.partial = t0 < span.lo || t0 + ATT_TILE > span.end;
-    x.seen = 0xff;
+    tile.partial = t0 < span.lo || t0 + ATT_TILE > span.end;
+    tile.seen = 0xff;
     const auto key = [&](int h, int i, const char* p) {
       const key_t w = *reinterpret_cast<const stored_key*>(p);
 #pragma unroll
-      for (int r = 0; r < KREGS; ++r) x.k[h][i][r] = w[r];
+      for (int r = 0; r < KREGS; ++r) tile.k[h][i][r] = w[r];
     };
     const auto value = [&](int h, int j, const char* p) {
       const value_t w = *reinterpret_cast<const stored_value*>(p);
 #pragma unroll
-      for (int r = 0; r < VREGS; ++r) x.v[h][j][r] = w[r];
+      for (int r = 0; r < VREGS; ++r) tile.v[h][j][r] = w[r];
     };
     if constexpr (PAGE16) {
       // addresses are the page's, the same for the wave, and 32 bits that do not change from tile to tile
@@ -278,64 +287,73 @@ struct Attention {
         int block = pages.block[h];
         if ((uint32_t)block >= (uint32_t)a.blocks) {
           block = 0;
-          x.partial = true;
-          x.seen &= h ? 0x0f : 0xf0;
+          tile.partial = true;
+          tile.seen &= h ? 0x0f : 0xf0;
         }
-        const auto kb = rows_at(key_base + (block * a.key.block_stride + in_block * a.key.slot_stride));
-        const auto vb = rows_at(value_base + (block * a.value.block_stride + in_block * a.value.slot_stride));
+        const auto kb = rows_at(key_base + (block * a.key.block_stride + in_block * a.key.slot_stride), any);
+        const auto vb = rows_at(value_base + (block * a.value.block_stride + in_block * a.value.slot_stride), any);
         const uint32_t ks = (uint32_t)a.key.slot_stride, vs = (uint32_t)a.value.slot_stride;
 #pragma unroll
-        for (int i = 0; i < KP; ++i) fetch<KREGS>(x.k[h][i], kb, key_rows + (FULL ? 0 : key_piece(i)), 0, FULL ? 32 * i * EL : 0);
+        for (int i = 0; i < KP; ++i) fetch<KREGS>(tile.k[h][i], kb, key_rows + (FULL ? 0 : key_piece(i)), 0, FULL ? 32 * i * EL : 0);
         if (ROWS8) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x.k_pair[4 * h + j] = __builtin_amdgcn_raw_buffer_load_b32(kb, 4 * g * ks, j * ks, 0);
+          for (int j = 0; j < 4; ++j) tile.k_pair[4 * h + j] = __builtin_amdgcn_raw_buffer_load_b32(kb, 4 * g * ks, j * ks, 0);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
-          for (int c = 0; c < HALVES; ++c) fetch<VREGS>(x.v[c][4 * h + j], vb, value_rows + (FULL ? 0 : value_piece(c)), j * vs, FULL ? 128 * c * EL : 0);
-          if (ROWS8) x.v_pair[4 * h + j] = __builtin_amdgcn_raw_buffer_load_b32(vb, 4 * g * vs, j * vs, 0);
+          for (int c = 0; c < HALVES; ++c) fetch<VREGS>(tile.v[c][4 * h + j], vb, value_rows + (FULL ? 0 : value_piece(c)), j * vs, FULL ? 128 * c * EL : 0);
+          if (ROWS8) tile.v_pair[4 * h + j] = __builtin_amdgcn_raw_buffer_load_b32(vb, 4 * g * vs, j * vs, 0);
         }
       }
     } else {
       // lane i finds where the row of token i is, and lanes fetch it from there
-      int t = t0 + (lane & 31);
-      t = t < span.lo ? span.lo : t >= span.end ? span.end - 1 : t;
+      const int t = t0 + (lane & 31);
       const int in_block = t - (int)divide((uint32_t)t, a.block) * a.block_size;
       int block = pages.block[0];
       const bool bad = (uint32_t)block >= (uint32_t)a.blocks;
       if (bad) block = 0;
       const uint32_t bads = (uint32_t)__builtin_amdgcn_ballot_w64(bad);
-      if (bads) x.partial = true;
+      if (bads) tile.partial = true;
       const uint64_t kt = (uint64_t)(key_base + (block * a.key.block_stride + in_block * a.key.slot_stride));
       const uint64_t vt = (uint64_t)(value_base + (block * a.value.block_stride + in_block * a.value.slot_stride));
       const auto row = [&](uint64_t v, int src) {
         return reinterpret_cast<const char*>((uint64_t)__shfl((uint32_t)v, src, 64) | ((uint64_t)__shfl((uint32_t)(v >> 32), src, 64) << 32));
       };
+      // lanes 16 h + n of either half of the wave have the rows of tokens 16 h + n
+      const auto low = __builtin_amdgcn_permlane16_swap((uint32_t)kt, (uint32_t)kt, false, false);
+      const auto high = __builtin_amdgcn_permlane16_swap((uint32_t)(kt >> 32), (uint32_t)(kt >> 32), false, false);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const char* p = row(kt, 16 * h + n) + key_lane;
+        const char* p = reinterpret_cast<const char*>((uint64_t)low[h] | ((uint64_t)high[h] << 32)) + key_lane;
 #pragma unroll
         for (int i = 0; i < KP; ++i) key(h, i, p + (int32_t)key_piece(i));
       }
-      if (ROWS8) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x.k_pair[j] = *reinterpret_cast<const uint32_t*>(row(kt, token_of(j)));
-      }
+      const bool fours = a.block_size % 4 == 0; // four tokens in a row share a page: the first one's row is enough
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const char* p = row(vt, token_of(j));
-        if ((bads >> token_of(j)) & 1) x.seen &= ~(1u << j);
+        const char *kr = nullptr, *vr;
+        if (fours) {
+          if (ROWS8) kr = row(kt, token_of(j & 4)) + (j & 3) * a.key.slot_stride;
+          vr = row(vt, token_of(j & 4)) + (j & 3) * a.value.slot_stride;
+        } else {
+          if (ROWS8) kr = row(kt, token_of(j));
+          vr = row(vt, token_of(j));
+        }
+        if ((bads >> token_of(j)) & 1) tile.seen &= ~(1u << j);
 #pragma unroll
-        for (int c = 0; c < HALVES; ++c) value(c, j, p + value_lane + value_piece(c));
-        if (ROWS8) x.v_pair[j] = *reinterpret_cast<const uint32_t*>(p);
+        for (int c = 0; c < HALVES; ++c) value(c, j, vr + value_lane + value_piece(c));
+        if (ROWS8) {
+          tile.k_pair[j] = *reinterpret_cast<const uint32_t*>(kr);
+          tile.v_pair[j] = *reinterpret_cast<const uint32_t*>(vr);
+        }
       }
     }
-    if (x.partial) {
+    if (tile.partial) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int t = t0 + token_of(j);
-        if (t < span.lo || t >= span.end) x.seen &= ~(1u << j);
+        if (t < span.lo || t >= span.end) tile.seen &= ~(1u << j);
       }
     }
   }
@@ -372,7 +390,7 @@ struct Attention {
     l = bias = 0.0f;
   }
 
-  __device__ __forceinline__ void add(Tile& x) {
+  __device__ __forceinline__ void add(Tile& tile) {
     // ---- scores ----
     float s[8];
 #pragma unroll
@@ -380,34 +398,34 @@ struct Attention {
       f32x4 r = {0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < KP; ++i) {
-        const auto& k = x.k[h][i];
+        const auto& k = tile.k[h][i];
         if constexpr (ROWS8) r = product<BF16>(widen<BF16>(k[0], k[1]), q[i], r);
         else r = product<BF16>(make_uint4(k[0], k[1], k[2], k[3]), q[i], r);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float y = r[j];
-        if (ROWS8) y = __builtin_fmaf(half_at(x.k_pair[4 * h + j], 0), y, half_at(x.k_pair[4 * h + j], 1) * q_sum);
+        if (ROWS8) y = __builtin_fmaf(half_at(tile.k_pair[4 * h + j], 0), y, half_at(tile.k_pair[4 * h + j], 1) * q_sum);
         s[4 * h + j] = y * a.scale;
       }
     }
     if (a.softcap > 0.0f) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = a.softcap * ATT_LOG2E * tanhf(s[j]);
+      for (int j = 0; j < 8; ++j) s[j] = a.softcap * ATT_LOG2E * tanh_fast(s[j]);
     }
-    if (x.partial) {
+    if (tile.partial) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t keep = (uint32_t)((int32_t)(x.seen << (31 - j)) >> 31); // all bits or none
+        const uint32_t keep = (uint32_t)((int32_t)(tile.seen << (31 - j)) >> 31); // all bits or none
         s[j] = keep ? s[j] : -__builtin_inff();
         // what a row without a token holds may be anything: its weight of 0 would not hide it
         if (ROWS8) {
-          x.v_pair[j] &= keep;
+          tile.v_pair[j] &= keep;
         } else {
 #pragma unroll
           for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-            for (int r = 0; r < VREGS; ++r) x.v[h][j][r] &= keep;
+            for (int r = 0; r < VREGS; ++r) tile.v[h][j][r] &= keep;
         }
       }
     }
@@ -437,8 +455,8 @@ struct Attention {
     if (ROWS8) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        bias = __builtin_fmaf(p[j], half_at(x.v_pair[j], 1), bias);
-        p[j] *= half_at(x.v_pair[j], 0);
+        bias = __builtin_fmaf(p[j], half_at(tile.v_pair[j], 1), bias);
+        p[j] *= half_at(tile.v_pair[j], 0);
       }
     }
     uint4 hi, lo;
@@ -452,10 +470,10 @@ struct Attention {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if constexpr (ROWS8) {
-            const float y0 = (float)((x.v[h][2 * j][i / 4] >> (i % 4 * 8)) & 0xffu), y1 = (float)((x.v[h][2 * j + 1][i / 4] >> (i % 4 * 8)) & 0xffu);
+            const float y0 = (float)((tile.v[h][2 * j][i / 4] >> (i % 4 * 8)) & 0xffu), y1 = (float)((tile.v[h][2 * j + 1][i / 4] >> (i % 4 * 8)) & 0xffu);
             t[j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y1), __builtin_bit_cast(uint32_t, y0), 0x07060302u);
           } else {
-            t[j] = __builtin_amdgcn_perm(x.v[h][2 * j + 1][i / 2], x.v[h][2 * j][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+            t[j] = __builtin_amdgcn_perm(tile.v[h][2 * j + 1][i / 2], tile.v[h][2 * j][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
           }
         }
         const uint4 col = make_uint4(t[0], t[1], t[2], t[3]);
@@ -464,49 +482,93 @@ struct Attention {
       }
   }
 
-  // tiles t0, t0 + CHUNK, ... below `end`: the next tile's rows are on their way while one is added, and the pages of the one
-  // behind it are being looked up
-  __device__ __forceinline__ void run(int t0, int end) {
-    if (t0 >= end) return;
-    Tile x, y;
-    // Behind the last tile it is loaded again, out of the caches: with a branch around the loads the compiler would wait for
-    // the rows of both tiles where the two ways meet, and the loads ahead would be none
-    const int last = t0 + (end - 1 - t0) / ATT_CHUNK * ATT_CHUNK;
+  // tiles first, first + STEP, ... up to last of the segment that is set up, if any
+  int first, last;
+  Tile x;
+
+  __device__ __forceinline__ void run_ahead() {
+    if (first <= last) load(x, first, pages(first), true);
+  }
+  // The next tile's rows are on their way while one is added, and the pages of the one behind it are being looked up. There is
+  // no branch around the loads: behind the last tile they load nothing (PAGE16) or that tile again, out of the caches. Where two
+  // ways met the compiler would wait for the rows of both tiles, and the loads ahead would be none
+  __device__ __forceinline__ void run() {
+    if (first > last) return;
+    Tile y;
     const auto clamped = [&](int t) { return t < last ? t : last; };
-    load(x, t0, pages(t0));
-    Pages p = pages(clamped(t0 + ATT_CHUNK));
-    for (int t = t0;;) {
-      Pages after = pages(clamped(t + 2 * ATT_CHUNK)); // in front of the rows' loads: waiting for it is not waiting for them
-      load(y, clamped(t + ATT_CHUNK), p);
+    Pages p = pages(clamped(first + ATT_STEP));
+    for (int t = first;;) {
+      Pages after = pages(clamped(t + 2 * ATT_STEP)); // in front of the rows' loads: waiting for it is not waiting for them
+      load(y, clamped(t + ATT_STEP), p, t < last);
       add(x);
-      t += ATT_CHUNK;
+      t += ATT_STEP;
       if (t > last) return;
-      p = pages(clamped(t + 2 * ATT_CHUNK));
-      load(x, clamped(t + ATT_CHUNK), after);
+      p = pages(clamped(t + 2 * ATT_STEP));
+      load(x, clamped(t + ATT_STEP), after, t < last);
       add(y);
-      t += ATT_CHUNK;
+      t += ATT_STEP;
       if (t > last) return;
     }
   }
 };
 
+// What workers leave for each other: words that are read and written where all of the device sees them (agent-scope atomics go
+// past the L2 caches, of which each die has its own), in order by the wait between the last of them and the arrival
+// that says so. Plain stores and loads would need fences that write back and empty whole caches: 768 workers
+// with one each took 300 us.
+__device__ __forceinline__ void leave(float* to, float a, float b) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(to), (uint64_t)__builtin_bit_cast(uint32_t, a) | ((uint64_t)__builtin_bit_cast(uint32_t, b) << 32),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void found(const float* from, float& a, float& b) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  a = __builtin_bit_cast(float, (uint32_t)v);
+  b = __builtin_bit_cast(float, (uint32_t)(v >> 32));
+}
+__device__ __forceinline__ void all_left() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Four columns of a row of sums, as they come
+struct Sums {
+  float m, l;
+  f32x4 y;
+  __device__ __forceinline__ void add(float om, float ol, f32x4 oy) {
+    const float now = __builtin_fmaxf(m, om);
+    const float f = m == -__builtin_inff() ? 0.0f : exp2_fast(m - now), of = om == -__builtin_inff() ? 0.0f : exp2_fast(om - now);
+    m = now;
+    l = l * f + ol * of;
+    y = y * f + oy * of;
+  }
+};
+
+template <bool BF16>
+__device__ __forceinline__ void write_out(const AttentionArgs& a, int64_t at, int d, const Sums& s, float shift) {
+  const float f = s.l == 0.0f ? 0.0f : 1.0f / s.l; // nothing seen
+  uint32_t* o = reinterpret_cast<uint32_t*>(a.out + (at * a.dim + d) * 2);
+  o[0] = pack16<BF16>(s.y[0] * f, s.y[1] * f);
+  o[1] = pack16<BF16>(s.y[2] * f, s.y[3] * f);
+  if (d == 0) a.lse[at] = s.l == 0.0f ? -__builtin_inff() : (s.m - shift + __builtin_amdgcn_logf(s.l)) * (1.0f / ATT_LOG2E);
+}
+
 template <bool BF16, bool ROWS8, int DP, bool FULL, bool PAGE16>
-__global__ __launch_bounds__(64 * ATT_WAVES, DP > 128 ? 1 : 2) void paged_attention_kernel(const AttentionArgs a) {
+__global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP)) void paged_attention_kernel(const AttentionArgs a) {
   using A = Attention<BF16, ROWS8, DP, FULL, PAGE16>;
-  __shared__ float s_acc[ATT_WAVES][ATTENTION_ROWS][DP + 4];
+  constexpr int THREADS = 64 * ATT_WAVES;
+  __shared__ __attribute__((aligned(16))) float s_acc[ATT_WAVES][ATTENTION_ROWS][DP + 4];
   __shared__ float s_ml[ATT_WAVES][ATTENTION_ROWS][2];
+  __shared__ uint32_t s_arrived;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t worker = blockIdx.x;
 
-  // ---- the worker's units (every wave finds them by itself: lengths come out of L2) ----
+  // ---- the worker's units: of a pair one for itself, then its steps (every wave finds them by itself: lengths come out of L2) ----
   const uint32_t sets = (uint32_t)(a.kv_heads * a.q_tiles);
+  const auto units_of = [&](int32_t b) { return b < a.requests ? (uint32_t)span_of(a, b).steps + 1 : 0u; };
+  const uint32_t sum_first = inclusive_sum(units_of(lane), lane); // of the first 64 requests: often all there are
   uint32_t total = 0;
-  for (int32_t b = lane; b < a.requests; b += 64) total += (uint32_t)span_of(a, b).units;
-  total = __builtin_amdgcn_readlane(inclusive_sum(total, lane), 63);
+  for (int32_t b = 64 + lane; b < a.requests; b += 64) total += units_of(b);
+  total = __builtin_amdgcn_readlane(sum_first, 63) + (a.requests > 64 ? __builtin_amdgcn_readlane(inclusive_sum(total, lane), 63) : 0u);
   const uint32_t U = total * sets;
   const uint32_t W = U < (uint32_t)a.workers ? U : (uint32_t)a.workers; // each has a unit at least
-  if (tid == 0) a.joins[worker] = make_int4(-1, 0, 0, 0);
   if (worker >= W) return;
   const Shares shares(U, W);
   uint32_t unit = shares.begin(worker);
@@ -514,8 +576,8 @@ __global__ __launch_bounds__(64 * ATT_WAVES, DP > 128 ? 1 : 2) void paged_attent
   // the request that holds the first one: the first whose inclusive sum is above unit / sets
   int32_t request = 0;
   uint32_t before = 0; // units (without sets) of the requests before it
-  for (const uint32_t want = unit / sets;; request += 64) {
-    const uint32_t sum = inclusive_sum(request + lane < a.requests ? (uint32_t)span_of(a, request + lane).units : 0u, lane);
+  const uint32_t want = unit / sets;
+  for (uint32_t sum = sum_first;; sum = inclusive_sum(units_of(request + lane), lane)) {
     const uint64_t above = __builtin_amdgcn_ballot_w64(before + sum > want);
     if (above) {
       const int i = __builtin_ctzll(above);
@@ -524,25 +586,51 @@ __global__ __launch_bounds__(64 * ATT_WAVES, DP > 128 ? 1 : 2) void paged_attent
       break;
     }
     before += __builtin_amdgcn_readlane(sum, 63);
+    request += 64;
   }
 
+  // ---- segment after segment: steps c0 .. c1 - 1 of one pair (request, key head with its tile of queries) ----
+  struct Segment {
+    int64_t row; // of the output: its first query
+    uint32_t c0, c1, steps, first; // first: the unit of the pair's first step
+    int rows;
+  };
   A x(a, lane);
-  // ---- segment after segment: units of one (request, key head, tile of queries) ----
-  while (unit < unit_end) {
+  const auto set_up = [&]() {
+    Segment s;
     x.span = span_of(a, request);
-    const uint32_t in_request = unit - before * sets, units = (uint32_t)x.span.units;
-    const uint32_t set = in_request / units, c0 = in_request - set * units;
-    const uint32_t c1 = unit_end - unit < units - c0 ? c0 + (unit_end - unit) : units;
+    const uint32_t units = (uint32_t)x.span.steps + 1, in_request = unit - before * sets;
+    const uint32_t set = in_request / units, u0 = in_request - set * units;
+    const uint32_t u1 = unit_end - unit < units - u0 ? u0 + (unit_end - unit) : units;
+    s.steps = (uint32_t)x.span.steps;
+    s.c0 = u0 > 0 ? u0 - 1 : 0;
+    s.c1 = u1 - 1; // none, where the pair's own unit is all that is left for this worker
+    s.first = unit - u0 + 1;
     const int head = (int)(set / (uint32_t)a.q_tiles), q0 = ((int)set - head * a.q_tiles) * ATTENTION_ROWS;
-    const int rows = a.group - q0 < ATTENTION_ROWS ? a.group - q0 : ATTENTION_ROWS;
+    s.rows = a.group - q0 < ATTENTION_ROWS ? a.group - q0 : ATTENTION_ROWS;
+    s.row = request * (int64_t)(a.kv_heads * a.group) + head * a.group + q0;
     x.key_base = a.key.base + head * a.key.head_stride;
     x.value_base = a.value.base + head * a.value.head_stride;
     x.table = a.tables + request * a.table_stride;
+    x.first_column = (int)divide((uint32_t)x.span.lo, a.block);
     x.last_column = x.span.end > 0 ? (int)divide((uint32_t)(x.span.end - 1), a.block) : 0;
-    x.begin(request, head, q0, rows);
-    const int64_t stop = x.span.base + (int64_t)c1 * ATT_CHUNK;
-    x.run(x.span.base + (int)c0 * ATT_CHUNK + wave * ATT_TILE, stop < x.span.end ? (int)stop : x.span.end);
-
+    // this wave's tiles: one of each step, as long as there are tokens
+    x.first = x.span.base + (int)s.c0 * ATT_STEP + wave * ATT_TILE;
+    x.last = x.first + (int)(s.c1 - s.c0 - 1) * ATT_STEP;
+    if (x.last >= x.span.end) x.last -= ATT_STEP;
+    x.run_ahead();
+    x.begin(request, head, q0, s.rows);
+    unit += u1 - u0;
+    if (u1 == units && set == sets - 1) {
+      before += units;
+      ++request;
+    }
+    return s;
+  };
+  while (unit < unit_end) {
+    const Segment s = set_up();
+    if (s.c1 == s.c0) return;
+    x.run();
     // ---- the four waves' sums, joined ----
     const int n = x.n, g = x.g;
     x.l += __shfl_xor(x.l, 16, 64);
@@ -561,108 +649,72 @@ __global__ __launch_bounds__(64 * ATT_WAVES, DP > 128 ? 1 : 2) void paged_attent
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int i = 0; i < A::VC; ++i) s_acc[wave][n][h * 128 + (4 * g + r) * A::VC + i] = x.acc[h][i][r] + x.bias;
+    const bool whole = s.c0 == 0 && s.c1 == s.steps;
     __syncthreads();
-    const bool whole = c0 == 0 && c1 == units;
-    const int slot = c0 == 0 ? 1 : 0;
-    for (int i = tid; i < rows * DP; i += 64 * ATT_WAVES) {
-      const int row = i / DP, d = i - row * DP;
-      float M = s_ml[0][row][0];
-#pragma unroll
-      for (int w = 1; w < ATT_WAVES; ++w) M = __builtin_fmaxf(M, s_ml[w][row][0]);
-      float L = 0.0f, y = 0.0f;
-#pragma unroll
-      for (int w = 0; w < ATT_WAVES; ++w) {
-        const float mw = s_ml[w][row][0];
-        const float f = mw == -__builtin_inff() ? 0.0f : exp2_fast(mw - M);
-        L += f * s_ml[w][row][1];
-        y += f * s_acc[w][row][d];
+    const auto each_four = [&](auto&& f) { // f(query, first of four columns)
+      for (int i = tid; i < s.rows * (DP / 4); i += THREADS) {
+        const int row = i / (DP / 4), d = 4 * (i - row * (DP / 4));
+        if (FULL || d < a.dim) f(row, d);
       }
-      if (d >= a.dim) continue;
-      const int64_t at = request * (int64_t)(a.kv_heads * a.group) + head * a.group + q0 + row;
-      if (whole) {
-        y = L == 0.0f ? 0.0f : y / L;
-        *reinterpret_cast<uint16_t*>(a.out + (at * a.dim + d) * 2) = (uint16_t)pack16<BF16>(y, y);
-        if (d == 0) a.lse[at] = L == 0.0f ? -__builtin_inff() : (M - A::SHIFT + __builtin_amdgcn_logf(L)) * (1.0f / ATT_LOG2E);
-      } else {
-        const int64_t part = ((int64_t)worker * 2 + slot) * ATTENTION_ROWS + row;
-        a.partial[part * a.dim + d] = y;
-        if (d == 0) {
-          a.partial_ml[part * 2] = M;
-          a.partial_ml[part * 2 + 1] = L;
+    };
+    // a worker's two places: the second for a pair that begins with it
+    const uint32_t first = s.c0 == 0 ? worker : shares.worker_of(s.first);
+    const auto place = [&](uint32_t w, int row) { return ((int64_t)w * 2 + (w == first ? 1 : 0)) * ATTENTION_ROWS + row; };
+    const auto leave_sum = [&](uint32_t w, int row, int d, const Sums& sum) {
+      const int64_t at = place(w, row);
+      leave(&a.partial[at * a.dim + d], sum.y[0], sum.y[1]);
+      leave(&a.partial[at * a.dim + d + 2], sum.y[2], sum.y[3]);
+      if (d == 0) leave(&a.partial_ml[at * 2], sum.m, sum.l);
+    };
+    each_four([&](int row, int d) {
+      Sums sum{-__builtin_inff(), 0.0f, {0, 0, 0, 0}};
+#pragma unroll
+      for (int w = 0; w < ATT_WAVES; ++w) sum.add(s_ml[w][row][0], s_ml[w][row][1], *reinterpret_cast<const f32x4*>(&s_acc[w][row][d]));
+      if (whole) write_out<BF16>(a, s.row + row, d, sum, A::SHIFT);
+      else leave_sum(worker, row, d, sum);
+    });
+    if (!whole) {
+      // ---- sums left by the workers first, first + 1, ...: `count` of them at a distance of `stride`, ours is number `at` ----
+      uint32_t count = shares.worker_of(s.first + s.steps - 1) - first + 1, at = worker - first, stride = 1;
+      for (uint32_t* counters = a.counters;; counters += ATTENTION_COUNTERS) {
+        const uint32_t group = at / ATT_JOIN, members = count - group * ATT_JOIN < ATT_JOIN ? count - group * ATT_JOIN : ATT_JOIN;
+        const uint32_t leader = first + group * ATT_JOIN * stride;
+        all_left();
+        __syncthreads();
+        if (tid == 0) {
+          s_arrived = __hip_atomic_fetch_add(&counters[leader], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          if (s_arrived == members - 1) __hip_atomic_store(&counters[leader], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
         }
+        __syncthreads();
+        if (s_arrived != members - 1) break;
+        const bool all = count <= ATT_JOIN;
+        each_four([&](int row, int d) {
+          float m[ATT_JOIN], l[ATT_JOIN];
+          f32x4 y[ATT_JOIN];
+#pragma unroll
+          for (uint32_t k = 0; k < ATT_JOIN; ++k) {
+            const int64_t p = place(leader + (k < members ? k : 0) * stride, row);
+            float y0, y1, y2, y3;
+            found(&a.partial_ml[p * 2], m[k], l[k]);
+            found(&a.partial[p * a.dim + d], y0, y1);
+            found(&a.partial[p * a.dim + d + 2], y2, y3);
+            y[k] = f32x4{y0, y1, y2, y3};
+          }
+          Sums sum{m[0], l[0], y[0]};
+#pragma unroll
+          for (uint32_t k = 1; k < ATT_JOIN; ++k)
+            if (k < members) sum.add(m[k], l[k], y[k]);
+          if (all) write_out<BF16>(a, s.row + row, d, sum, A::SHIFT);
+          else leave_sum(leader, row, d, sum); // in the leader's place: nobody else looks there before we arrive
+        });
+        if (all) break;
+        count = (count + ATT_JOIN - 1) / ATT_JOIN;
+        at = group;
+        stride *= ATT_JOIN;
       }
     }
-    // the pair goes on with the next workers, up to the one that has its last unit
-    if (c0 == 0 && c1 < units && tid == 0) a.joins[worker] = make_int4(request, (int)set, (int)shares.worker_of(unit + units - 1), 0);
     __syncthreads();
-    unit += c1 - c0;
-    if (c1 == units && set == sets - 1) {
-      before += units;
-      ++request;
-    }
   }
-}
-
-// One workgroup per (worker, query): where a pair of requests and heads begins with this worker and goes on
-// with others, its sums are added up in the workers' order.
-template <bool BF16, int COLUMNS>
-__global__ __launch_bounds__(256) void paged_attention_join_kernel(const AttentionArgs a, const int rows_max, const float shift) {
-  __shared__ float s_acc[4][64 * COLUMNS];
-  __shared__ float s_l[4];
-  const int worker = blockIdx.x / rows_max, row = blockIdx.x - worker * rows_max;
-  const int4 join = a.joins[worker];
-  if (join.x < 0) return;
-  const int head = join.y / a.q_tiles, q0 = (join.y - head * a.q_tiles) * ATTENTION_ROWS;
-  if (q0 + row >= a.group) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int parts = join.z - worker + 1; // this worker's second place, the others' first
-  const auto place = [&](int i) { return ((int64_t)(worker + i) * 2 + (i == 0 ? 1 : 0)) * ATTENTION_ROWS + row; };
-  float M = -__builtin_inff();
-  for (int i = lane; i < parts; i += 64) M = __builtin_fmaxf(M, a.partial_ml[place(i) * 2]);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) M = __builtin_fmaxf(M, __shfl_xor(M, d, 64));
-  // a wave takes every fourth part, 64 of these at a time: lane i has the weight of the i-th
-  float x[COLUMNS] = {}, L = 0.0f;
-  for (int i0 = wave; i0 < parts; i0 += 4 * 64) {
-    const int mine = i0 + 4 * lane;
-    float f = 0.0f, lf = 0.0f;
-    if (mine < parts) {
-      const float mw = a.partial_ml[place(mine) * 2];
-      f = mw == -__builtin_inff() ? 0.0f : exp2_fast(mw - M);
-      lf = f * a.partial_ml[place(mine) * 2 + 1];
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) lf += __shfl_xor(lf, d, 64);
-    L += lf;
-    const int count = (parts - i0 + 3) / 4 < 64 ? (parts - i0 + 3) / 4 : 64;
-    for (int k0 = 0; k0 < count; k0 += 8) {
-      float v[8][COLUMNS];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int i = i0 + 4 * (k0 + k < count ? k0 + k : count - 1);
-#pragma unroll
-        for (int c = 0; c < COLUMNS; ++c) v[k][c] = lane + 64 * c < a.dim ? a.partial[place(i) * a.dim + lane + 64 * c] : 0.0f;
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float fk = k0 + k < count ? __shfl(f, k0 + k, 64) : 0.0f;
-#pragma unroll
-        for (int c = 0; c < COLUMNS; ++c) x[c] += fk * v[k][c];
-      }
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < COLUMNS; ++c) s_acc[wave][lane + 64 * c] = x[c];
-  if (lane == 0) s_l[wave] = L;
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= a.dim) return;
-  L = s_l[0] + s_l[1] + s_l[2] + s_l[3];
-  const float y = s_acc[0][d] + s_acc[1][d] + s_acc[2][d] + s_acc[3][d];
-  const int64_t at = (int64_t)join.x * (a.kv_heads * a.group) + head * a.group + q0 + row;
-  const float r = L == 0.0f ? 0.0f : y / L;
-  *reinterpret_cast<uint16_t*>(a.out + (at * a.dim + d) * 2) = (uint16_t)pack16<BF16>(r, r);
-  if (d == 0) a.lse[at] = L == 0.0f ? -__builtin_inff() : (M - shift + __builtin_amdgcn_logf(L)) * (1.0f / ATT_LOG2E);
 }
 
 template <bool BF16, bool ROWS8, int DP, bool FULL>
@@ -675,10 +727,6 @@ template <bool BF16, bool ROWS8, int DP>
 hipError_t launch_dp(const AttentionArgs& a, hipStream_t stream) {
   if (a.dim == DP) launch_kernel<BF16, ROWS8, DP, true>(a, stream);
   else launch_kernel<BF16, ROWS8, DP, false>(a, stream);
-  if (hipError_t e = hipGetLastError()) return e;
-  if (a.max_tokens <= ATT_CHUNK - 15) return hipSuccess; // every request is one unit
-  const int rows = a.group < ATTENTION_ROWS ? a.group : ATTENTION_ROWS;
-  paged_attention_join_kernel<BF16, DP / 64><<<a.workers * rows, 256, 0, stream>>>(a, rows, ROWS8 || BF16 ? 0.0f : 14.0f);
   return hipGetLastError();
 }
 
