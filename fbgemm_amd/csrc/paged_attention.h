@@ -137,16 +137,20 @@ __device__ __forceinline__ constant<T> as_constant(const void* p) {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const char* p, bool any) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, any ? 0x7fffffff : 0, 0x00027000);
 }
-template <int N>
+// Rows of 16-bit numbers are read once, in whole lines, and marked so (non-temporal): 256 requests of 16 to 8 192 tokens,
+// 64 queries on 8 heads of 128, 738 -> 663 us. A line of 8-bit rows takes several loads, which then miss it (262 143 tokens
+// 110 -> 171 us), and the halves of a line that a key of 64 numbers is loaded in do, a little.
+constexpr int READ_ONCE = 2;
+template <int AUX, int N>
 __device__ __forceinline__ void fetch(uint32_t (&to)[N], __amdgpu_buffer_rsrc_t rows, uint32_t lane, uint32_t row, uint32_t piece) {
   if constexpr (N == 4) {
-    const auto w = __builtin_amdgcn_raw_buffer_load_b128(rows, lane + piece, row, 0);
+    const auto w = __builtin_amdgcn_raw_buffer_load_b128(rows, lane + piece, row, AUX);
     to[0] = w[0], to[1] = w[1], to[2] = w[2], to[3] = w[3];
   } else if constexpr (N == 2) {
-    const auto w = __builtin_amdgcn_raw_buffer_load_b64(rows, lane + piece, row, 0);
+    const auto w = __builtin_amdgcn_raw_buffer_load_b64(rows, lane + piece, row, AUX);
     to[0] = w[0], to[1] = w[1];
   } else {
-    to[0] = __builtin_amdgcn_raw_buffer_load_b32(rows, lane + piece, row, 0);
+    to[0] = __builtin_amdgcn_raw_buffer_load_b32(rows, lane + piece, row, AUX);
   }
 }
 
@@ -208,6 +212,8 @@ struct Attention {
   static constexpr float SHIFT = PBF16 ? 0.0f : 14.0f; // weights are 2^SHIFT times larger
   static constexpr int VREGS = ROWS8 ? (VC + 3) / 4 : VC / 2; // registers of a value piece
   static constexpr int KREGS = ROWS8 ? 2 : 4;          // registers of a key piece
+  static constexpr int DEPTH = 1;                      // tiles loaded ahead
+  static constexpr int KEY_AUX = ROWS8 || DP == 64 ? 0 : READ_ONCE, VALUE_AUX = ROWS8 ? 0 : READ_ONCE;
 
   // what a wave has loaded of 32 tokens
   struct Tile {
@@ -269,12 +275,14 @@ struct Attention {
     tile.partial = t0 < span.lo || t0 + ATT_TILE > span.end;
     tile.seen = 0xff;
     const auto key = [&](int h, int i, const char* p) {
-      const key_t w = *reinterpret_cast<const stored_key*>(p);
+      const auto* at = reinterpret_cast<const stored_key*>(p);
+      const key_t w = KEY_AUX ? __builtin_nontemporal_load(at) : *at;
 #pragma unroll
       for (int r = 0; r < KREGS; ++r) tile.k[h][i][r] = w[r];
     };
     const auto value = [&](int h, int j, const char* p) {
-      const value_t w = *reinterpret_cast<const stored_value*>(p);
+      const auto* at = reinterpret_cast<const stored_value*>(p);
+      const value_t w = VALUE_AUX ? __builtin_nontemporal_load(at) : *at;
 #pragma unroll
       for (int r = 0; r < VREGS; ++r) tile.v[h][j][r] = w[r];
     };
@@ -294,7 +302,7 @@ struct Attention {
         const auto vb = rows_at(value_base + (block * a.value.block_stride + in_block * a.value.slot_stride), any);
         const uint32_t ks = (uint32_t)a.key.slot_stride, vs = (uint32_t)a.value.slot_stride;
 #pragma unroll
-        for (int i = 0; i < KP; ++i) fetch<KREGS>(tile.k[h][i], kb, key_rows + (FULL ? 0 : key_piece(i)), 0, FULL ? 32 * i * EL : 0);
+        for (int i = 0; i < KP; ++i) fetch<KEY_AUX>(tile.k[h][i], kb, key_rows + (FULL ? 0 : key_piece(i)), 0, FULL ? 32 * i * EL : 0);
         if (ROWS8) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) tile.k_pair[4 * h + j] = __builtin_amdgcn_raw_buffer_load_b32(kb, 4 * g * ks, j * ks, 0);
@@ -302,7 +310,7 @@ struct Attention {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
-          for (int c = 0; c < HALVES; ++c) fetch<VREGS>(tile.v[c][4 * h + j], vb, value_rows + (FULL ? 0 : value_piece(c)), j * vs, FULL ? 128 * c * EL : 0);
+          for (int c = 0; c < HALVES; ++c) fetch<VALUE_AUX>(tile.v[c][4 * h + j], vb, value_rows + (FULL ? 0 : value_piece(c)), j * vs, FULL ? 128 * c * EL : 0);
           if (ROWS8) tile.v_pair[4 * h + j] = __builtin_amdgcn_raw_buffer_load_b32(vb, 4 * g * vs, j * vs, 0);
         }
       }
@@ -482,32 +490,33 @@ struct Attention {
       }
   }
 
-  // tiles first, first + STEP, ... up to last of the segment that is set up, if any
+  // Tiles first, first + STEP, ... up to last. The rows of the DEPTH next ones are on their way while one is added, and the pages of
+  // the one behind these are being looked up. There is no branch around the loads: behind the last tile they load nothing
+  // (PAGE16) or that tile again, out of the caches. Where two ways met the compiler would wait for the rows of all
+  // tiles, and the loads ahead would be none
   int first, last;
-  Tile x;
-
-  __device__ __forceinline__ void run_ahead() {
-    if (first <= last) load(x, first, pages(first), true);
-  }
-  // The next tile's rows are on their way while one is added, and the pages of the one behind it are being looked up. There is
-  // no branch around the loads: behind the last tile they load nothing (PAGE16) or that tile again, out of the caches. Where two
-  // ways met the compiler would wait for the rows of both tiles, and the loads ahead would be none
   __device__ __forceinline__ void run() {
     if (first > last) return;
-    Tile y;
+    Tile ring[DEPTH + 1];
     const auto clamped = [&](int t) { return t < last ? t : last; };
-    Pages p = pages(clamped(first + ATT_STEP));
+    Pages p = pages(first);
+#pragma unroll
+    for (int k = 0; k < DEPTH; ++k) {
+      const Pages after = pages(clamped(first + (k + 1) * ATT_STEP));
+      load(ring[k], clamped(first + k * ATT_STEP), p, first + k * ATT_STEP <= last);
+      p = after;
+    }
     for (int t = first;;) {
-      Pages after = pages(clamped(t + 2 * ATT_STEP)); // in front of the rows' loads: waiting for it is not waiting for them
-      load(y, clamped(t + ATT_STEP), p, t < last);
-      add(x);
-      t += ATT_STEP;
-      if (t > last) return;
-      p = pages(clamped(t + 2 * ATT_STEP));
-      load(x, clamped(t + ATT_STEP), after, t < last);
-      add(y);
-      t += ATT_STEP;
-      if (t > last) return;
+#pragma unroll
+      for (int k = 0; k <= DEPTH; ++k) {
+        const int ahead = t + DEPTH * ATT_STEP;
+        const Pages after = pages(clamped(ahead + ATT_STEP)); // in front of the rows' loads: waiting for it is not waiting for them
+        load(ring[(k + DEPTH) % (DEPTH + 1)], clamped(ahead), p, ahead <= last);
+        p = after;
+        add(ring[k]);
+        t += ATT_STEP;
+        if (t > last) return;
+      }
     }
   }
 };
@@ -618,7 +627,6 @@ __global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP)) void paged
     x.first = x.span.base + (int)s.c0 * ATT_STEP + wave * ATT_TILE;
     x.last = x.first + (int)(s.c1 - s.c0 - 1) * ATT_STEP;
     if (x.last >= x.span.end) x.last -= ATT_STEP;
-    x.run_ahead();
     x.begin(request, head, q0, s.rows);
     unit += u1 - u0;
     if (u1 == units && set == sets - 1) {
