@@ -59,7 +59,7 @@ struct AppendArgs {
   Status* status;
 };
 hipError_t launch_kv_append(const AppendArgs& a, int piece_bytes, hipStream_t stream);
-hipError_t launch_kv_append_rows8(const AppendArgs& a, int32_t input_ty, hipStream_t stream);
+hipError_t launch_kv_append_rows8(const AppendArgs& a, int32_t input_ty, bool aligned16, hipStream_t stream); // aligned16: input rows are
 
 struct AttentionArgs {
   const char* query; // [requests][heads][dim], 16 bits

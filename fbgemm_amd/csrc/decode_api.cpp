@@ -181,7 +181,9 @@ int fbgemm_amd_kv_cache_append(
   a.status = (Status*)d_status;
   if (rows8) {
     if ((uintptr_t)d_key_cache % 4 || (uintptr_t)d_value_cache % 4) return fail(FBGEMM_AMD_E_ARG, "8-bit rows begin on 4-byte boundaries");
-    HIP_TRY(launch_kv_append_rows8(a, input_ty, (hipStream_t)stream));
+    const bool aligned16 = (uintptr_t)d_key % 16 == 0 && (uintptr_t)d_value % 16 == 0 &&
+        divides(16, {a.token_stride[0], a.head_stride[0], a.token_stride[1], a.head_stride[1]});
+    HIP_TRY(launch_kv_append_rows8(a, input_ty, aligned16, (hipStream_t)stream));
     return 0;
   }
   // the largest piece that every row is made of and begins at
