@@ -550,3 +550,58 @@ def test_refusals(decode):
     torch.cuda.synchronize()
     with pytest.raises(NotImplementedError):  # no CPU path
         decode.paged_attention(*[cpu[n] for n in ("query", "kc", "vc", "tables", "lengths")])
+
+
+@pytest.mark.parametrize("rows8", [False, True])
+def test_attention_on_two_streams_at_once(decode, rows8):
+    """Calls whose pairs are shared by many workers, side by side: each stream joins its own."""
+    cases = [attention_case(decode, 20 + k, 64, 2, 1, 16, [30011, 5, 4099], torch.bfloat16, rows8) for k in range(2)]
+    want = [decode.paged_attention(q, *c, t, n) for q, c, _, t, n in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                q, c, _, t, n = cases[k]
+                got[k].append(decode.paged_attention(q, *c, t, n))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(a, b) for pair in got[k] for a, b in zip(pair, want[k]))
+
+
+def test_attention_in_many_captures(decode):
+    """More captures than the operator keeps counters of, replayed out of order, beside eager calls."""
+    q, c, _, t, n = attention_case(decode, 30, 64, 2, 1, 16, [9001, 70], torch.bfloat16)
+    want = decode.paged_attention(q, *c, t, n)
+    graphs = []
+    for _ in range(20):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = [decode.paged_attention(q, *c, t, n) for _ in range(2)]
+        graphs.append((graph, got))
+    for k in (3, 19, 0, 7, 3, 0):
+        eager = decode.paged_attention(q, *c, t, n)
+        graphs[k][0].replay()
+        torch.cuda.synchronize()
+        for pair in [eager, *graphs[k][1]]:
+            assert all(torch.equal(a, b) for a, b in zip(pair, want))
+
+
+@pytest.mark.parametrize("rows8", [False, True])
+def test_the_example_generates_what_a_dense_layer_does(rows8):
+    """Logits of the paged path against the dense layer: attention's outputs round to bf16 in both (2^-8 of each number, two
+    products behind them average it out), 8-bit rows are off by half a step of 1/255 of a row's range, some 6 standard deviations."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_decode.py")
+    spec = importlib.util.spec_from_file_location("paged_decode", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    said, lengths, logits, d = example.generate(requests=5, steps=20, rows8=rows8)
+    for r in range(5):
+        n = int(lengths[r])
+        assert (said[r, :n] >= 0).all() and (said[r, n:] == -1).all()
+        want = example.dense_logits(d, said[r, :n - 1]).float()
+        off = float((logits[r].float() - want).norm() / want.norm())
+        assert off < (0.05 if rows8 else 0.02), off
