@@ -81,7 +81,7 @@ SYMBOLS = {
     "fbgemm_amd_kv_block_tables": (C.c_int, [_P, _P, _I32, _I64, _P, _I64, _I64, _P, _I64, _P, _I32, _I64, _P, _P, _P, _P, _P, _P, _P]),
     "fbgemm_amd_kv_cache_append": (C.c_int, [C.POINTER(PagedCache), _P, _P, _I32, _I64, C.POINTER(_I64), C.POINTER(_I64), _P, _P, _P, _P, _P]),
     "fbgemm_amd_paged_attention_workspace": (_I64, [C.POINTER(PagedCache), _I64, _I32, _I64]),
-    "fbgemm_amd_paged_attention": (C.c_int, [C.POINTER(PagedCache), _P, _I32, _I64, _I32, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I32, C.c_float, _I64, C.c_float, _P, _P, _P, _I64, _P, _P]),
+    "fbgemm_amd_paged_attention": (C.c_int, [C.POINTER(PagedCache), _P, _I32, _I64, _I32, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I32, C.c_float, _I64, C.c_float, _P, _P, _P, _I64, _P]),
     "fbgemm_amd_penalize_logits": (C.c_int, [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P, _I32, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _I64, _P]),
     "fbgemm_amd_unpadded_row_size_in_bytes": (_I32, [_I32, _I32, _I32]),
     "fbgemm_amd_padded_row_size_in_bytes": (_I32, [_I32, _I32, _I32, _I32]),

@@ -82,11 +82,9 @@ struct AttentionArgs {
   int32_t workers;
   float* partial;     // [workers][2][rows][dim]
   float* partial_ml;  // [workers][2][rows][2]
-  uint32_t* counters; // [levels][ATTENTION_COUNTERS], zero before and behind a call
+  int4* joins;        // [workers]: the last worker of the pair that begins with this one (-1: none goes on), its rows, the first of them
 };
 constexpr int ATTENTION_STEP = 128; // tokens of a unit of work
-// The most workers, and the levels by which groups of eight of them, of eight such groups and so on are joined
-constexpr int ATTENTION_COUNTERS = 2048, ATTENTION_LEVELS = 4;
 // workgroups of the attention kernel that a compute unit holds at once: what its registers leave room for
 constexpr int attention_residents(int dim) { return dim > 128 ? 1 : dim > 64 ? 2 : 3; }
 constexpr int ATTENTION_ROWS = 16; // queries of a key head that one tile of the matrix cores takes

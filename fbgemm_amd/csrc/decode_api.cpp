@@ -14,7 +14,6 @@ using namespace fbgemm_amd;
 namespace {
 
 constexpr int64_t MOST = 0x7fffffff;
-static_assert(FBGEMM_AMD_PAGED_ATTENTION_COUNTERS == ATTENTION_COUNTERS * ATTENTION_LEVELS, "");
 
 bool divides(int64_t a, std::initializer_list<int64_t> values) {
   for (int64_t v : values)
@@ -69,7 +68,7 @@ int compute_units() {
 int attention_workers(const fbgemm_amd_paged_cache& c, int64_t requests, int32_t query_heads, int64_t max_tokens) {
   const int64_t sets = (int64_t)c.heads * ((query_heads / c.heads + ATTENTION_ROWS - 1) / ATTENTION_ROWS);
   const int64_t each = std::max<int64_t>(1, (max_tokens + 15 + ATTENTION_STEP - 1) / ATTENTION_STEP);
-  const int64_t most = std::min<int64_t>(ATTENTION_COUNTERS, (int64_t)compute_units() * attention_residents(c.dim));
+  const int64_t most = (int64_t)compute_units() * attention_residents(c.dim);
   if (requests * sets >= most || each >= most) return (int)most;
   return (int)std::min(most, requests * sets * each);
 }
@@ -80,13 +79,14 @@ int64_t attention_max_tokens(const fbgemm_amd_paged_cache& c, int64_t table_widt
 }
 
 struct AttentionSpace {
-  int64_t partial, ml, total;
+  int64_t partial, ml, joins, total;
 };
 AttentionSpace attention_space(int workers, int32_t dim) {
   AttentionSpace s;
   s.partial = (int64_t)workers * 2 * ATTENTION_ROWS * dim * (int64_t)sizeof(float);
   s.ml = (int64_t)workers * 2 * ATTENTION_ROWS * 2 * (int64_t)sizeof(float);
-  s.total = s.partial + s.ml;
+  s.joins = (int64_t)workers * (int64_t)sizeof(int4);
+  s.total = s.partial + s.ml + s.joins;
   return s;
 }
 
@@ -212,7 +212,7 @@ int fbgemm_amd_paged_attention(
     const fbgemm_amd_paged_cache* cache, const void* d_query, int32_t query_ty, int64_t requests, int32_t query_heads,
     int64_t query_request_stride, int64_t query_head_stride, const void* d_key_cache, const void* d_value_cache,
     const int32_t* d_block_tables, int64_t table_stride, int64_t table_width, const void* d_lengths, int32_t index_bits,
-    float scale, int64_t window, float softcap, void* d_output, float* d_lse, void* d_workspace, int64_t workspace_bytes, uint32_t* d_counters, void* stream) {
+    float scale, int64_t window, float softcap, void* d_output, float* d_lse, void* d_workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = check_attention(cache, requests, query_heads, table_width)) return rc;
   const bool rows8 = cache->row_ty == ST_INT8;
   if (query_ty != ST_FP16 && query_ty != ST_BF16) return fail(FBGEMM_AMD_E_UNSUPPORTED, "queries are FP16 or BF16");
@@ -223,7 +223,7 @@ int fbgemm_amd_paged_attention(
   if (!(softcap >= 0.0f) || !std::isfinite(softcap)) return fail(FBGEMM_AMD_E_ARG, "softcap must be finite and not negative");
   if (requests == 0) return 0;
   const int64_t max_tokens = attention_max_tokens(*cache, table_width);
-  if (!d_query || !d_lengths || !d_output || !d_lse || !d_workspace || !d_counters || (max_tokens > 0 && (!d_block_tables || !d_key_cache || !d_value_cache)))
+  if (!d_query || !d_lengths || !d_output || !d_lse || !d_workspace || (max_tokens > 0 && (!d_block_tables || !d_key_cache || !d_value_cache)))
     return fail(FBGEMM_AMD_E_ARG, "null data pointer");
   AttentionArgs a;
   a.query = (const char*)d_query;
@@ -261,7 +261,7 @@ int fbgemm_amd_paged_attention(
   if (workspace_bytes < space.total) return fail(FBGEMM_AMD_E_ARG, "workspace of %lld bytes: %lld are needed", (long long)workspace_bytes, (long long)space.total);
   a.partial = (float*)d_workspace;
   a.partial_ml = (float*)((char*)d_workspace + space.partial);
-  a.counters = d_counters;
+  a.joins = (int4*)((char*)d_workspace + space.partial + space.ml);
   if (query_ty == ST_BF16) HIP_TRY(rows8 ? launch_paged_attention_bf16_rows8(a, (hipStream_t)stream) : launch_paged_attention_bf16(a, (hipStream_t)stream));
   else HIP_TRY(rows8 ? launch_paged_attention_fp16_rows8(a, (hipStream_t)stream) : launch_paged_attention_fp16(a, (hipStream_t)stream));
   return 0;

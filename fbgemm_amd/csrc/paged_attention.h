@@ -29,9 +29,10 @@
 // that order. Each of W workers takes a W-th of them in a row, whatever requests they are of, so that all end together
 // however long the requests are; a pair of request and head weighs one more than its steps, or a worker that meets
 // many short ones would be late. The waves' sums of a pair are joined in LDS. A pair that a worker has whole it writes
-// out; of one that it shares with its neighbours (its first and its last, at
-// most) it leaves the sums, and the last of eight workers to leave some adds theirs up in the workers' order, the last of
-// eight such groups these, and so on: one launch, few loads in a row, and results that depend on no order.
+// out; of one that it shares with its neighbours (its first and its last, at most) it leaves the sums, which a second
+// launch adds up in the workers' order: results depend on no order of theirs. (Joining them in the first launch, by the last worker
+// to arrive, takes fences that write back and empty whole caches, each die having its own: with those 64 requests of 1 to
+// 4 096 tokens took 367 us where two launches take 109.)
 #pragma once
 #include "decode.h"
 
@@ -41,7 +42,6 @@ constexpr int ATT_WAVES = 4;
 constexpr int ATT_TILE = 32; // tokens of a wave's step
 constexpr int ATT_STEP = ATT_WAVES * ATT_TILE; // of all waves'
 static_assert(ATT_STEP == ATTENTION_STEP, "");
-constexpr uint32_t ATT_JOIN = 8;               // workers whose sums are added up at once
 constexpr float ATT_LOG2E = 1.4426950408889634f;
 
 #if defined(__HIPCC__)
@@ -521,21 +521,6 @@ struct Attention {
   }
 };
 
-// What workers leave for each other: words that are read and written where all of the device sees them (agent-scope atomics go
-// past the L2 caches, of which each die has its own), in order by the wait between the last of them and the arrival
-// that says so. Plain stores and loads would need fences that write back and empty whole caches: 768 workers
-// with one each took 300 us.
-__device__ __forceinline__ void leave(float* to, float a, float b) {
-  __hip_atomic_store(reinterpret_cast<uint64_t*>(to), (uint64_t)__builtin_bit_cast(uint32_t, a) | ((uint64_t)__builtin_bit_cast(uint32_t, b) << 32),
-                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void found(const float* from, float& a, float& b) {
-  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  a = __builtin_bit_cast(float, (uint32_t)v);
-  b = __builtin_bit_cast(float, (uint32_t)(v >> 32));
-}
-__device__ __forceinline__ void all_left() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 // Four columns of a row of sums, as they come
 struct Sums {
   float m, l;
@@ -564,7 +549,6 @@ __global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP)) void paged
   constexpr int THREADS = 64 * ATT_WAVES;
   __shared__ __attribute__((aligned(16))) float s_acc[ATT_WAVES][ATTENTION_ROWS][DP + 4];
   __shared__ float s_ml[ATT_WAVES][ATTENTION_ROWS][2];
-  __shared__ uint32_t s_arrived;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t worker = blockIdx.x;
@@ -578,6 +562,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP)) void paged
   total = __builtin_amdgcn_readlane(sum_first, 63) + (a.requests > 64 ? __builtin_amdgcn_readlane(inclusive_sum(total, lane), 63) : 0u);
   const uint32_t U = total * sets;
   const uint32_t W = U < (uint32_t)a.workers ? U : (uint32_t)a.workers; // each has a unit at least
+  if (tid == 0) a.joins[worker] = make_int4(-1, 0, 0, 0);
   if (worker >= W) return;
   const Shares shares(U, W);
   uint32_t unit = shares.begin(worker);
@@ -665,64 +650,64 @@ __global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP)) void paged
         if (FULL || d < a.dim) f(row, d);
       }
     };
-    // a worker's two places: the second for a pair that begins with it
-    const uint32_t first = s.c0 == 0 ? worker : shares.worker_of(s.first);
-    const auto place = [&](uint32_t w, int row) { return ((int64_t)w * 2 + (w == first ? 1 : 0)) * ATTENTION_ROWS + row; };
-    const auto leave_sum = [&](uint32_t w, int row, int d, const Sums& sum) {
-      const int64_t at = place(w, row);
-      leave(&a.partial[at * a.dim + d], sum.y[0], sum.y[1]);
-      leave(&a.partial[at * a.dim + d + 2], sum.y[2], sum.y[3]);
-      if (d == 0) leave(&a.partial_ml[at * 2], sum.m, sum.l);
-    };
     each_four([&](int row, int d) {
       Sums sum{-__builtin_inff(), 0.0f, {0, 0, 0, 0}};
 #pragma unroll
       for (int w = 0; w < ATT_WAVES; ++w) sum.add(s_ml[w][row][0], s_ml[w][row][1], *reinterpret_cast<const f32x4*>(&s_acc[w][row][d]));
-      if (whole) write_out<BF16>(a, s.row + row, d, sum, A::SHIFT);
-      else leave_sum(worker, row, d, sum);
-    });
-    if (!whole) {
-      // ---- sums left by the workers first, first + 1, ...: `count` of them at a distance of `stride`, ours is number `at` ----
-      uint32_t count = shares.worker_of(s.first + s.steps - 1) - first + 1, at = worker - first, stride = 1;
-      for (uint32_t* counters = a.counters;; counters += ATTENTION_COUNTERS) {
-        const uint32_t group = at / ATT_JOIN, members = count - group * ATT_JOIN < ATT_JOIN ? count - group * ATT_JOIN : ATT_JOIN;
-        const uint32_t leader = first + group * ATT_JOIN * stride;
-        all_left();
-        __syncthreads();
-        if (tid == 0) {
-          s_arrived = __hip_atomic_fetch_add(&counters[leader], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          if (s_arrived == members - 1) __hip_atomic_store(&counters[leader], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
+      if (whole) {
+        write_out<BF16>(a, s.row + row, d, sum, A::SHIFT);
+      } else { // a worker's two places: the second for a pair that begins with it
+        const int64_t at = ((int64_t)worker * 2 + (s.c0 == 0 ? 1 : 0)) * ATTENTION_ROWS + row;
+        *reinterpret_cast<f32x4*>(&a.partial[at * a.dim + d]) = sum.y;
+        if (d == 0) {
+          a.partial_ml[at * 2] = sum.m;
+          a.partial_ml[at * 2 + 1] = sum.l;
         }
-        __syncthreads();
-        if (s_arrived != members - 1) break;
-        const bool all = count <= ATT_JOIN;
-        each_four([&](int row, int d) {
-          float m[ATT_JOIN], l[ATT_JOIN];
-          f32x4 y[ATT_JOIN];
-#pragma unroll
-          for (uint32_t k = 0; k < ATT_JOIN; ++k) {
-            const int64_t p = place(leader + (k < members ? k : 0) * stride, row);
-            float y0, y1, y2, y3;
-            found(&a.partial_ml[p * 2], m[k], l[k]);
-            found(&a.partial[p * a.dim + d], y0, y1);
-            found(&a.partial[p * a.dim + d + 2], y2, y3);
-            y[k] = f32x4{y0, y1, y2, y3};
-          }
-          Sums sum{m[0], l[0], y[0]};
-#pragma unroll
-          for (uint32_t k = 1; k < ATT_JOIN; ++k)
-            if (k < members) sum.add(m[k], l[k], y[k]);
-          if (all) write_out<BF16>(a, s.row + row, d, sum, A::SHIFT);
-          else leave_sum(leader, row, d, sum); // in the leader's place: nobody else looks there before we arrive
-        });
-        if (all) break;
-        count = (count + ATT_JOIN - 1) / ATT_JOIN;
-        at = group;
-        stride *= ATT_JOIN;
       }
-    }
+    });
+    if (!whole && s.c0 == 0 && tid == 0) a.joins[worker] = make_int4((int)shares.worker_of(s.first + s.steps - 1), s.rows, (int)s.row, (int)(s.row >> 32));
     __syncthreads();
   }
+}
+
+// Where a pair begins with a worker and goes on with others, their sums are added up. A workgroup has 256 / DP of its
+// rows: a thread four columns of one and every fourth worker, eight at a time.
+template <bool BF16, int DP>
+__global__ __launch_bounds__(256) void paged_attention_join_kernel(const AttentionArgs a, const int groups, const float shift) {
+  constexpr int COLUMNS = DP / 4, ROWS = 64 / COLUMNS, SLICES = 4, AT_ONCE = 8;
+  __shared__ Sums s_sums[SLICES][64];
+  const int worker = blockIdx.x / groups, group = blockIdx.x - worker * groups;
+  const int4 join = a.joins[worker];
+  const int place = threadIdx.x & 63, slice = threadIdx.x >> 6;
+  const int row = group * ROWS + place / COLUMNS, d = 4 * (place % COLUMNS);
+  if (join.x < 0 || group * ROWS >= join.y) return; // the whole workgroup
+  const bool mine = row < join.y && d < a.dim;
+  const int parts = join.x - worker + 1;
+  Sums sum{-__builtin_inff(), 0.0f, {0, 0, 0, 0}};
+  if (mine) {
+    for (int k0 = slice; k0 < parts; k0 += SLICES * AT_ONCE) {
+      float m[AT_ONCE], l[AT_ONCE];
+      f32x4 y[AT_ONCE];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int k = k0 + SLICES * i < parts ? k0 + SLICES * i : k0;
+        const int64_t at = ((int64_t)(worker + k) * 2 + (k == 0 ? 1 : 0)) * ATTENTION_ROWS + row;
+        m[i] = a.partial_ml[at * 2];
+        l[i] = a.partial_ml[at * 2 + 1];
+        y[i] = *reinterpret_cast<const f32x4*>(&a.partial[at * a.dim + d]);
+      }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i)
+        if (k0 + SLICES * i < parts) sum.add(m[i], l[i], y[i]);
+    }
+  }
+  s_sums[slice][place] = sum;
+  __syncthreads();
+  if (slice || !mine) return;
+#pragma unroll
+  for (int i = 1; i < SLICES; ++i) sum.add(s_sums[i][place].m, s_sums[i][place].l, s_sums[i][place].y);
+  const int64_t first = (int64_t)(uint32_t)join.z | ((int64_t)join.w << 32);
+  write_out<BF16>(a, first + row, d, sum, shift);
 }
 
 template <bool BF16, bool ROWS8, int DP, bool FULL>
@@ -735,6 +720,10 @@ template <bool BF16, bool ROWS8, int DP>
 hipError_t launch_dp(const AttentionArgs& a, hipStream_t stream) {
   if (a.dim == DP) launch_kernel<BF16, ROWS8, DP, true>(a, stream);
   else launch_kernel<BF16, ROWS8, DP, false>(a, stream);
+  if (hipError_t e = hipGetLastError()) return e;
+  if (a.max_tokens <= ATT_STEP - 15) return hipSuccess; // a pair is one step: nobody shares it
+  const int rows = a.group < ATTENTION_ROWS ? a.group : ATTENTION_ROWS, groups = (rows + 256 / DP - 1) / (256 / DP);
+  paged_attention_join_kernel<BF16, DP><<<a.workers * groups, 256, 0, stream>>>(a, groups, ROWS8 || BF16 ? 0.0f : 14.0f);
   return hipGetLastError();
 }
 

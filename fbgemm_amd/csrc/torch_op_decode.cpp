@@ -8,8 +8,6 @@
 #include <torch/library.h>
 
 #include <cmath>
-#include <map>
-#include <mutex>
 #include <optional>
 #include <tuple>
 
@@ -128,43 +126,6 @@ void kv_cache_append(const Tensor& key, const Tensor& value, Tensor key_cache, T
                                         status_pointer(status, key), current_stream(key)));
 }
 
-// The counters of the attention kernel, zero between calls: one set per device and stream, whose calls run in order, and one
-// per capture and stream, cleared by a kernel that becomes part of the graph: no replay meets another's or an eager call's. A
-// capture's set is let go when later captures have come (its memory stays the graph's).
-struct CounterKey {
-  int device;
-  void* stream;
-  unsigned long long capture; // 0: none
-  bool operator<(const CounterKey& o) const { return std::tie(device, stream, capture) < std::tie(o.device, o.stream, o.capture); }
-};
-std::mutex g_counters_mu;
-std::map<CounterKey, Tensor> g_counters;
-constexpr size_t CAPTURES_KEPT = 16;
-
-Tensor counters_for(const Tensor& like, void* stream) {
-  CounterKey key{(int)like.device().index(), stream, 0};
-  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  unsigned long long id = 0;
-  TORCH_CHECK(hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) == hipSuccess, "fbgemm_amd: hipStreamGetCaptureInfo failed");
-  if (status == hipStreamCaptureStatusActive) key.capture = id + 1;
-  std::lock_guard<std::mutex> lk(g_counters_mu);
-  auto it = g_counters.find(key);
-  if (it == g_counters.end()) {
-    if (key.capture) {
-      size_t captures = 0;
-      auto oldest = g_counters.end();
-      for (auto e = g_counters.begin(); e != g_counters.end(); ++e)
-        if (e->first.capture) {
-          ++captures;
-          if (oldest == g_counters.end() || e->first.capture < oldest->first.capture) oldest = e;
-        }
-      if (captures >= CAPTURES_KEPT) g_counters.erase(oldest);
-    }
-    it = g_counters.emplace(key, at::zeros({FBGEMM_AMD_PAGED_ATTENTION_COUNTERS}, like.options().dtype(at::kInt))).first;
-  }
-  return it->second;
-}
-
 std::tuple<Tensor, Tensor> paged_attention(
     const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& block_tables, const Tensor& lengths,
     std::optional<double> scale, int64_t window, double softcap) {
@@ -186,13 +147,11 @@ std::tuple<Tensor, Tensor> paged_attention(
   Tensor out = at::empty({B, heads, dim}, query.options());
   Tensor lse = at::empty({B, heads}, query.options().dtype(at::kFloat));
   Tensor space = at::empty({bytes}, query.options().dtype(at::kByte));
-  void* stream = current_stream(query);
-  const Tensor counters = counters_for(query, stream);
   CHECK_CALL(fbgemm_amd_paged_attention(
       &cache, query.data_ptr(), float_type(query.scalar_type(), "query"), B, (int32_t)heads, stride_of(query, 0), stride_of(query, 1),
       key_cache.data_ptr(), value_cache.data_ptr(), (const int32_t*)block_tables.data_ptr(), stride_of(block_tables, 0), block_tables.size(1),
       lengths.data_ptr(), index_bits(lengths, "lengths"), (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)dim)), window, (float)softcap,
-      out.data_ptr(), (float*)lse.data_ptr(), space.data_ptr(), bytes, (uint32_t*)counters.data_ptr(), stream));
+      out.data_ptr(), (float*)lse.data_ptr(), space.data_ptr(), bytes, current_stream(query)));
   return {out, lse};
 }
 

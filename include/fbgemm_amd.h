@@ -640,16 +640,13 @@ int fbgemm_amd_kv_cache_append(
  * requests * heads * table_width * block_size below some 2^37. Scores, weights
  * and sums are fp32 (weights go to the matrix cores as two 16-bit numbers); results do
  * not depend on the order in which workgroups run. d_workspace: scratch of
- * fbgemm_amd_paged_attention_workspace bytes. d_counters:
- * FBGEMM_AMD_PAGED_ATTENTION_COUNTERS words that are zero before the first call that
- * takes them (every call leaves them zero). No other call may use either at the same time. */
-enum { FBGEMM_AMD_PAGED_ATTENTION_COUNTERS = 8192 };
+ * fbgemm_amd_paged_attention_workspace bytes that no other call uses at the same time. */
 int64_t fbgemm_amd_paged_attention_workspace(const fbgemm_amd_paged_cache* cache, int64_t requests, int32_t query_heads, int64_t table_width);
 int fbgemm_amd_paged_attention(
     const fbgemm_amd_paged_cache* cache, const void* d_query, int32_t query_ty, int64_t requests, int32_t query_heads,
     int64_t query_request_stride, int64_t query_head_stride, const void* d_key_cache, const void* d_value_cache,
     const int32_t* d_block_tables, int64_t table_stride, int64_t table_width, const void* d_lengths, int32_t index_bits,
-    float scale, int64_t window, float softcap, void* d_output, float* d_lse, void* d_workspace, int64_t workspace_bytes, uint32_t* d_counters, void* stream);
+    float scale, int64_t window, float softcap, void* d_output, float* d_lse, void* d_workspace, int64_t workspace_bytes, void* stream);
 
 /* Logits [rows][vocab] (FP32, FP16 or BF16) made ready to sample from. A row's tokens
  * are d_tokens[d_offsets[row] .. d_offsets[row + 1] - 1], the first

@@ -570,8 +570,23 @@ def test_attention_on_two_streams_at_once(decode, rows8):
         assert all(torch.equal(a, b) for pair in got[k] for a, b in zip(pair, want[k]))
 
 
+def test_attention_call_behind_call(decode):
+    """Calls of other inputs one behind the other, nothing waiting between: each one's sums are its own, though their scratch is one."""
+    cases = [attention_case(decode, 40 + k, 64, 4, 2, 16, lengths, torch.bfloat16, rows8)
+             for k, (lengths, rows8) in enumerate((([20011, 300, 5], False), ([77, 9000, 4099], False), ([12345], True), ([1, 30003], True)))]
+    call = lambda case: decode.paged_attention(case[0], *case[1], case[3], case[4])  # noqa: E731
+    want = []
+    for case in cases:
+        want.append(call(case))
+        torch.cuda.synchronize()
+    for order in ((0, 1, 0, 1, 2, 3, 2, 0), (3, 2, 1, 0, 0, 3, 1, 2)):
+        got = [(k, call(cases[k])) for k in order for _ in range(3)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for k, pair in got for a, b in zip(pair, want[k]))
+
+
 def test_attention_in_many_captures(decode):
-    """More captures than the operator keeps counters of, replayed out of order, beside eager calls."""
+    """Many captures, replayed out of order, beside eager calls."""
     q, c, _, t, n = attention_case(decode, 30, 64, 2, 1, 16, [9001, 70], torch.bfloat16)
     want = decode.paged_attention(q, *c, t, n)
     graphs = []

@@ -70,12 +70,12 @@ def test_append_refusals(lib):
 
 
 def test_attention_refusals(lib):
-    def call(c=None, ty=5, requests=2, heads=4, stride=256, width=3, bits=32, scale=0.1, window=0, softcap=0.0, query=P, out=P, space=P, size=1 << 30, counters=P):
+    def call(c=None, ty=5, requests=2, heads=4, stride=256, width=3, bits=32, scale=0.1, window=0, softcap=0.0, query=P, out=P, space=P, size=1 << 30):
         return lib.fbgemm_amd_paged_attention(C.byref(c or cache()), query, ty, requests, heads, stride, 64, P, P, P, width, width, P, bits, scale, window,
-                                              softcap, out, P, space, size, counters, None)
+                                              softcap, out, P, space, size, None)
     for change, word in (({"ty": 0}, "FP16 or BF16"), ({"ty": 1}, "type"), ({"requests": -1}, "requests"), ({"heads": 3}, "multiple"), ({"heads": 0}, "multiple"),
                          ({"width": -1}, "table_width"), ({"bits": 8}, "index_bits"), ({"scale": float("inf")}, "scale"), ({"window": -1}, "window"),
-                         ({"softcap": -1.0}, "softcap"), ({"softcap": float("nan")}, "softcap"), ({"query": None}, "null"), ({"space": None}, "null"), ({"counters": None}, "null"),
+                         ({"softcap": -1.0}, "softcap"), ({"softcap": float("nan")}, "softcap"), ({"query": None}, "null"), ({"space": None}, "null"),
                          ({"size": 100}, "workspace"), ({"stride": 260}, "16-byte"), ({"query": C.c_void_p(4104)}, "16-byte"), ({"out": C.c_void_p(4104)}, "16-byte"),
                          ({"c": cache(dim=60)}, "multiple of 8"), ({"c": cache(dim=264)}, "256"), ({"c": cache(row_ty=0)}, "FP16, BF16 or INT8"),
                          ({"c": cache(key_strides=(2048, 1024, 60))}, "16-byte")):
