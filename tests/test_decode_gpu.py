@@ -404,7 +404,8 @@ def check_logits(decode, c, logits=None, out=None):
 @pytest.mark.parametrize("index", [np.int32, np.int64])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("rows,vocab,history,biases,mask", [
-    (1, 1, 3, 1, True), (2, 31, 40, 0, True), (3, 33, 0, 4, False), (4, 8191, 500, 5, True), (5, 8193, 3000, 0, False), (2, 40_001, 70_000, 300, True)])
+    (1, 1, 3, 1, True), (2, 31, 40, 0, True), (3, 33, 0, 4, False), (4, 8191, 500, 5, True), (5, 8193, 3000, 0, False), (2, 40_001, 70_000, 300, True),
+    (2, 6000, 900, 2047, True), (3, 6000, 900, 2048, False), (1, 5000, 1_060_000, 7, True)])
 def test_logits(decode, rows, vocab, history, biases, mask, dtype, index):
     check_logits(decode, logits_case(vocab, rows, vocab, history, biases, mask, dtype, index))
 
