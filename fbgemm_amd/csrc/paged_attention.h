@@ -34,6 +34,8 @@
 // to arrive, takes fences that write back and empty whole caches, each die having its own: with those 64 requests of 1 to
 // 4 096 tokens took 367 us where two launches take 109.)
 #pragma once
+#include <type_traits>
+
 #include "decode.h"
 
 namespace fbgemm_amd {
@@ -671,10 +673,11 @@ __global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP)) void paged
 }
 
 // Where a pair begins with a worker and goes on with others, their sums are added up. A workgroup has 256 / DP of its
-// rows: a thread four columns of one and every fourth worker, eight at a time.
+// rows: a thread four columns of one and every fourth worker, sixteen of them at a time where there are many: rounds of
+// loads are what it takes, not bytes (64 workers a pair, 8 rows of 128: 11.2 us in rounds of eight).
 template <bool BF16, int DP>
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(const AttentionArgs a, const int groups, const float shift) {
-  constexpr int COLUMNS = DP / 4, ROWS = 64 / COLUMNS, SLICES = 4, AT_ONCE = 8;
+  constexpr int COLUMNS = DP / 4, ROWS = 64 / COLUMNS, SLICES = 4;
   __shared__ Sums s_sums[SLICES][64];
   const int worker = blockIdx.x / groups, group = blockIdx.x - worker * groups;
   const int4 join = a.joins[worker];
@@ -684,7 +687,8 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const Attenti
   const bool mine = row < join.y && d < a.dim;
   const int parts = join.x - worker + 1;
   Sums sum{-__builtin_inff(), 0.0f, {0, 0, 0, 0}};
-  if (mine) {
+  const auto add_all = [&](auto at_once) {
+    constexpr int AT_ONCE = decltype(at_once)::value;
     for (int k0 = slice; k0 < parts; k0 += SLICES * AT_ONCE) {
       float m[AT_ONCE], l[AT_ONCE];
       f32x4 y[AT_ONCE];
@@ -700,6 +704,10 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const Attenti
       for (int i = 0; i < AT_ONCE; ++i)
         if (k0 + SLICES * i < parts) sum.add(m[i], l[i], y[i]);
     }
+  };
+  if (mine) {
+    if (parts <= 2 * SLICES) add_all(std::integral_constant<int, 2>());
+    else add_all(std::integral_constant<int, 16>());
   }
   s_sums[slice][place] = sum;
   __syncthreads();
