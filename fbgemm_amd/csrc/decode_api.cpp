@@ -37,6 +37,7 @@ int check_cache(const fbgemm_amd_paged_cache* c) {
   if (c->dim <= 0 || c->dim > (1 << 16)) return fail(FBGEMM_AMD_E_ARG, "dim must be in 1..65536");
   if (!cache_row_bytes(*c)) return fail(FBGEMM_AMD_E_ARG, "a cache holds FP32, FP16, BF16 or INT8 rows");
   if (c->heads <= 0 || c->heads > (1 << 16)) return fail(FBGEMM_AMD_E_ARG, "heads must be in 1..65536");
+  if ((int64_t)c->heads * c->dim > (1 << 28)) return fail(FBGEMM_AMD_E_ARG, "heads * dim must not exceed 2^28");
   if (c->block_size <= 0 || c->block_size > (1 << 20)) return fail(FBGEMM_AMD_E_ARG, "block_size must be in 1..1048576");
   if (c->blocks < 0 || c->blocks > MOST) return fail(FBGEMM_AMD_E_ARG, "blocks must be in 0..2^31-1");
   for (int k = 0; k < 3; ++k)
