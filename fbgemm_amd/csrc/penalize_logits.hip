@@ -16,7 +16,8 @@
 //
 // 256 rows of 131 071 bf16 logits: 26 us with nothing to do (5.1 TB/s), 35 with lists of 0 .. 4 096
 // tokens, 48 with biases and a mask too, by then bound by vector instructions. Tried: copying all under
-// the mask first and writing the named ones again (99), counts and biases in one word (49).
+// the mask first and writing the named ones again (99), counts and biases in one word (49), a list of
+// the named ones made from what the counts' atomics return (58).
 #include "decode.h"
 
 namespace fbgemm_amd {
