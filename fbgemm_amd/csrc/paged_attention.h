@@ -5,8 +5,10 @@
 //
 // in one pass over the tokens with the running m and sum, all in fp32 (exp as exp2 of s * log2 e).
 //
-// Bound by memory: every row of the cache is read once for all the queries that share its head.
-// That the rows need no staging in LDS, no transposition through it and no exchange between lanes
+// Bound by memory: every row of the cache is read once for up to 16 queries that share its head (more
+// read it once per 16). 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, bf16: 674 us,
+// 6.39 TB/s; 64 requests of 1 to 4 096, 32 queries on 8: 92 us, 5.87 TB/s; one of 262 143 in 8-bit rows:
+// 110 us, 5.0 TB/s; one of 500: 9.7 us, launches and a chain of dependent steps. That the rows need no staging in LDS, no transposition through it and no exchange between lanes
 // is what the operand layouts of the 16x16x32 products give, written here as l = 16 g + n:
 //   keys     A = K [token n][8 of dim], B = Q^T [8 of dim][query n]: C holds tokens 4g .. 4g+3 of query n
 //   values   A = V^T [a column][8 tokens], B = P^T [8 tokens][query n]: a product sums over tokens in any
@@ -32,7 +34,7 @@
 // out; of one that it shares with its neighbours (its first and its last, at most) it leaves the sums, which a second
 // launch adds up in the workers' order: results depend on no order of theirs. (Joining them in the first launch, by the last worker
 // to arrive, takes fences that write back and empty whole caches, each die having its own: with those 64 requests of 1 to
-// 4 096 tokens took 367 us where two launches take 109.)
+// 4 096 tokens took 367 us where two launches took 109 at the time.)
 #pragma once
 #include <type_traits>
 
