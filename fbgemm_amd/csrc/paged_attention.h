@@ -8,7 +8,7 @@
 // Bound by memory: every row of the cache is read once for up to 16 queries that share its head (more
 // read it once per 16). 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, bf16: 674 us,
 // 6.39 TB/s; 64 requests of 1 to 4 096, 32 queries on 8: 92 us, 5.87 TB/s; one of 262 143 in 8-bit rows:
-// 110 us, 5.0 TB/s; one of 500: 9.7 us, launches and a chain of dependent steps. That the rows need no staging in LDS, no transposition through it and no exchange between lanes
+// 102 us, 5.4 TB/s; one of 500: 9.7 us, launches and a chain of dependent steps. That the rows need no staging in LDS, no transposition through it and no exchange between lanes
 // is what the operand layouts of the 16x16x32 products give, written here as l = 16 g + n:
 //   keys     A = K [token n][8 of dim], B = Q^T [8 of dim][query n]: C holds tokens 4g .. 4g+3 of query n
 //   values   A = V^T [a column][8 tokens], B = P^T [8 tokens][query n]: a product sums over tokens in any
@@ -206,7 +206,8 @@ __device__ __forceinline__ uint32_t inclusive_sum(uint32_t v, int lane) {
 // columns behind read the row's first ones in their place, which meet zeros in the queries or make outputs that nobody wants.
 // PAGE16: pages are whole 16-token tiles, whose addresses are then the same for the wave. PACKED (FULL 8-bit rows, PAGE16): the
 // rows of a page's tokens follow each other without gaps. 16 of them are then read as one run of bytes, every line by one
-// load and marked as read once, and go through LDS, where a lane finds its pieces: 262 143 tokens XX us, 110 without.
+// load and marked as read once, and go through LDS, where a lane finds its pieces: 262 143 tokens 102 us, 110 without
+// (two tiles ahead instead of one: 104); 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, 408 us, 464 without.
 template <bool BF16, bool ROWS8, int DP, bool FULL, bool PAGE16, bool PACKED>
 struct Attention {
   static constexpr int KP = DP / 32;                   // products of a key tile
