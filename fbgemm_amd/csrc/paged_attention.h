@@ -24,8 +24,12 @@
 // those 2^-28 of the largest are still normal numbers. The second product costs matrix time of
 // which there is plenty (24 products, 384 cycles, for the 16 KB of 32 tokens x 128 columns).
 //
-// 8-bit rows (fp16 scale a_t and bias b_t in front): s_t = a_t (q . k8_t) + b_t sum(q), and weights
-// p_t a_t for the bytes, p_t b_t for the bias: 0 .. 255 are exact in bf16 and fp16.
+// 8-bit rows (fp16 scale a_t and bias b_t in front): s_t = a_t (q . k8_t) + b_t sum(q); values by c8 = v8 - 128 and
+// b'_t = b_t + 128 a_t: weights p_t a_t for c8, p_t b'_t beside them. -128 .. 255 are exact in bf16 and fp16. Rows lie
+// about zero, so b' is small and both sums are of the result's size. By v8 and b both are some 128 steps of a row's scale
+// and cancel, with what the cut of the weights and the sums' roundings made of them: columns of zeros came out as 2^-18 of
+// the scale, not as zeros. Flipping the bytes' top bits costs 0.7 to 2 % (262 143 tokens 101.5 -> 102.2 us). A score's
+// rounding is 2^-24 of that anyway; keys are centred where it is free (fp16).
 //
 // Work: steps of 128 tokens of a (request, key head, 16 queries), 32 for each of a worker's (workgroup's) four waves, numbered in
 // that order. Each of W workers takes a W-th of them in a row, whatever requests they are of, so that all end together
@@ -98,7 +102,16 @@ __device__ __forceinline__ void split(const float (&p)[8], uint4& hi, uint4& lo)
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// 8 bytes -> 8 numbers of 16 bits, exactly
+// Bytes with their top bits flipped are byte - 128 in two's complement. Four at a time, and the compiler is kept from doing it
+// byte by byte: then each is one conversion of a signed byte in place, as without (else a third instruction each).
+__device__ __forceinline__ uint32_t centre(uint32_t bytes) {
+  bytes ^= 0x80808080u;
+  asm("" : "+v"(bytes));
+  return bytes;
+}
+__device__ __forceinline__ float centred(uint32_t flipped, int i) { return (float)(int8_t)(flipped >> (8 * i)); }
+
+// 8 bytes -> 8 numbers of 16 bits, exactly: byte - 128 for fp16, which a constant gives, the byte for bf16
 template <bool BF16>
 __device__ __forceinline__ uint4 widen(uint32_t a, uint32_t b) {
   uint32_t r[4];
@@ -111,7 +124,7 @@ __device__ __forceinline__ uint4 widen(uint32_t a, uint32_t b) {
       r[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u);
     } else { // 1024 + byte is the byte under fp16's exponent 0x64
       const uint32_t v = __builtin_amdgcn_perm(0x64646464u, w, i & 1 ? 0x04030402u : 0x04010400u);
-      const f16x2 off = {(_Float16)1024.0f, (_Float16)1024.0f};
+      const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
       r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, v) - off);
     }
   }
@@ -119,6 +132,8 @@ __device__ __forceinline__ uint4 widen(uint32_t a, uint32_t b) {
 }
 
 __device__ __forceinline__ float half_at(uint32_t pair, int i) { return (float)__builtin_bit_cast(f16x2, pair)[i]; }
+// what byte 128 of a row stands for, by its scale and bias
+__device__ __forceinline__ float middle(uint32_t pair) { return __builtin_fmaf(128.0f, half_at(pair, 0), half_at(pair, 1)); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // (1 - t) / (1 + t), t = exp(-2 |x|): off by some 2^-23 of 1
 __device__ __forceinline__ float tanh_fast(float x) {
@@ -505,7 +520,7 @@ struct Attention {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float y = r[j];
-        if (ROWS8) y = __builtin_fmaf(half_at(tile.k_pair[4 * h + j], 0), y, half_at(tile.k_pair[4 * h + j], 1) * q_sum);
+        if (ROWS8) y = __builtin_fmaf(half_at(tile.k_pair[4 * h + j], 0), y, (BF16 ? half_at(tile.k_pair[4 * h + j], 1) : middle(tile.k_pair[4 * h + j])) * q_sum);
         s[4 * h + j] = y * a.scale;
       }
     }
@@ -555,13 +570,21 @@ struct Attention {
     if (ROWS8) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        bias = __builtin_fmaf(p[j], half_at(tile.v_pair[j], 1), bias);
+        bias = __builtin_fmaf(p[j], middle(tile.v_pair[j]), bias);
         p[j] *= half_at(tile.v_pair[j], 0);
       }
     }
     uint4 hi, lo;
     split<PBF16>(p, hi, lo);
     // ---- values ----
+    if constexpr (ROWS8) {
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int r = 0; r < VREGS; ++r) tile.v[h][j][r] = centre(tile.v[h][j][r]);
+    }
 #pragma unroll
     for (int h = 0; h < HALVES; ++h)
 #pragma unroll
@@ -570,7 +593,7 @@ struct Attention {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if constexpr (ROWS8) {
-            const float y0 = (float)((tile.v[h][2 * j][i / 4] >> (i % 4 * 8)) & 0xffu), y1 = (float)((tile.v[h][2 * j + 1][i / 4] >> (i % 4 * 8)) & 0xffu);
+            const float y0 = centred(tile.v[h][2 * j][i / 4], i % 4), y1 = centred(tile.v[h][2 * j + 1][i / 4], i % 4);
             t[j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y1), __builtin_bit_cast(uint32_t, y0), 0x07060302u);
           } else {
             t[j] = __builtin_amdgcn_perm(tile.v[h][2 * j + 1][i / 2], tile.v[h][2 * j][i / 2], i & 1 ? 0x07060302u : 0x05040100u);

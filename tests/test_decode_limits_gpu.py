@@ -1,0 +1,90 @@
+"""The operators of a decoding step at the limits of their arguments and of the number formats they keep."""
+import numpy as np
+import pytest
+
+import decode_reference as R
+from test_decode_finite_gpu import close_and_finite as close
+from test_decode_gpu import attention_case, np64
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def decode():
+    from fbgemm_amd import decode as d
+    return d
+
+
+def rows8_sizes(cache, dim):
+    """Of every element of 8-bit rows, |scale| |byte - 128| + |bias + 128 scale|: the terms that attention adds up."""
+    rows = cache.cpu().numpy()
+    pair = np.ascontiguousarray(rows[..., :4]).view(np.float16).astype(np.float64)
+    return np.abs(pair[..., :1]) * np.abs(rows[..., 4:4 + dim] - 128.0) + np.abs(pair[..., 1:] + 128 * pair[..., :1])
+
+
+def attention64(query, values, sizes, tables, lengths, scale, window=0, softcap=0.0):
+    """(out, lse, bound of out's error, bound of lse's error) in 64 bits, before the last rounding.
+
+    A score is off by at most (D + 8) 2^-24 of the sum of its terms' sizes and 2^-22 of itself, with a cap by 2^-19 of
+    itself: the roundings of scale, ratio and products (10 of 2^-24) and of tanh as a polynomial or as (1 - t) / (1 + t) with
+    t <= 1/2 (6 of 2^-23). A weight: the errors of its score and of the maximum, exp2 (2^-22) and the cut to 16 bits (2^-17),
+    relatively; the sums' own roundings are within the same 2^-16. Neither bound knows of a cap's size."""
+    B, Hq, D = query.shape
+    blocks, H, S, _ = values[0].shape
+    out, lse = np.zeros((B, Hq, D)), np.full((B, Hq), -np.inf)
+    out_off, lse_off = np.zeros((B, Hq, D)), np.zeros((B, Hq))
+    for b in range(B):
+        n = min(max(int(lengths[b]), 0), tables.shape[1] * S)
+        t = np.arange(max(0, n - window) if window else 0, n)
+        page = tables[b, t // S]
+        if not len(t):
+            continue
+        for h in range(Hq):
+            at = (page, h // (Hq // H), t % S)
+            q = query[b, h]
+            s = scale * (values[0][at] @ q)
+            if softcap:
+                s = softcap * np.tanh(s / softcap)
+            wrong = (D + 8) * 2.0 ** -24 * abs(scale) * (sizes[0][at] @ np.abs(q)) + (2.0 ** -19 if softcap else 2.0 ** -22) * np.abs(s)
+            m = s.max()
+            p = np.exp(s - m)
+            total = p.sum()
+            out[b, h], lse[b, h] = p @ values[1][at] / total, m + np.log(total)
+            out_off[b, h] = (2 * wrong.max() + 2.0 ** -15) * (p @ sizes[1][at]) / total
+            lse_off[b, h] = wrong.max() + 2.0 ** -20 * (1 + abs(lse[b, h]))
+    return out, lse, out_off, lse_off
+
+
+def check(decode, case, dtype, scale=None, window=0, softcap=0.0):
+    query, caches, values, tables, lengths = case
+    dim = query.shape[2]
+    rows8 = caches[0].dtype == torch.uint8
+    sizes = [rows8_sizes(c, dim) if rows8 else np.abs(v) for c, v in zip(caches, values)]
+    got, lse = decode.paged_attention(query, *caches, tables, lengths, scale=scale, window=window, softcap=softcap)
+    want, want_lse, off, lse_off = attention64(np64(query), values, sizes, tables.cpu().numpy(), lengths.cpu().numpy(),
+                                               dim ** -0.5 if scale is None else scale, window, softcap)
+    close(got, want, off, dtype)
+    close(lse, want_lse, lse_off, torch.float32)
+
+
+# ---- 8-bit rows -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("layout,block", [("hnd", 16), ("nhd", 16), ("hnd", 10)])
+@pytest.mark.parametrize("dim", [64, 128, 256, 96])
+def test_rows_whose_range_a_single_channel_sets(decode, dim, layout, block, dtype):
+    """One element of a row sets its scale, the others are a step or none away from zero: their sums are of a step's size, not of
+    the range's, and columns of zeros stay zeros."""
+    query, caches, values, tables, lengths = attention_case(decode, dim + block, dim, 4, 2, block, [2, 40, 300, 4099], dtype, True, layout, poison=False)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(dim)
+    for k, c in enumerate(caches):
+        c[..., 4:4 + dim] = torch.randint(127, 130, (*c.shape[:3], dim), device="cuda", generator=g).to(torch.uint8)
+        c[..., 4] = torch.where(torch.rand(c.shape[:3], device="cuda", generator=g) < 0.5, 0, 255).to(torch.uint8)
+        c[..., 4 + dim // 2: 4 + dim] = 128
+        scale = (2.0 / 255 * (0.5 + torch.rand((*c.shape[:3], 1), device="cuda", generator=g))).half()
+        c[..., :4] = torch.cat((scale, -128 * scale), -1).view(torch.uint8)
+        values[k] = R.rows8_values(c.cpu().numpy(), dim)
+    check(decode, (query, caches, values, tables, lengths), dtype)
