@@ -73,8 +73,9 @@ struct AttentionArgs {
   int32_t blocks, block_size;
   int64_t max_tokens; // table width * block size
   Divisor block;
-  float scale;   // of the scores, times log2(e) where there is no cap
-  float softcap; // 0: none
+  float scale;       // of the scores, times log2(e)
+  float softcap;     // times log2(e); 0: none
+  float cap_inverse; // 1 / softcap
   int64_t window; // 0: none
   char* out; // [requests][heads][dim], dense
   float* lse; // [requests][heads]

@@ -252,8 +252,10 @@ int fbgemm_amd_paged_attention(
   a.block_size = cache->block_size;
   a.max_tokens = max_tokens;
   a.block = make_divisor((uint32_t)cache->block_size);
-  a.scale = softcap > 0.0f ? scale / softcap : scale * 1.4426950408889634f;
-  a.softcap = softcap;
+  constexpr double LOG2E = 1.4426950408889634;
+  a.scale = (float)(scale * LOG2E);
+  a.softcap = (float)(softcap * LOG2E);
+  a.cap_inverse = softcap > 0.0f ? (float)(1.0 / (softcap * LOG2E)) : 0.0f;
   a.window = window;
   a.out = (char*)d_output;
   a.lse = d_lse;

@@ -135,7 +135,18 @@ __device__ __forceinline__ float half_at(uint32_t pair, int i) { return (float)_
 // what byte 128 of a row stands for, by its scale and bias
 __device__ __forceinline__ float middle(uint32_t pair) { return __builtin_fmaf(128.0f, half_at(pair, 0), half_at(pair, 1)); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-// (1 - t) / (1 + t), t = exp(-2 |x|): off by some 2^-23 of 1
+// tanh(x) / x = 1 - x^2/3 + 2 x^4/15 - ..., for |x| < TANH_SMALL to 2^-24 (the next term: 0.0036 x^12)
+constexpr float TANH_SMALL = 0.35f;
+__device__ __forceinline__ float tanh_ratio(float x) {
+  const float z = x * x;
+  float p = -1382.0f / 155925.0f;
+  p = __builtin_fmaf(p, z, 62.0f / 2835.0f);
+  p = __builtin_fmaf(p, z, -17.0f / 315.0f);
+  p = __builtin_fmaf(p, z, 2.0f / 15.0f);
+  p = __builtin_fmaf(p, z, -1.0f / 3.0f);
+  return __builtin_fmaf(p, z, 1.0f);
+}
+// (1 - t) / (1 + t), t = exp(-2 |x|): off by some 2^-23 of 1, so for others than small x
 __device__ __forceinline__ float tanh_fast(float x) {
   const float t = exp2_fast(-2.0f * ATT_LOG2E * __builtin_fabsf(x));
   return __builtin_copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
@@ -524,9 +535,14 @@ struct Attention {
         s[4 * h + j] = y * a.scale;
       }
     }
+    // cap tanh(s / cap): small scores as s times tanh(x) / x, off by some 2^-22 of themselves, not of the cap, which may be
+    // any number. (131 requests of 12 heads, cap 30: 69.2 -> 70.2 us. With the two forms in branches of their own registers spill.)
     if (a.softcap > 0.0f) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = a.softcap * ATT_LOG2E * tanh_fast(s[j]);
+      for (int j = 0; j < 8; ++j) {
+        const float x = s[j] * a.cap_inverse;
+        s[j] = __builtin_fabsf(x) < TANH_SMALL ? s[j] * tanh_ratio(x) : a.softcap * tanh_fast(x);
+      }
     }
     if (partial) {
 #pragma unroll

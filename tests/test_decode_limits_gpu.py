@@ -88,3 +88,20 @@ def test_rows_whose_range_a_single_channel_sets(decode, dim, layout, block, dtyp
         c[..., :4] = torch.cat((scale, -128 * scale), -1).view(torch.uint8)
         values[k] = R.rows8_values(c.cpu().numpy(), dim)
     check(decode, (query, caches, values, tables, lengths), dtype)
+
+
+# ---- caps -------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows8", [False, True])
+@pytest.mark.parametrize("block", [16, 10])
+@pytest.mark.parametrize("softcap", [1e-3, 0.7, 3.0, 30.0, 1e4, 1e6, 1e8, 3e38])
+def test_caps_of_every_size(decode, softcap, block, rows8):
+    check(decode, attention_case(decode, block, 64, 4, 2, block, [0, 1, 40, 300], torch.float16, rows8), torch.float16, softcap=softcap)
+
+
+def test_a_cap_that_no_score_meets_is_none(decode):
+    q, c, _, t, n = attention_case(decode, 3, 128, 4, 2, 16, [1, 77, 500], torch.bfloat16)
+    plain, capped = decode.paged_attention(q, *c, t, n), decode.paged_attention(q, *c, t, n, softcap=1e8)
+    # the scores' roundings alone: some 2^-22 of scores below 8
+    assert (plain[1] - capped[1]).abs().max() < 2.0 ** -18
