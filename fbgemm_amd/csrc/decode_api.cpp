@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 
 #include "../../include/fbgemm_amd.h"
 #include "api_error.h"
@@ -254,8 +255,10 @@ int fbgemm_amd_paged_attention(
   a.block = make_divisor((uint32_t)cache->block_size);
   constexpr double LOG2E = 1.4426950408889634;
   a.scale = (float)(scale * LOG2E);
-  a.softcap = (float)(softcap * LOG2E);
-  a.cap_inverse = softcap > 0.0f ? (float)(1.0 / (softcap * LOG2E)) : 0.0f;
+  // normal and of a finite inverse for the smallest cap too: a score of zero times infinity would be none
+  const double cap = softcap > 0.0f ? std::max(softcap * LOG2E, (double)std::numeric_limits<float>::min()) : 0.0;
+  a.softcap = (float)cap;
+  a.cap_inverse = softcap > 0.0f ? (float)(1.0 / cap) : 0.0f;
   a.window = window;
   a.out = (char*)d_output;
   a.lse = d_lse;

@@ -7,7 +7,9 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cmath>
+#include <limits>
 #include <optional>
 #include <tuple>
 
@@ -143,6 +145,8 @@ std::tuple<Tensor, Tensor> paged_attention(
   TORCH_CHECK(heads <= 0x7fffffff, "fbgemm_amd: too many heads");
   const int64_t bytes = fbgemm_amd_paged_attention_workspace(&cache, B, (int32_t)heads, block_tables.size(1));
   TORCH_CHECK(bytes >= 0, "fbgemm_amd: ", fbgemm_amd_last_error());
+  // a cap below every fp32 number is one all the same: 0 would be none
+  const float cap = softcap == 0.0 ? 0.0f : (float)std::copysign(std::max(std::fabs(softcap), (double)std::numeric_limits<float>::min()), softcap);
   const c10::OptionalDeviceGuard guard(query.device());
   Tensor out = at::empty({B, heads, dim}, query.options());
   Tensor lse = at::empty({B, heads}, query.options().dtype(at::kFloat));
@@ -150,7 +154,7 @@ std::tuple<Tensor, Tensor> paged_attention(
   CHECK_CALL(fbgemm_amd_paged_attention(
       &cache, query.data_ptr(), float_type(query.scalar_type(), "query"), B, (int32_t)heads, stride_of(query, 0), stride_of(query, 1),
       key_cache.data_ptr(), value_cache.data_ptr(), (const int32_t*)block_tables.data_ptr(), stride_of(block_tables, 0), block_tables.size(1),
-      lengths.data_ptr(), index_bits(lengths, "lengths"), (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)dim)), window, (float)softcap,
+      lengths.data_ptr(), index_bits(lengths, "lengths"), (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)dim)), window, cap,
       out.data_ptr(), (float*)lse.data_ptr(), space.data_ptr(), bytes, current_stream(query)));
   return {out, lse};
 }

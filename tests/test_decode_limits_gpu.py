@@ -105,3 +105,15 @@ def test_a_cap_that_no_score_meets_is_none(decode):
     plain, capped = decode.paged_attention(q, *c, t, n), decode.paged_attention(q, *c, t, n, softcap=1e8)
     # the scores' roundings alone: some 2^-22 of scores below 8
     assert (plain[1] - capped[1]).abs().max() < 2.0 ** -18
+
+
+@pytest.mark.parametrize("softcap", [1e-36, 1e-40, 1e-44, 1e-50])
+def test_caps_below_every_score_leave_equal_weights(decode, softcap):
+    """Scores between -softcap and softcap are zero to fp32: every token counts the same, and a score of zero is one of them."""
+    query, caches, values, tables, lengths = attention_case(decode, 5, 64, 2, 1, 16, [1, 50, 200], torch.float16)
+    query[1] = 0
+    out, lse = decode.paged_attention(query, *caches, tables, lengths, softcap=softcap)
+    want, want_lse, off, lse_off = attention64(0 * np64(query), [np.nan_to_num(v, posinf=0) for v in values], [np.abs(np.nan_to_num(v, posinf=0)) for v in values],
+                                               tables.cpu().numpy(), lengths.cpu().numpy(), 1.0)
+    close(out, want, off, torch.float16)
+    close(lse, want_lse, lse_off, torch.float32)
