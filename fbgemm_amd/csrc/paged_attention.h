@@ -473,10 +473,17 @@ struct Attention {
     l = bias = 0.0f;
   }
 
-  // PACKED: a lane's part of the runs, through LDS, where nobody else looks: a wave's writes and reads keep their order
+  // PACKED: a lane's part of the runs, through LDS, where no other wave looks. Lanes read what others wrote: that the wave's
+  // writes and reads keep their order is said to the compiler, for which the addresses of one lane have nothing to do with each other
+  static __device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
   __device__ __forceinline__ void unpack(const Tile& loaded, Rows& rows) const {
     typedef __attribute__((ext_vector_type(4))) uint32_t piece_t;
     if constexpr (PACKED) {
+      wave_sync(); // the last tile's reads, these writes
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -486,6 +493,7 @@ struct Attention {
         }
       if (lane < 16)
         *reinterpret_cast<piece_t*>(stage + (n >> 2) * RUN + RUN_LOADS * 1024 + (n & 3) * 16) = piece_t{loaded.last[0], loaded.last[1], loaded.last[2], loaded.last[3]};
+      wave_sync();
       constexpr int ROW = DP * EL + HEAD;
       const char *keys = stage, *values = stage + 2 * RUN;
 #pragma unroll

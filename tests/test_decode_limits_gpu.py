@@ -117,3 +117,22 @@ def test_caps_below_every_score_leave_equal_weights(decode, softcap):
                                                tables.cpu().numpy(), lengths.cpu().numpy(), 1.0)
     close(out, want, off, torch.float16)
     close(lse, want_lse, lse_off, torch.float32)
+
+
+# ---- tiles behind tiles -----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("layout,block", [("hnd", 16), ("hnd", 64), ("nhd", 16), ("hnd", 24)])
+@pytest.mark.parametrize("rows8", [False, True])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_tiles_of_a_wave(decode, dim, rows8, layout, block, dtype):
+    """64 requests over one context: more steps than the device has workers, so that each wave adds tile behind tile, rows of
+    8 bits through its part of LDS."""
+    longest, requests = 3000, 64
+    query, caches, values, tables, _ = attention_case(decode, dim + block, dim, 4, 4, block, [longest], dtype, rows8, layout)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(block)
+    query = torch.randn((requests, 4, dim), device="cuda", generator=g).to(dtype)
+    lengths = longest - torch.arange(requests, device="cuda") * 11
+    check(decode, (query, caches, values, tables.expand(requests, -1), lengths), dtype)
