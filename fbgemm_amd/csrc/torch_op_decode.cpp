@@ -143,11 +143,11 @@ std::tuple<Tensor, Tensor> paged_attention(
               "fbgemm_amd: block_tables must be int32 [", B, ", blocks], got ", block_tables.scalar_type(), " ", block_tables.sizes());
   rows_dense(block_tables, "block_tables");
   TORCH_CHECK(heads <= 0x7fffffff, "fbgemm_amd: too many heads");
+  const c10::OptionalDeviceGuard guard(query.device()); // sizes go by the current device's compute units
   const int64_t bytes = fbgemm_amd_paged_attention_workspace(&cache, B, (int32_t)heads, block_tables.size(1));
   TORCH_CHECK(bytes >= 0, "fbgemm_amd: ", fbgemm_amd_last_error());
   // a cap below every fp32 number is one all the same: 0 would be none
   const float cap = softcap == 0.0 ? 0.0f : (float)std::copysign(std::max(std::fabs(softcap), (double)std::numeric_limits<float>::min()), softcap);
-  const c10::OptionalDeviceGuard guard(query.device());
   Tensor out = at::empty({B, heads, dim}, query.options());
   Tensor lse = at::empty({B, heads}, query.options().dtype(at::kFloat));
   Tensor space = at::empty({bytes}, query.options().dtype(at::kByte));
