@@ -237,6 +237,12 @@ Tensor penalize_logits_new_meta(
     const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&) {
   return at::empty(logits.sizes(), logits.options());
 }
+Tensor penalize_logits_out_meta(
+    const Tensor& logits, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+    const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, Tensor out) {
+  TORCH_CHECK(out.sizes() == logits.sizes() && out.scalar_type() == logits.scalar_type(), "fbgemm_amd: out must have the logits' shape and type");
+  return out;
+}
 
 } // namespace
 
@@ -265,4 +271,5 @@ TORCH_LIBRARY_IMPL(fbgemm_amd, Meta, m) {
   m.impl("kv_cache_append", TORCH_FN(kv_cache_append_meta));
   m.impl("paged_attention", TORCH_FN(paged_attention_meta));
   m.impl("penalize_logits", TORCH_FN(penalize_logits_new_meta));
+  m.impl("penalize_logits.out", TORCH_FN(penalize_logits_out_meta));
 }
