@@ -284,10 +284,10 @@ int fbgemm_amd_penalize_logits(
   if (tokens_numel < 0 || tokens_numel > MOST || bias_numel < 0 || bias_numel > MOST) return fail(FBGEMM_AMD_E_ARG, "lists must hold fewer than 2^31 entries");
   if (rows == 0 || vocab == 0) return 0;
   if (!d_logits || !d_output) return fail(FBGEMM_AMD_E_ARG, "null data pointer");
-  if (rows > 1 && (logits_stride < vocab || output_stride < vocab)) return fail(FBGEMM_AMD_E_ARG, "rows must not overlap");
+  if (rows > 1 && ((logits_stride != 0 && logits_stride < vocab) || output_stride < vocab)) return fail(FBGEMM_AMD_E_ARG, "rows must not overlap");
   if (tokens_numel > 0 && (!d_tokens || !d_offsets)) return fail(FBGEMM_AMD_E_ARG, "tokens need their offsets");
   if (bias_numel > 0 && (!d_bias_ids || !d_bias_values || !d_bias_offsets)) return fail(FBGEMM_AMD_E_ARG, "biases need ids, values and offsets");
-  if (d_mask && rows > 1 && mask_stride < (vocab + 31) / 32) return fail(FBGEMM_AMD_E_ARG, "a row of the mask has one bit per token of the vocabulary");
+  if (d_mask && rows > 1 && mask_stride != 0 && mask_stride < (vocab + 31) / 32) return fail(FBGEMM_AMD_E_ARG, "a row of the mask has one bit per token of the vocabulary");
   LogitsArgs a;
   a.logits = d_logits;
   a.out = d_output;

@@ -101,7 +101,8 @@ def penalize_logits(logits, tokens=None, offsets=None, prompt_lengths=None, repe
     its prompt's. ``repetition``, ``frequency``, ``presence``: fp32 ``[rows]``, or None for none. A token of the list is
     divided by ``repetition`` (multiplied where it is not positive), one that was said behind the prompt loses ``frequency``
     for every time and ``presence`` once. ``bias_ids``, ``bias_values``, ``bias_offsets``: added to single tokens (of several
-    for one the last counts). ``mask``: int32 ``[rows, ceil(vocab / 32)]``, a token whose bit is 0 becomes -inf.
+    for one the last counts). ``mask``: int32 ``[rows, ceil(vocab / 32)]``, a token whose bit is 0 becomes -inf;
+    one row of it may be expanded over all.
 
     In fp32, rounded once. Returns a new tensor, or ``out``, which may be ``logits``."""
     if out is None:

@@ -136,3 +136,23 @@ def test_many_tiles_of_a_wave(decode, dim, rows8, layout, block, dtype):
     query = torch.randn((requests, 4, dim), device="cuda", generator=g).to(dtype)
     lengths = longest - torch.arange(requests, device="cuda") * 11
     check(decode, (query, caches, values, tables.expand(requests, -1), lengths), dtype)
+
+
+# ---- operands that rows share, results over inputs ---------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_and_masks_that_all_rows_share(decode, dtype):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    rows, vocab = 5, 9001
+    one = torch.randn((1, vocab), device="cuda", generator=g).to(dtype)
+    words = torch.randint(-(1 << 31), 1 << 31, (1, (vocab + 31) // 32), device="cuda", generator=g).to(torch.int32)
+    tokens = torch.randint(0, vocab, (rows * 40,), device="cuda", generator=g)
+    offsets = torch.arange(rows + 1, device="cuda") * 40
+    penalty = torch.rand(rows, device="cuda", generator=g)
+    call = lambda x, m: decode.penalize_logits(x, tokens, offsets, frequency=penalty, mask=m)  # noqa: E731
+    want = call(one.repeat(rows, 1), words.repeat(rows, 1))
+    assert torch.equal(call(one.expand(rows, -1), words.repeat(rows, 1)), want)
+    assert torch.equal(call(one.repeat(rows, 1), words.expand(rows, -1)), want)
+    assert torch.equal(call(one.expand(rows, -1), words.expand(rows, -1)), want)
