@@ -49,6 +49,15 @@ int check_cache(const fbgemm_amd_paged_cache* c) {
   return 0;
 }
 
+// rows of a cache that is written: of two, neither reaches into the other
+bool rows_apart(const fbgemm_amd_paged_cache& c, const int64_t (&strides)[3]) {
+  const int64_t row = c.row_ty == ST_INT8 ? cache_row_bytes(c) : c.dim;
+  const int64_t size[3] = {c.blocks, c.heads, c.block_size};
+  for (int k = 0; k < 3; ++k)
+    if (size[k] > 1 && strides[k] < row) return false;
+  return true;
+}
+
 CacheRows rows_of(void* base, const int64_t (&strides)[3], int32_t ty) {
   const int64_t e = storage_bytes(ty);
   return CacheRows{(char*)base, strides[0] * e, strides[1] * e, strides[2] * e};
@@ -181,8 +190,15 @@ int fbgemm_amd_kv_cache_append(
   a.block = make_divisor((uint32_t)cache->block_size);
   a.per_row = make_divisor(1);
   a.status = (Status*)d_status;
+  // one cache for both holds the same rows twice, or which of the two is left to chance
+  const auto check_shared = [&]() -> int {
+    const bool same = d_key == d_value && key_strides[0] == value_strides[0] && key_strides[1] == value_strides[1];
+    return d_key_cache == d_value_cache && cache->blocks > 0 && !same ? fail(FBGEMM_AMD_E_ARG, "keys and values that differ must not overlap in the cache") : 0;
+  };
+  if (!rows_apart(*cache, cache->key_strides) || !rows_apart(*cache, cache->value_strides)) return fail(FBGEMM_AMD_E_ARG, "rows of a cache must not overlap");
   if (rows8) {
     if ((uintptr_t)d_key_cache % 4 || (uintptr_t)d_value_cache % 4) return fail(FBGEMM_AMD_E_ARG, "8-bit rows begin on 4-byte boundaries");
+    if (int rc = check_shared()) return rc;
     const bool aligned16 = (uintptr_t)d_key % 16 == 0 && (uintptr_t)d_value % 16 == 0 &&
         divides(16, {a.token_stride[0], a.head_stride[0], a.token_stride[1], a.head_stride[1]});
     HIP_TRY(launch_kv_append_rows8(a, input_ty, aligned16, (hipStream_t)stream));
@@ -199,6 +215,7 @@ int fbgemm_amd_kv_cache_append(
   };
   while (piece > 2 && !fits(piece)) piece >>= 1;
   if (!fits(piece)) return fail(FBGEMM_AMD_E_ARG, "rows are not aligned to their elements");
+  if (int rc = check_shared()) return rc;
   a.per_row = make_divisor((uint32_t)(a.row_bytes / piece));
   HIP_TRY(launch_kv_append(a, piece, (hipStream_t)stream));
   return 0;

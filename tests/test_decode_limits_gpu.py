@@ -156,3 +156,31 @@ def test_logits_and_masks_that_all_rows_share(decode, dtype):
     assert torch.equal(call(one.expand(rows, -1), words.repeat(rows, 1)), want)
     assert torch.equal(call(one.repeat(rows, 1), words.expand(rows, -1)), want)
     assert torch.equal(call(one.expand(rows, -1), words.expand(rows, -1)), want)
+
+
+def test_caches_whose_rows_are_one_are_refused(decode):
+    new = torch.randn((3, 2, 64), device="cuda").bfloat16()
+    slots = torch.arange(3, device="cuda")
+    whole = lambda: torch.zeros((4, 2, 16, 64), device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    shared = [whole()[:1].expand(4, -1, -1, -1), whole()[:, :1].expand(-1, 2, -1, -1), whole()[:, :, :1].expand(-1, -1, 16, -1)]
+    for cache in shared:
+        with pytest.raises(RuntimeError, match="overlap"):
+            decode.kv_cache_append(new, new, cache, whole(), slots)
+        with pytest.raises(RuntimeError, match="overlap"):
+            decode.kv_cache_append(new, new, whole(), cache, slots)
+    same = whole()
+    with pytest.raises(RuntimeError, match="overlap"):
+        decode.kv_cache_append(new, 2 * new, same, same, slots)
+    decode.kv_cache_append(new, new, same, same, slots)  # one row for both
+    assert torch.equal(same[0, :, :3], new.transpose(0, 1))
+    # keys and values side by side in one tensor are two caches
+    both = torch.zeros((4, 2, 2, 16, 64), device="cuda", dtype=torch.bfloat16)
+    decode.kv_cache_append(new, 2 * new, both[:, 0], both[:, 1], slots)
+    assert torch.equal(both[0, 0, :, :3], new.transpose(0, 1)) and torch.equal(both[0, 1, :, :3], 2 * new.transpose(0, 1))
+    # reading rows that are one is nobody's harm
+    q = torch.randn((1, 2, 64), device="cuda").bfloat16()
+    table, length = torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.tensor([16], device="cuda")
+    kv = torch.randn((1, 1, 16, 64), device="cuda").bfloat16()
+    got = decode.paged_attention(q, kv.expand(-1, 2, -1, -1), kv.expand(-1, 2, -1, -1), table, length)
+    want = decode.paged_attention(q, kv.repeat(1, 2, 1, 1), kv.repeat(1, 2, 1, 1), table, length)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -1,10 +1,11 @@
 """What the decoding-step operators promise beside their results, without a GPU."""
+import ctypes as C
 import os
 import re
 
 import pytest
 
-from test_decode_host import decode  # noqa: F401  (a fixture)
+from test_decode_host import P, cache, decode, lib, refused  # noqa: F401  (decode, lib: fixtures)
 
 torch = pytest.importorskip("torch")
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fbgemm_amd", "csrc")
@@ -29,3 +30,17 @@ def test_sizes_are_asked_of_the_tensors_device():
     for body in guarded:
         calls = [m.start() for m in re.finditer(r"\bfbgemm_amd_\w+\(", body)]
         assert calls and body.index("OptionalDeviceGuard") < min(calls), body[:80]
+
+
+def test_caches_whose_rows_overlap_are_refused(lib):  # noqa: F811
+    def call(c=None, kc=P, vc=C.c_void_p(1 << 20)):
+        s = (C.c_int64 * 2)(128, 64)
+        return lib.fbgemm_amd_kv_cache_append(C.byref(c or cache()), P, C.c_void_p(8192), 5, 3, s, s, P, kc, vc, None, None)
+    for k in range(3):
+        for step in (0, 32):
+            strides = [2048, 1024, 64]
+            strides[k] = step
+            refused(lib, call(cache(key_strides=tuple(strides))), "overlap")
+            refused(lib, call(cache(value_strides=tuple(strides))), "overlap")
+    refused(lib, call(vc=P), "overlap")
+    refused(lib, call(cache(row_ty=2, key_strides=(2176, 1088, 64), value_strides=(2176, 1088, 68))), "overlap")
