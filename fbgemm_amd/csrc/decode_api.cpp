@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 #include <limits>
+#include <numeric>
 
 #include "../../include/fbgemm_amd.h"
 #include "api_error.h"
@@ -56,6 +57,17 @@ bool rows_apart(const fbgemm_amd_paged_cache& c, const int64_t (&strides)[3]) {
   for (int k = 0; k < 3; ++k)
     if (size[k] > 1 && strides[k] < row) return false;
   return true;
+}
+
+// Two arrays of rows of `width` bytes, `stride_a` and `stride_b` apart, that share a byte (or may, where neither stride divides the other)
+bool rows_meet(const void* a, int64_t stride_a, const void* b, int64_t stride_b, int64_t rows, int64_t width) {
+  typedef __int128 wide; // strides are the caller's
+  const wide d = (wide)(uintptr_t)b - (wide)(uintptr_t)a, last_a = (wide)(rows - 1) * stride_a + width, last_b = (wide)(rows - 1) * stride_b + width;
+  if (d >= last_a || -d >= last_b) return false;
+  const int64_t every = std::gcd(stride_a, stride_b);
+  if (rows == 1 || every == 0) return true;
+  const wide r = (d % every + every) % every;
+  return r < width || every - r < width;
 }
 
 CacheRows rows_of(void* base, const int64_t (&strides)[3], int32_t ty) {
@@ -305,6 +317,10 @@ int fbgemm_amd_penalize_logits(
   if (tokens_numel > 0 && (!d_tokens || !d_offsets)) return fail(FBGEMM_AMD_E_ARG, "tokens need their offsets");
   if (bias_numel > 0 && (!d_bias_ids || !d_bias_values || !d_bias_offsets)) return fail(FBGEMM_AMD_E_ARG, "biases need ids, values and offsets");
   if (d_mask && rows > 1 && mask_stride != 0 && mask_stride < (vocab + 31) / 32) return fail(FBGEMM_AMD_E_ARG, "a row of the mask has one bit per token of the vocabulary");
+  const int64_t e = storage_bytes(logits_ty);
+  const bool in_place = d_output == d_logits && (rows == 1 || output_stride == logits_stride);
+  if (!in_place && rows_meet(d_logits, rows > 1 ? logits_stride * e : 0, d_output, rows > 1 ? output_stride * e : 0, rows, vocab * e))
+    return fail(FBGEMM_AMD_E_ARG, "the result may be the logits themselves, but must not overlap them otherwise");
   LogitsArgs a;
   a.logits = d_logits;
   a.out = d_output;

@@ -197,8 +197,6 @@ Tensor penalize_logits(
   on_device(out, logits, "out");
   TORCH_CHECK(out.sizes() == logits.sizes() && out.scalar_type() == logits.scalar_type(), "fbgemm_amd: out must have the logits' shape and type");
   rows_dense(out, "out");
-  TORCH_CHECK(out.data_ptr() != logits.data_ptr() || rows <= 1 || out.stride(0) == logits.stride(0),
-              "fbgemm_amd: out over the logits must have their strides");
   CHECK_CALL(fbgemm_amd_penalize_logits(
       logits.data_ptr(), ty, rows, vocab, rows > 1 ? logits.stride(0) : vocab, pointer(tokens), tokens.has_value() ? tokens->numel() : 0,
       pointer(offsets), pointer(prompt_lengths), index == at::kLong ? 64 : 32, (const float*)pointer(repetition), (const float*)pointer(frequency),

@@ -660,7 +660,7 @@ int fbgemm_amd_paged_attention(
  * (id, value) per row like the tokens' (all lists have index_bits), the mask one bit
  * per token, bit v % 32 of word v / 32 of a row (mask_stride words apart). With a stride
  * of 0 all rows share the logits, or the mask. d_output may be d_logits (with the same
- * stride, not 0). */
+ * stride, not 0); rows of the two that overlap otherwise are refused. */
 int fbgemm_amd_penalize_logits(
     const void* d_logits, int32_t logits_ty, int64_t rows, int64_t vocab, int64_t logits_stride, const void* d_tokens,
     int64_t tokens_numel, const void* d_offsets, const void* d_prompt_lengths, int32_t index_bits, const float* d_repetition,

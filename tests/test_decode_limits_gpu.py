@@ -158,6 +158,25 @@ def test_logits_and_masks_that_all_rows_share(decode, dtype):
     assert torch.equal(call(one.expand(rows, -1), words.expand(rows, -1)), want)
 
 
+def test_logits_beside_their_result_in_one_tensor(decode):
+    """Columns, rows and ends of one tensor that do not meet are fine; logits and results that share elements are refused, but the
+    same elements of both."""
+    both = torch.randn((4, 2100), device="cuda")
+    left, right = both[:, :1000], both[:, 1000:2000]
+    penalty = torch.full((4,), 0.5, device="cuda")
+    tokens, offsets = torch.arange(40, device="cuda"), torch.arange(5, device="cuda") * 10
+    call = lambda x, out=None: decode.penalize_logits(x, tokens, offsets, presence=penalty, out=out)  # noqa: E731
+    want = call(left)
+    assert torch.equal(call(left, right), want) and torch.equal(right, want)
+    rows = torch.randn((8, 2100), device="cuda")  # ends of rows beside the beginnings of others
+    want = call(rows[:4, 1000:2000])
+    assert torch.equal(call(rows[:4, 1000:2000], rows[2:6, :1000]), want)
+    for logits, out in ((left, both[:, 1:1001]), (left, both[:, 999:1999]), (both[:, 500:1500], both[:, 1100:]), (rows[:4, :1000], rows[3:7, :1000]),
+                        (left[:1].expand(4, -1), left), (left, right[:1].expand(4, -1)), (left[:1], both[:1, 7:1007])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            decode.penalize_logits(logits, out=out)
+
+
 def test_caches_whose_rows_are_one_are_refused(decode):
     new = torch.randn((3, 2, 64), device="cuda").bfloat16()
     slots = torch.arange(3, device="cuda")

@@ -44,3 +44,15 @@ def test_caches_whose_rows_overlap_are_refused(lib):  # noqa: F811
             refused(lib, call(cache(value_strides=tuple(strides))), "overlap")
     refused(lib, call(vc=P), "overlap")
     refused(lib, call(cache(row_ty=2, key_strides=(2176, 1088, 64), value_strides=(2176, 1088, 68))), "overlap")
+
+
+def test_logits_whose_result_overlaps_them_are_refused(lib):  # noqa: F811
+    at = lambda elements: C.c_void_p(1 << 20 | 4 * elements)  # noqa: E731
+    def call(logits, out, stride=100, ostride=100, rows=2, vocab=100, mask=None, words=4):
+        return lib.fbgemm_amd_penalize_logits(logits, 0, rows, vocab, stride, None, 0, None, None, 64, None, None, None, None, None, 0, None, mask, words,
+                                              out, ostride, None)
+    for change in ({"out": at(1)}, {"out": at(199)}, {"out": at(100)}, {"logits": at(50)}, {"out": at(0), "ostride": 101}, {"out": at(0), "stride": 0},
+                   {"out": at(1), "rows": 1, "stride": 0, "ostride": 0}, {"out": at(150), "stride": 250, "ostride": 250, "vocab": 101, "logits": at(50)},
+                   {"out": at(950), "ostride": 0}):
+        refused(lib, call(**{"logits": at(0), "out": at(0), **change}), "overlap")
+    refused(lib, call(at(0), at(0), mask=P, words=3), "mask")
