@@ -18,6 +18,8 @@
 // tokens, 48 with biases and a mask too, by then bound by vector instructions. Tried: copying all under
 // the mask first and writing the named ones again (99), counts and biases in one word (49), a list of
 // the named ones made from what the counts' atomics return (58).
+#include <type_traits>
+
 #include "decode.h"
 
 namespace fbgemm_amd {
@@ -222,14 +224,37 @@ __global__ __launch_bounds__(THREADS) void penalize_logits_kernel(const LogitsAr
   }
 }
 
+// the same from a later row on
+LogitsArgs rows_from(LogitsArgs a, int64_t row, int64_t element_bytes, int64_t index_bytes) {
+  const auto later = [&](auto*& p, int64_t bytes) {
+    if (p) p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(reinterpret_cast<uintptr_t>(p) + row * bytes);
+  };
+  later(a.logits, a.logits_stride * element_bytes);
+  later(a.out, a.out_stride * element_bytes);
+  later(a.offsets, index_bytes);
+  later(a.prompt_lengths, index_bytes);
+  later(a.bias_offsets, index_bytes);
+  later(a.repetition, sizeof(float));
+  later(a.frequency, sizeof(float));
+  later(a.presence, sizeof(float));
+  later(a.mask, a.mask_stride * (int64_t)sizeof(uint32_t));
+  a.rows -= row;
+  return a;
+}
+
 template <int TY, int THREADS, int PIECES>
-hipError_t launch_shape(const LogitsArgs& a, bool idx64, hipStream_t stream) {
-  constexpr int CHUNK = THREADS * PIECES * Piece<TY>::N;
-  const int64_t grid = (a.vocab + CHUNK - 1) / CHUNK * a.rows;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  if (idx64) penalize_logits_kernel<TY, int64_t, THREADS, PIECES><<<(unsigned)grid, THREADS, 0, stream>>>(a);
-  else penalize_logits_kernel<TY, int32_t, THREADS, PIECES><<<(unsigned)grid, THREADS, 0, stream>>>(a);
-  return hipGetLastError();
+hipError_t launch_shape(const LogitsArgs& all, bool idx64, hipStream_t stream) {
+  constexpr int64_t CHUNK = THREADS * PIECES * Piece<TY>::N;
+  const int64_t chunks = (all.vocab + CHUNK - 1) / CHUNK;
+  const int64_t most = 0xffffffffll / THREADS / chunks; // rows of a launch: fewer than 2^32 threads
+  for (int64_t row = 0; row < all.rows; row += most) {
+    const LogitsArgs a = rows_from(all, row, Piece<TY>::BYTES, idx64 ? 8 : 4);
+    const unsigned grid = (unsigned)(chunks * (a.rows < most ? a.rows : most));
+    if (idx64) penalize_logits_kernel<TY, int64_t, THREADS, PIECES><<<grid, THREADS, 0, stream>>>(a);
+    else penalize_logits_kernel<TY, int32_t, THREADS, PIECES><<<grid, THREADS, 0, stream>>>(a);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 template <int TY>
 hipError_t launch(const LogitsArgs& a, bool idx64, hipStream_t stream) {

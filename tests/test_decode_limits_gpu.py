@@ -203,3 +203,24 @@ def test_caches_whose_rows_are_one_are_refused(decode):
     got = decode.paged_attention(q, kv.expand(-1, 2, -1, -1), kv.expand(-1, 2, -1, -1), table, length)
     want = decode.paged_attention(q, kv.repeat(1, 2, 1, 1), kv.repeat(1, 2, 1, 1), table, length)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_as_many_rows_of_logits_as_there_may_be(decode):
+    """More than one grid holds: the last rows are those of a second launch, with their own penalties, lists and mask."""
+    rows = 1 << 24
+    x = torch.arange(rows, device="cuda", dtype=torch.int32).bitwise_and_(1023).half().view(rows, 1)
+    x[-3:] = 8
+    value = lambda *last: torch.cat((torch.ones(rows - 3, device="cuda"), torch.tensor(last, device="cuda")))  # noqa: E731
+    repetition, frequency, presence = value(1.0, 2.0, 4.0), value(1.0, 0.5, 0.25), value(2.0, 0.25, 0.5)
+    mask = torch.full((rows, 1), -1, dtype=torch.int32, device="cuda")
+    mask[-3] = 0
+    offsets = torch.zeros(rows + 1, dtype=torch.int32, device="cuda")
+    offsets[-3:] = torch.tensor([1, 2, 4], device="cuda", dtype=torch.int32)  # a token of each of the last three rows, two of the last
+    prompts = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    prompts[-1] = 1  # its first is its prompt's
+    zeros = torch.zeros(4, dtype=torch.int32, device="cuda")
+    got = decode.penalize_logits(x, zeros, offsets, prompts, repetition=repetition, frequency=frequency, presence=presence,
+                                 bias_ids=zeros, bias_values=torch.tensor([1.0, 3.0, 5.0, 7.0], device="cuda"), bias_offsets=offsets, mask=mask)
+    want = x.clone()
+    want[-3], want[-2], want[-1] = -float("inf"), 8 / 2 - 0.5 - 0.25 + 3, 8 / 4 - 0.25 - 0.5 + 7
+    assert torch.equal(got, want)
