@@ -75,7 +75,8 @@ def kv_cache_append(key, value, key_cache, value_cache, slots, status=None):
     fp32, fp16 and bf16 caches take rows of their own type as they are; a uint8 cache takes any of the three and holds
     what ``ops.quantize_rowwise(rows, 8, layout=QLAYOUT_TBE)`` makes of them (elements beyond fp16's range at its end, NaN as 0).
     A token of slot -1 is skipped, and one whose slot the cache does not have: that one is recorded in ``status``
-    (``ERR_INDEX_OUT_OF_RANGE`` and its number). Key and value may be slices of a fused projection's output."""
+    (``ERR_INDEX_OUT_OF_RANGE`` and its number). Slots differ from each other, but for -1: what a slot holds that several tokens have
+    is a mixture of theirs. Key and value may be slices of a fused projection's output; the caches' rows must not overlap."""
     _append(key, value, key_cache, value_cache, slots, None if status is None else status.buf)
 
 

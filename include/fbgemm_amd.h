@@ -617,8 +617,10 @@ typedef struct fbgemm_amd_paged_cache {
  * (bit_rate 8, sb_float 0, FBGEMM_AMD_QLAYOUT_TBE) makes of them, with elements beyond
  * fp16's range at its end and NaN as 0 (a zero bias may have either sign). Slot -1 is
  * skipped; another slot outside the cache too, and is recorded in d_status (may be
- * NULL) as INDEX_OUT_OF_RANGE with the token's number. Of several tokens with one slot
- * any one is stored. */
+ * NULL) as INDEX_OUT_OF_RANGE with the token's number. Slots differ from each other
+ * (but for -1): a slot that several tokens have ends as a mixture of their rows, which
+ * are written by many threads in no order; no other slot is touched. Rows of the cache
+ * must not overlap. */
 int fbgemm_amd_kv_cache_append(
     const fbgemm_amd_paged_cache* cache, const void* d_key, const void* d_value, int32_t input_ty, int64_t tokens,
     const int64_t* key_strides, const int64_t* value_strides, const int64_t* d_slots, void* d_key_cache, void* d_value_cache,
