@@ -586,6 +586,8 @@ int fbgemm_amd_rowwise_prune_gather(const void* d_weights, int64_t rows, int64_t
  * number d_offsets[r] + k of the step, its position is d_lengths[r] + k, its slot
  * table[position / block_size] * block_size + position % block_size, or -1 where
  * there is no block for it (table too narrow, free list exhausted, a negative entry).
+ * Positions count from the table's room where a request holds more than that: from
+ * table_width * block_size on they are no tokens' places, and their slots are -1.
  * d_slots and d_positions hold num_tokens entries: those behind the last token are -1
  * and 0; tokens beyond num_tokens get none. d_total_lengths = lengths + new tokens.
  * Called again with the same inputs it writes the same. d_status (may be NULL: then
