@@ -64,7 +64,9 @@ def kv_block_tables(lengths, new_tokens, block_tables, free_blocks, free_start, 
     ``block_tables`` are left as they are, so the same call gives the same again.
 
     ``status`` records ``ERR_NEGATIVE_LENGTH`` (counted as 0), ``ERR_BAG_OVERRUN`` (a table too narrow for its tokens),
-    ``ERR_OUT_OF_BLOCKS`` and ``ERR_LENGTH_MISMATCH`` (``num_tokens`` is not the sum)."""
+    ``ERR_OUT_OF_BLOCKS`` and ``ERR_LENGTH_MISMATCH`` (``num_tokens`` is not the sum). A step that is padded on purpose records the
+    last too: it is told from a list that was cut by ``offsets[-1]``, which is below ``num_tokens`` then. Positions of a request that
+    holds more than its table has room for count from the table's room; their slots are -1."""
     return BlockTables._make(_block_tables(lengths, new_tokens, block_tables, free_blocks, free_start, block_size, num_tokens,
                                            None if status is None else status.buf))
 

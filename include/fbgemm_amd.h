@@ -592,7 +592,9 @@ int fbgemm_amd_rowwise_prune_gather(const void* d_weights, int64_t rows, int64_t
  * and 0; tokens beyond num_tokens get none. d_total_lengths = lengths + new tokens.
  * Called again with the same inputs it writes the same. d_status (may be NULL: then
  * the entries say it all): NEGATIVE_LENGTH (counted as 0), BAG_OVERRUN (a table too
- * narrow), OUT_OF_BLOCKS, LENGTH_MISMATCH (the new tokens' sum is not num_tokens).
+ * narrow), OUT_OF_BLOCKS, LENGTH_MISMATCH (the new tokens' sum is not num_tokens: set
+ * by a step that is padded on purpose too, whose d_offsets[requests] is below
+ * num_tokens; of a list that is cut it is num_tokens).
  * d_free_next must not be d_free_start, nor d_total_lengths d_lengths. */
 int fbgemm_amd_kv_block_tables(
     const void* d_lengths, const void* d_new_tokens, int32_t index_bits, int64_t requests, int32_t* d_block_tables,
