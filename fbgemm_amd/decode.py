@@ -92,7 +92,8 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
 
     Returns the outputs (the queries' type and shape) and the logarithm of each softmax's sum (fp32 ``[requests,
     query_heads]``), by which results over several caches can be joined. Tokens of a block that the cache does not have
-    are left out; where none is left the output is 0 and the logarithm -inf."""
+    are left out; where none is left the output is 0 and the logarithm -inf. Rows without a token are never looked at for their
+    contents; a token's NaN reaches its queries' outputs, a score of -inf weighs nothing."""
     return _attention(query, key_cache, value_cache, block_tables, lengths, scale, window, softcap)
 
 

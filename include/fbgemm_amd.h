@@ -639,8 +639,10 @@ int fbgemm_amd_kv_cache_append(
  *   d_output [requests][query_heads][dim] (the queries' type, dense) = softmax(s) v,
  *   d_lse [requests][query_heads] = log(sum_t exp(s_t)).
  * Tokens of a block outside [0, blocks) are left out; where no token is left the output
- * is 0 and d_lse -inf. What the cache holds where no token is may be anything; a
- * token's key or value that is not finite makes its queries' outputs not finite. A
+ * is 0 and d_lse -inf. What the cache holds where no token is may be anything. A score
+ * of NaN, or of +inf without a cap, and a value that is not finite make their queries'
+ * outputs not finite; a score of -inf weighs 0. Tokens of a block are less than 64 MiB
+ * apart. A
  * cache of FP16 / BF16 rows must have the queries' type and rows on 16-byte boundaries,
  * one of INT8 rows goes with either. dim: a multiple of 8, at most 256;
  * requests * heads * table_width * block_size below some 2^37. Scores, weights

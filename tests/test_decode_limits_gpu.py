@@ -224,3 +224,37 @@ def test_as_many_rows_of_logits_as_there_may_be(decode):
     want = x.clone()
     want[-3], want[-2], want[-1] = -float("inf"), 8 / 2 - 0.5 - 0.25 + 3, 8 / 4 - 0.25 - 0.5 + 7
     assert torch.equal(got, want)
+
+
+# ---- numbers that are not finite --------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("block", [16, 10])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_of_tokens_that_are_not_finite(decode, dtype, block):
+    """A score of -inf weighs nothing, one of +inf or NaN, and a value that is not finite, reach the outputs; a cap makes +inf a number."""
+    def run(softcap=0.0):
+        return decode.paged_attention(query, *caches, tables, lengths, softcap=softcap)
+    query, caches, _, tables, lengths = attention_case(decode, block, 64, 2, 1, block, [200, 90], dtype, poison=False)
+    query[:, :, 0] = 1
+    page, place = tables[0, 30 // block].long(), 30 % block
+    key, value = caches[0][page, 0, place], caches[1][page, 0, place]
+    held, kept = key.clone(), value.clone()
+    fine = run()
+    key[0] = -float("inf")
+    without = run()
+    assert all(torch.isfinite(x).all() for x in without) and not torch.equal(without[0][0], fine[0][0])
+    value[5] = float("nan")
+    out, lse = run()
+    assert torch.isnan(out[0, :, 5]).all() and torch.isfinite(out[0, :, 6:]).all() and torch.equal(lse, without[1])
+    value.copy_(kept)
+    key[0] = float("inf")
+    out, lse = run()
+    assert not torch.isfinite(out[0]).any()
+    out, lse = run(softcap=20.0)
+    assert torch.isfinite(out).all() and (lse[0] >= 20).all() and (lse[0] < 21).all()  # one score of 20 among others of a few units
+    key.copy_(held)
+    key[3] = float("nan")
+    for got in (run(), run(softcap=20.0)):
+        assert torch.isnan(got[0][0]).all() and torch.isnan(got[1][0]).all()
+        assert torch.isfinite(got[0][1]).all() and torch.isfinite(got[1][1]).all()  # the other request's tokens are others
