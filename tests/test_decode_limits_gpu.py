@@ -4,7 +4,7 @@ import pytest
 
 import decode_reference as R
 from test_decode_finite_gpu import close_and_finite as close
-from test_decode_gpu import attention_case, np64
+from test_decode_gpu import EDGES, attention_case, make_cache, np64
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -258,3 +258,42 @@ def test_attention_of_tokens_that_are_not_finite(decode, dtype, block):
     for got in (run(), run(softcap=20.0)):
         assert torch.isnan(got[0][0]).all() and torch.isnan(got[1][0]).all()
         assert torch.isfinite(got[0][1]).all() and torch.isfinite(got[1][1]).all()  # the other request's tokens are others
+
+
+# ---- instances of the kernels that other files' shapes do not reach ----------------------------------
+
+
+@pytest.mark.parametrize("rows8", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("block", [7, 16, 24])
+@pytest.mark.parametrize("dim", [8, 56, 72, 80, 96, 120, 136, 200, 248])
+def test_dims_between_in_pages_of_any_size(decode, dim, block, dtype, rows8):
+    check(decode, attention_case(decode, dim + block, dim, 6, 2, block, [0, 1, 40, 133, 300], dtype, rows8), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("layout,block", [("nhd", 16), ("padded", 32), ("padded", 10)])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_rows_of_8_bits_with_gaps_at_the_edges_of_tiles_and_pages(decode, dim, layout, block, dtype):
+    check(decode, attention_case(decode, dim + block, dim, 4, 2, block, EDGES, dtype, True, layout), dtype)
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("layout", ["hnd", "nhd", "padded"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [1, 2, 7, 30, 64, 100, 264, 512, 520])
+def test_append_quantizes_rows_of_any_length_from_any_address(decode, dim, dtype, layout, shift):
+    from fbgemm_amd import ops
+    tokens, heads, block = 37, 3, 5
+    g = torch.Generator(device="cuda")
+    g.manual_seed(dim)
+    blocks, row = -(-tokens // block) + 1, decode.kv_row_bytes(dim)
+    wide = (torch.randn((tokens, 2 * heads, dim + 8), device="cuda", generator=g) - 0.25).to(dtype)
+    key, value = wide[:, :heads, shift:shift + dim], wide[:, heads:, shift:shift + dim]
+    kc, vc = (make_cache(blocks, heads, block, row, torch.uint8, layout, fill=9) for _ in range(2))
+    slots = torch.randperm(blocks * block, device="cuda", generator=g)[:tokens]
+    decode.kv_cache_append(key, value, kc, vc, slots)
+    for new, cache in ((key, kc), (value, vc)):
+        want = torch.full((blocks * block, heads, row), 9, dtype=torch.uint8, device="cuda")
+        want[slots, :, : dim + 4] = ops.quantize_rowwise(new.float().reshape(-1, dim), 8, layout=ops.QLAYOUT_TBE).view(tokens, heads, dim + 4)
+        assert torch.equal(cache, want.view(blocks, block, heads, row).permute(0, 2, 1, 3))
