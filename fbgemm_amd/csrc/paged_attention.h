@@ -6,9 +6,9 @@
 // in one pass over the tokens with the running m and sum, all in fp32 (exp as exp2 of s * log2 e).
 //
 // Bound by memory: every row of the cache is read once for up to 16 queries that share its head (more
-// read it once per 16). 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, bf16: 674 us,
-// 6.39 TB/s; 64 requests of 1 to 4 096, 32 queries on 8: 92 us, 5.87 TB/s; one of 262 143 in 8-bit rows:
-// 102 us, 5.4 TB/s; one of 500: 9.7 us, launches and a chain of dependent steps. That the rows need no staging in LDS, no transposition through it and no exchange between lanes
+// read it once per 16). 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, bf16: 677 us,
+// 6.37 TB/s; 64 requests of 1 to 4 096, 32 queries on 8: 92 us, 5.87 TB/s; one of 262 143 in 8-bit rows:
+// 103 us, 5.4 TB/s; one of 500: 10.3 us, launches and a chain of dependent steps. That the rows need no staging in LDS, no transposition through it and no exchange between lanes
 // is what the operand layouts of the 16x16x32 products give, written here as l = 16 g + n:
 //   keys     A = K [token n][8 of dim], B = Q^T [8 of dim][query n]: C holds tokens 4g .. 4g+3 of query n
 //   values   A = V^T [a column][8 tokens], B = P^T [8 tokens][query n]: a product sums over tokens in any
@@ -103,7 +103,7 @@ __device__ __forceinline__ void split(const float (&p)[8], uint4& hi, uint4& lo)
 }
 
 // Bytes with their top bits flipped are byte - 128 in two's complement. Four at a time, and the compiler is kept from doing it
-// byte by byte: then each is one conversion of a signed byte in place, as without (else a third instruction each).
+// byte by byte: then each is one conversion of a signed byte in place, as for plain bytes (else there is a third instruction for each).
 __device__ __forceinline__ uint32_t centre(uint32_t bytes) {
   bytes ^= 0x80808080u;
   asm("" : "+v"(bytes));
@@ -168,7 +168,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const char* p, bool an
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, any ? 0x7fffffff : 0, 0x00027000);
 }
 // Rows of 16-bit numbers are read once, in whole lines, and marked so (non-temporal): 256 requests of 16 to 8 192 tokens,
-// 64 queries on 8 heads of 128, 738 -> 663 us. A line of 8-bit rows takes several loads, which then miss it (262 143 tokens
+// 64 queries on 8 heads of 128, 738 -> 677 us. A line of 8-bit rows takes several loads, which then miss it (262 143 tokens
 // 110 -> 171 us), and the halves of a line that a key of 64 numbers is loaded in do, a little.
 constexpr int READ_ONCE = 2;
 template <int AUX, int N>
@@ -232,8 +232,8 @@ __device__ __forceinline__ uint32_t inclusive_sum(uint32_t v, int lane) {
 // columns behind read the row's first ones in their place, which meet zeros in the queries or make outputs that nobody wants.
 // PAGE16: pages are whole 16-token tiles, whose addresses are then the same for the wave. PACKED (FULL 8-bit rows, PAGE16): the
 // rows of a page's tokens follow each other without gaps. 16 of them are then read as one run of bytes, every line by one
-// load and marked as read once, and go through LDS, where a lane finds its pieces: 262 143 tokens 102 us, 110 without
-// (two tiles ahead instead of one: 104); 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, 408 us, 464 without.
+// load and marked as read once, and go through LDS, where a lane finds its pieces: 262 143 tokens 103 us, 118 with a gap
+// of 4 bytes behind each row (two tiles ahead instead of one: 2 % more); 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, 400 us, 459 with gaps.
 template <bool BF16, bool ROWS8, int DP, bool FULL, bool PAGE16, bool PACKED>
 struct Attention {
   static constexpr int KP = DP / 32;                   // products of a key tile

@@ -14,8 +14,8 @@
 // their way meanwhile and stay in registers. Counts are integers and a bias is chosen by its place in
 // the list: the order in which LDS is updated changes nothing.
 //
-// 256 rows of 131 071 bf16 logits: 26 us with nothing to do (5.1 TB/s), 35 with lists of 0 .. 4 096
-// tokens, 48 with biases and a mask too, by then bound by vector instructions. Tried: copying all under
+// 256 rows of 131 071 bf16 logits: 28 us with nothing to do (4.8 TB/s), 35 with lists of 0 .. 4 096
+// tokens, 48 with biases and a mask too, by then memory and some 25 us of vector instructions one behind the other. Tried: copying all under
 // the mask first and writing the named ones again (99), counts and biases in one word (49), a list of
 // the named ones made from what the counts' atomics return (58).
 #include <type_traits>
@@ -259,7 +259,7 @@ hipError_t launch_shape(const LogitsArgs& all, bool idx64, hipStream_t stream) {
 template <int TY>
 hipError_t launch(const LogitsArgs& a, bool idx64, hipStream_t stream) {
   // Every chunk's workgroup reads the row's whole list: long lists ask for larger chunks, others for more workgroups side by side.
-  // 256 rows of 131 071 bf16 logits: lists of 0 .. 4 096 tokens 48.7 us (512 x 32: 57.3), of 0 .. 60 000 tokens 149 us (104)
+  // 256 rows of 131 071 bf16 logits: lists of 0 .. 4 096 tokens 48.7 us (512 x 32: 57.3), of 0 .. 60 000 tokens 149 us (107)
   if (a.tokens_numel / a.rows > 8192) return launch_shape<TY, 512, 32 / Piece<TY>::N>(a, idx64, stream);
   return launch_shape<TY, 256, 16 / Piece<TY>::N>(a, idx64, stream);
 }
