@@ -70,6 +70,11 @@ bool rows_meet(const void* a, int64_t stride_a, const void* b, int64_t stride_b,
   return r < width || every - r < width;
 }
 
+// a status block holds a 64-bit number that kernels update atomically
+int check_status(const void* d_status) {
+  return (uintptr_t)d_status % 8 ? fail(FBGEMM_AMD_E_ARG, "a status block begins on an 8-byte boundary") : 0;
+}
+
 CacheRows rows_of(void* base, const int64_t (&strides)[3], int32_t ty) {
   const int64_t e = storage_bytes(ty);
   return CacheRows{(char*)base, strides[0] * e, strides[1] * e, strides[2] * e};
@@ -147,6 +152,7 @@ int fbgemm_amd_kv_block_tables(
   if (!d_offsets || !d_free_start || !d_free_next || (requests > 0 && (!d_lengths || !d_new_tokens || !d_total_lengths)) ||
       (requests > 0 && table_width > 0 && !d_block_tables) || (free_numel > 0 && !d_free_blocks) || (num_tokens > 0 && (!d_slots || !d_positions)))
     return fail(FBGEMM_AMD_E_ARG, "null data pointer");
+  if (int rc = check_status(d_status)) return rc;
   BlockTablesArgs a;
   a.lengths = d_lengths;
   a.new_tokens = d_new_tokens;
@@ -181,6 +187,7 @@ int fbgemm_amd_kv_cache_append(
   if (tokens == 0) return 0;
   if (!key_strides || !value_strides || !d_key || !d_value || !d_slots) return fail(FBGEMM_AMD_E_ARG, "null data pointer");
   if (cache->blocks > 0 && (!d_key_cache || !d_value_cache)) return fail(FBGEMM_AMD_E_ARG, "null data pointer");
+  if (int rc = check_status(d_status)) return rc;
   AppendArgs a;
   const int64_t e = storage_bytes(input_ty);
   a.in[0] = (const char*)d_key;

@@ -56,3 +56,11 @@ def test_logits_whose_result_overlaps_them_are_refused(lib):  # noqa: F811
                    {"out": at(950), "ostride": 0}):
         refused(lib, call(**{"logits": at(0), "out": at(0), **change}), "overlap")
     refused(lib, call(at(0), at(0), mask=P, words=3), "mask")
+
+
+def test_status_blocks_off_their_boundary_are_refused(lib):  # noqa: F811
+    s = (C.c_int64 * 2)(128, 64)
+    for at in (4097, 4098, 4100):
+        st = C.c_void_p(at)
+        refused(lib, lib.fbgemm_amd_kv_block_tables(P, P, 32, 3, P, 4, 4, P, 8, P, 16, 5, P, P, P, P, P, st, None), "status")
+        refused(lib, lib.fbgemm_amd_kv_cache_append(C.byref(cache()), P, P, 5, 3, s, s, P, P, C.c_void_p(1 << 20), st, None), "status")
