@@ -33,6 +33,11 @@ class PagedCache(C.Structure):
                 ("key_strides", _I64 * 3), ("value_strides", _I64 * 3)]
 
 
+class HeadRows(C.Structure):
+    """struct fbgemm_amd_head_rows."""
+    _fields_ = [("in_", _P), ("out", _P), ("in_strides", _I64 * 2), ("out_strides", _I64 * 2), ("heads", _I32)]
+
+
 SYMBOLS = {
     "fbgemm_amd_last_error": (C.c_char_p, []),
     "fbgemm_amd_version": (C.c_char_p, []),
@@ -83,6 +88,9 @@ SYMBOLS = {
     "fbgemm_amd_paged_attention_workspace": (_I64, [C.POINTER(PagedCache), _I64, _I32, _I64]),
     "fbgemm_amd_paged_attention": (C.c_int, [C.POINTER(PagedCache), _P, _I32, _I64, _I32, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I32, C.c_float, _I64, C.c_float, _P, _P, _P, _I64, _P]),
     "fbgemm_amd_penalize_logits": (C.c_int, [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P, _I32, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _I64, _P]),
+    "fbgemm_amd_kv_cache_read": (C.c_int, [C.POINTER(PagedCache), _P, _P, _P, _I64, _I64, _P, _P, _I32, _I64, _I64, _I32, _P, _P, _P, _P]),
+    "fbgemm_amd_rotate_positions": (C.c_int, [C.POINTER(HeadRows), C.POINTER(HeadRows), _I32, _I64, _I32, _P, _I32, _P, _I32, _I32, C.c_float, _I32, _P]),
+    "fbgemm_amd_sample_tokens": (C.c_int, [_P, _I32, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P]),
     "fbgemm_amd_unpadded_row_size_in_bytes": (_I32, [_I32, _I32, _I32]),
     "fbgemm_amd_padded_row_size_in_bytes": (_I32, [_I32, _I32, _I32, _I32]),
 }

@@ -59,7 +59,43 @@ struct AppendArgs {
   Status* status;
 };
 hipError_t launch_kv_append(const AppendArgs& a, int piece_bytes, hipStream_t stream);
-hipError_t launch_kv_append_rows8(const AppendArgs& a, int32_t input_ty, bool aligned16, hipStream_t stream); // aligned16: input rows are
+// rows of `bits` (8 or 4); aligned16: input rows are
+hipError_t launch_kv_append_coded(const AppendArgs& a, int bits, int32_t input_ty, bool aligned16, hipStream_t stream);
+
+// Rows of requests' tokens, out of their pages into dense arrays
+struct ReadArgs {
+  CacheRows cache[2]; // key, value
+  char* out[2];       // [tokens][heads][dim], dense
+  const int32_t* tables;
+  int64_t table_stride, table_width;
+  const void* offsets; // [requests + 1]
+  const void* starts;  // [requests] or null: zeros
+  int32_t idx64;
+  int32_t requests, heads, dim, blocks;
+  int64_t tokens;
+  Divisor block, per_row, per_token; // per_row, per_token: pieces of a row, and of a token's rows
+  Status* status;
+};
+constexpr int READ_RUN = 8; // codes of a piece
+hipError_t launch_kv_read(const ReadArgs& a, int piece_bytes, hipStream_t stream);                          // rows as they are
+hipError_t launch_kv_read_coded(const ReadArgs& a, int bits, int32_t output_ty, bool whole, hipStream_t stream); // whole: rows are whole pieces
+
+// Queries and keys turned by their positions
+struct RotateArgs {
+  const char* in[2]; // queries, keys: [tokens][heads][dim]
+  char* out[2];
+  int64_t in_token[2], in_head[2], out_token[2], out_head[2]; // bytes
+  int32_t heads[2], dim, pairs;                                // heads[1] may be 0
+  int64_t tokens;
+  const void* positions;
+  int32_t idx64, interleaved;
+  const double* frequencies; // [pairs], radians a position
+  float magnitude, sine;     // of cosines and sines: sine is -magnitude where turning back
+  int32_t token_group;       // tokens of a workgroup
+  Divisor units, all_heads;  // units: pieces of work of a head
+};
+constexpr int ROTATE_MOST_PAIRS = 1024; // their sines are in LDS
+hipError_t launch_rotate_positions(const RotateArgs& a, int32_t ty, bool aligned16, hipStream_t stream);
 
 struct AttentionArgs {
   const char* query; // [requests][heads][dim], 16 bits
@@ -93,6 +129,8 @@ hipError_t launch_paged_attention_bf16(const AttentionArgs& a, hipStream_t strea
 hipError_t launch_paged_attention_fp16(const AttentionArgs& a, hipStream_t stream);
 hipError_t launch_paged_attention_bf16_rows8(const AttentionArgs& a, hipStream_t stream);
 hipError_t launch_paged_attention_fp16_rows8(const AttentionArgs& a, hipStream_t stream);
+hipError_t launch_paged_attention_bf16_rows4(const AttentionArgs& a, hipStream_t stream);
+hipError_t launch_paged_attention_fp16_rows4(const AttentionArgs& a, hipStream_t stream);
 
 struct LogitsArgs {
   const void* logits;
@@ -113,5 +151,20 @@ struct LogitsArgs {
   int64_t mask_stride; // words
 };
 hipError_t launch_penalize_logits(const LogitsArgs& a, int32_t ty, bool idx64, hipStream_t stream);
+
+struct SampleArgs {
+  const void* logits;
+  int64_t rows, stride; // stride: elements
+  int32_t vocab;
+  const float* uniform;
+  const float* temperature; // [rows] or null, as the next ones
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t* tokens;
+  float* log_probability;
+};
+constexpr int SAMPLE_MOST_VOCAB = 1 << 20;
+hipError_t launch_sample_tokens(const SampleArgs& a, int32_t ty, hipStream_t stream);
 
 } // namespace fbgemm_amd

@@ -29,45 +29,65 @@ int32_t cache_row_bytes(const fbgemm_amd_paged_cache& c) {
     case ST_FP32: return c.dim * 4;
     case ST_FP16: case ST_BF16: return c.dim * 2;
     case ST_INT8: return c.dim + 4;
+    case ST_CACHE_INT4: return c.dim / 2 + 4;
     default: return 0;
   }
 }
-int32_t storage_bytes(int32_t ty) { return ty == ST_FP32 ? 4 : ty == ST_INT8 ? 1 : 2; }
+bool coded(int32_t ty) { return ty == ST_INT8 || ty == ST_CACHE_INT4; }
+int32_t storage_bytes(int32_t ty) { return ty == ST_FP32 ? 4 : coded(ty) ? 1 : 2; }
 
 int check_cache(const fbgemm_amd_paged_cache* c) {
   if (!c) return fail(FBGEMM_AMD_E_ARG, "cache is null");
   if (c->dim <= 0 || c->dim > (1 << 16)) return fail(FBGEMM_AMD_E_ARG, "dim must be in 1..65536");
-  if (!cache_row_bytes(*c)) return fail(FBGEMM_AMD_E_ARG, "a cache holds FP32, FP16, BF16 or INT8 rows");
+  if (!cache_row_bytes(*c)) return fail(FBGEMM_AMD_E_ARG, "a cache holds FP32, FP16, BF16, INT8 or CACHE_INT4 rows");
+  if (c->row_ty == ST_CACHE_INT4 && c->dim % 2) return fail(FBGEMM_AMD_E_ARG, "4-bit rows hold an even number of elements: got dim %d", c->dim);
   if (c->heads <= 0 || c->heads > (1 << 16)) return fail(FBGEMM_AMD_E_ARG, "heads must be in 1..65536");
   if ((int64_t)c->heads * c->dim > (1 << 28)) return fail(FBGEMM_AMD_E_ARG, "heads * dim must not exceed 2^28");
   if (c->block_size <= 0 || c->block_size > (1 << 20)) return fail(FBGEMM_AMD_E_ARG, "block_size must be in 1..1048576");
   if (c->blocks < 0 || c->blocks > MOST) return fail(FBGEMM_AMD_E_ARG, "blocks must be in 0..2^31-1");
   for (int k = 0; k < 3; ++k)
     if (c->key_strides[k] < 0 || c->value_strides[k] < 0) return fail(FBGEMM_AMD_E_ARG, "strides must not be negative");
-  if (c->row_ty == ST_INT8 && !(divides(4, {c->key_strides[0], c->key_strides[1], c->key_strides[2]}) &&
+  if (coded(c->row_ty) && !(divides(4, {c->key_strides[0], c->key_strides[1], c->key_strides[2]}) &&
                                 divides(4, {c->value_strides[0], c->value_strides[1], c->value_strides[2]})))
-    return fail(FBGEMM_AMD_E_ARG, "8-bit rows begin on 4-byte boundaries: strides must be multiples of 4");
+    return fail(FBGEMM_AMD_E_ARG, "8-bit and 4-bit rows begin on 4-byte boundaries: strides must be multiples of 4");
   return 0;
 }
 
 // rows of a cache that is written: of two, neither reaches into the other
 bool rows_apart(const fbgemm_amd_paged_cache& c, const int64_t (&strides)[3]) {
-  const int64_t row = c.row_ty == ST_INT8 ? cache_row_bytes(c) : c.dim;
+  const int64_t row = coded(c.row_ty) ? cache_row_bytes(c) : c.dim;
   const int64_t size[3] = {c.blocks, c.heads, c.block_size};
   for (int k = 0; k < 3; ++k)
     if (size[k] > 1 && strides[k] < row) return false;
   return true;
 }
 
-// Two arrays of rows of `width` bytes, `stride_a` and `stride_b` apart, that share a byte (or may, where neither stride divides the other)
-bool rows_meet(const void* a, int64_t stride_a, const void* b, int64_t stride_b, int64_t rows, int64_t width) {
+// Two arrays of rows of `width_a` and `width_b` bytes, `stride_a` and `stride_b` apart, that share a byte (or may, where neither stride divides the other)
+bool rows_meet(const void* a, int64_t stride_a, int64_t width_a, const void* b, int64_t stride_b, int64_t width_b, int64_t rows) {
   typedef __int128 wide; // strides are the caller's
-  const wide d = (wide)(uintptr_t)b - (wide)(uintptr_t)a, last_a = (wide)(rows - 1) * stride_a + width, last_b = (wide)(rows - 1) * stride_b + width;
+  const wide d = (wide)(uintptr_t)b - (wide)(uintptr_t)a, last_a = (wide)(rows - 1) * stride_a + width_a, last_b = (wide)(rows - 1) * stride_b + width_b;
   if (d >= last_a || -d >= last_b) return false;
   const int64_t every = std::gcd(stride_a, stride_b);
   if (rows == 1 || every == 0) return true;
-  const wide r = (d % every + every) % every;
-  return r < width || every - r < width;
+  const wide r = (d % every + every) % every; // of b's rows behind a's, whole steps left out
+  return r < width_a || every - r < width_b;
+}
+
+// [tokens][heads][dim] as rows of `width` bytes, `stride` apart: a token's heads, or a head's tokens. apart: no two elements are one.
+struct Span {
+  int64_t rows, stride, width;
+  bool apart;
+};
+Span span_of(const fbgemm_amd_head_rows& r, const int64_t (&strides)[2], int64_t tokens, int64_t dim, int64_t element) {
+  const int64_t size[2] = {tokens, r.heads};
+  const int outer = r.heads == 1 || (tokens > 1 && strides[0] >= strides[1]) ? 0 : 1, inner = 1 - outer;
+  Span s{size[outer], size[outer] > 1 ? strides[outer] * element : 0, ((size[inner] > 1 ? (size[inner] - 1) * strides[inner] : 0) + dim) * element, true};
+  s.apart = (size[inner] <= 1 || strides[inner] >= dim) && (s.rows <= 1 || s.stride >= s.width);
+  return s;
+}
+bool spans_meet(const void* a, const Span& x, const void* b, const Span& y) {
+  if (x.rows == y.rows) return rows_meet(a, x.stride, x.width, b, y.stride, y.width, x.rows);
+  return rows_meet(a, 0, (x.rows - 1) * x.stride + x.width, b, 0, (y.rows - 1) * y.stride + y.width, 1);
 }
 
 // a status block holds a 64-bit number that kernels update atomically
@@ -120,7 +140,7 @@ AttentionSpace attention_space(int workers, int32_t dim) {
 
 int check_attention(const fbgemm_amd_paged_cache* cache, int64_t requests, int32_t query_heads, int64_t table_width) {
   if (int rc = check_cache(cache)) return rc;
-  if (cache->row_ty == ST_FP32) return fail(FBGEMM_AMD_E_UNSUPPORTED, "attention reads FP16, BF16 or INT8 rows");
+  if (cache->row_ty == ST_FP32) return fail(FBGEMM_AMD_E_UNSUPPORTED, "attention reads FP16, BF16 or INT8 rows, or CACHE_INT4 ones");
   if (cache->dim % 8 || cache->dim > 256) return fail(FBGEMM_AMD_E_UNSUPPORTED, "attention takes a dim that is a multiple of 8, up to 256: got %d", cache->dim);
   if (requests < 0 || requests > (1 << 24)) return fail(FBGEMM_AMD_E_ARG, "requests must be in 0..2^24");
   if (query_heads <= 0 || query_heads > (1 << 20) || query_heads % cache->heads)
@@ -180,9 +200,9 @@ int fbgemm_amd_kv_cache_append(
     const int64_t* key_strides, const int64_t* value_strides, const int64_t* d_slots, void* d_key_cache, void* d_value_cache,
     void* d_status, void* stream) {
   if (int rc = check_cache(cache)) return rc;
-  const bool rows8 = cache->row_ty == ST_INT8;
+  const bool codes = coded(cache->row_ty);
   if (input_ty != ST_FP32 && input_ty != ST_FP16 && input_ty != ST_BF16) return fail(FBGEMM_AMD_E_ARG, "keys and values are FP32, FP16 or BF16");
-  if (!rows8 && input_ty != cache->row_ty) return fail(FBGEMM_AMD_E_ARG, "rows are stored as they come: the cache's type must be the keys'");
+  if (!codes && input_ty != cache->row_ty) return fail(FBGEMM_AMD_E_ARG, "rows are stored as they come: the cache's type must be the keys'");
   if (tokens < 0 || tokens > MOST) return fail(FBGEMM_AMD_E_ARG, "tokens must be in 0..2^31-1");
   if (tokens == 0) return 0;
   if (!key_strides || !value_strides || !d_key || !d_value || !d_slots) return fail(FBGEMM_AMD_E_ARG, "null data pointer");
@@ -215,12 +235,12 @@ int fbgemm_amd_kv_cache_append(
     return d_key_cache == d_value_cache && cache->blocks > 0 && !same ? fail(FBGEMM_AMD_E_ARG, "keys and values that differ must not overlap in the cache") : 0;
   };
   if (!rows_apart(*cache, cache->key_strides) || !rows_apart(*cache, cache->value_strides)) return fail(FBGEMM_AMD_E_ARG, "rows of a cache must not overlap");
-  if (rows8) {
-    if ((uintptr_t)d_key_cache % 4 || (uintptr_t)d_value_cache % 4) return fail(FBGEMM_AMD_E_ARG, "8-bit rows begin on 4-byte boundaries");
+  if (codes) {
+    if ((uintptr_t)d_key_cache % 4 || (uintptr_t)d_value_cache % 4) return fail(FBGEMM_AMD_E_ARG, "8-bit and 4-bit rows begin on 4-byte boundaries");
     if (int rc = check_shared()) return rc;
     const bool aligned16 = (uintptr_t)d_key % 16 == 0 && (uintptr_t)d_value % 16 == 0 &&
         divides(16, {a.token_stride[0], a.head_stride[0], a.token_stride[1], a.head_stride[1]});
-    HIP_TRY(launch_kv_append_rows8(a, input_ty, aligned16, (hipStream_t)stream));
+    HIP_TRY(launch_kv_append_coded(a, cache->row_ty == ST_INT8 ? 8 : 4, input_ty, aligned16, (hipStream_t)stream));
     return 0;
   }
   // the largest piece that every row is made of and begins at
@@ -240,6 +260,131 @@ int fbgemm_amd_kv_cache_append(
   return 0;
 }
 
+int fbgemm_amd_kv_cache_read(
+    const fbgemm_amd_paged_cache* cache, const void* d_key_cache, const void* d_value_cache, const int32_t* d_block_tables,
+    int64_t table_stride, int64_t table_width, const void* d_offsets, const void* d_starts, int32_t index_bits, int64_t requests,
+    int64_t tokens, int32_t output_ty, void* d_key, void* d_value, void* d_status, void* stream) {
+  if (int rc = check_cache(cache)) return rc;
+  const bool codes = coded(cache->row_ty);
+  if (output_ty != ST_FP32 && output_ty != ST_FP16 && output_ty != ST_BF16) return fail(FBGEMM_AMD_E_ARG, "keys and values are FP32, FP16 or BF16");
+  if (!codes && output_ty != cache->row_ty) return fail(FBGEMM_AMD_E_ARG, "rows come as they are stored: the keys' type must be the cache's");
+  if (index_bits != 32 && index_bits != 64) return fail(FBGEMM_AMD_E_ARG, "index_bits must be 32 or 64");
+  if (requests < 0 || requests > MOST - 1) return fail(FBGEMM_AMD_E_ARG, "requests must be in 0..2^31-2");
+  if (tokens < 0 || tokens > MOST) return fail(FBGEMM_AMD_E_ARG, "tokens must be in 0..2^31-1");
+  if (table_width < 0 || table_width > (MOST - cache->block_size) / cache->block_size) return fail(FBGEMM_AMD_E_ARG, "a table must hold fewer than 2^31 tokens");
+  if (tokens == 0) return 0;
+  if (!d_key || !d_value || !d_offsets || (requests > 0 && table_width > 0 && !d_block_tables) || (cache->blocks > 0 && (!d_key_cache || !d_value_cache)))
+    return fail(FBGEMM_AMD_E_ARG, "null data pointer");
+  if ((uintptr_t)d_key % 16 || (uintptr_t)d_value % 16) return fail(FBGEMM_AMD_E_ARG, "keys and values must begin on 16-byte boundaries");
+  if (int rc = check_status(d_status)) return rc;
+  ReadArgs a;
+  a.cache[0] = rows_of(const_cast<void*>(d_key_cache), cache->key_strides, cache->row_ty);
+  a.cache[1] = rows_of(const_cast<void*>(d_value_cache), cache->value_strides, cache->row_ty);
+  a.out[0] = (char*)d_key;
+  a.out[1] = (char*)d_value;
+  a.tables = d_block_tables;
+  a.table_stride = table_stride;
+  a.table_width = table_width;
+  a.offsets = d_offsets;
+  a.starts = d_starts;
+  a.idx64 = index_bits == 64;
+  a.requests = (int32_t)requests;
+  a.heads = cache->heads;
+  a.dim = cache->dim;
+  a.blocks = (int32_t)cache->blocks;
+  a.tokens = tokens;
+  a.block = make_divisor((uint32_t)cache->block_size);
+  a.status = (Status*)d_status;
+  const auto pieces = [&](int32_t of_row) {
+    a.per_row = make_divisor((uint32_t)of_row);
+    a.per_token = make_divisor((uint32_t)(of_row * cache->heads)); // heads * dim is at most 2^28
+  };
+  const auto on = [&](int64_t p) {
+    bool ok = true;
+    for (const CacheRows& c : a.cache) ok = ok && divides(p, {c.block_stride, c.head_stride, c.slot_stride}) && (uintptr_t)c.base % p == 0;
+    return ok;
+  };
+  if (codes) {
+    if (!on(4)) return fail(FBGEMM_AMD_E_ARG, "8-bit and 4-bit rows begin on 4-byte boundaries");
+    const bool whole = cache->dim % READ_RUN == 0;
+    pieces(whole ? cache->dim / READ_RUN : cache->dim);
+    HIP_TRY(launch_kv_read_coded(a, cache->row_ty == ST_INT8 ? 8 : 4, output_ty, whole, (hipStream_t)stream));
+    return 0;
+  }
+  const int32_t row_bytes = cache_row_bytes(*cache);
+  int piece = 16;
+  const auto fits = [&](int p) { return row_bytes % p == 0 && on(p); };
+  while (piece > 2 && !fits(piece)) piece >>= 1;
+  if (!fits(piece)) return fail(FBGEMM_AMD_E_ARG, "rows are not aligned to their elements");
+  pieces(row_bytes / piece);
+  HIP_TRY(launch_kv_read(a, piece, (hipStream_t)stream));
+  return 0;
+}
+
+int fbgemm_amd_rotate_positions(
+    const fbgemm_amd_head_rows* query, const fbgemm_amd_head_rows* key, int32_t ty, int64_t tokens, int32_t dim,
+    const void* d_positions, int32_t index_bits, const double* d_frequencies, int32_t pairs, int32_t interleaved,
+    float magnitude, int32_t inverse, void* stream) {
+  if (!query) return fail(FBGEMM_AMD_E_ARG, "query is null");
+  if (ty != ST_FP32 && ty != ST_FP16 && ty != ST_BF16) return fail(FBGEMM_AMD_E_ARG, "queries and keys are FP32, FP16 or BF16");
+  if (index_bits != 32 && index_bits != 64) return fail(FBGEMM_AMD_E_ARG, "index_bits must be 32 or 64");
+  if (tokens < 0 || tokens > MOST) return fail(FBGEMM_AMD_E_ARG, "tokens must be in 0..2^31-1");
+  if (dim <= 0 || dim > (1 << 16)) return fail(FBGEMM_AMD_E_ARG, "dim must be in 1..65536");
+  if (pairs < 0 || 2 * (int64_t)pairs > dim || pairs > ROTATE_MOST_PAIRS) return fail(FBGEMM_AMD_E_ARG, "a head of %d has at most %d pairs, and no more than %d are turned", dim, dim / 2, ROTATE_MOST_PAIRS);
+  if (!std::isfinite(magnitude)) return fail(FBGEMM_AMD_E_ARG, "magnitude must be finite");
+  const fbgemm_amd_head_rows* of[2] = {query, key};
+  int64_t heads = 0;
+  for (const auto* r : of) {
+    if (!r) continue;
+    if (r->heads < 0 || r->heads > (1 << 16)) return fail(FBGEMM_AMD_E_ARG, "heads must be in 0..65536");
+    for (int k = 0; k < 2; ++k)
+      if (r->in_strides[k] < 0 || r->out_strides[k] < 0) return fail(FBGEMM_AMD_E_ARG, "strides must not be negative");
+    heads += r->heads;
+  }
+  if (heads * dim > (1 << 28)) return fail(FBGEMM_AMD_E_ARG, "heads * dim must not exceed 2^28");
+  if (tokens == 0 || heads == 0) return 0;
+  if (!d_positions || (pairs > 0 && !d_frequencies)) return fail(FBGEMM_AMD_E_ARG, "null data pointer");
+  RotateArgs a = {};
+  const int64_t e = storage_bytes(ty);
+  bool aligned16 = true;
+  for (int k = 0; k < 2; ++k) {
+    const auto* r = of[k];
+    if (!r || r->heads == 0) continue;
+    if (!r->in || !r->out) return fail(FBGEMM_AMD_E_ARG, "null data pointer");
+    if ((uintptr_t)r->in % e || (uintptr_t)r->out % e) return fail(FBGEMM_AMD_E_ARG, "rows are not aligned to their elements");
+    if (!span_of(*r, r->out_strides, tokens, dim, e).apart) return fail(FBGEMM_AMD_E_ARG, "rows of a result must not overlap");
+    a.in[k] = (const char*)r->in;
+    a.out[k] = (char*)r->out;
+    a.in_token[k] = r->in_strides[0] * e;
+    a.in_head[k] = r->in_strides[1] * e;
+    a.out_token[k] = r->out_strides[0] * e;
+    a.out_head[k] = r->out_strides[1] * e;
+    a.heads[k] = r->heads;
+    aligned16 = aligned16 && divides(16, {a.in_token[k], a.in_head[k], a.out_token[k], a.out_head[k]}) && (uintptr_t)r->in % 16 == 0 && (uintptr_t)r->out % 16 == 0;
+  }
+  for (int k = 0; k < 2; ++k)
+    for (int i = 0; i < 2; ++i) {
+      if (!a.heads[k] || !a.heads[i]) continue;
+      const bool in_place = i == k && a.in[k] == a.out[k] && (tokens == 1 || a.in_token[k] == a.out_token[k]) && (a.heads[k] == 1 || a.in_head[k] == a.out_head[k]);
+      const Span out = span_of(*of[k], of[k]->out_strides, tokens, dim, e);
+      if (!in_place && spans_meet(a.in[i], span_of(*of[i], of[i]->in_strides, tokens, dim, e), a.out[k], out))
+        return fail(FBGEMM_AMD_E_ARG, "a result may be its own input, but must not overlap inputs otherwise");
+      if (i < k && spans_meet(a.out[i], span_of(*of[i], of[i]->out_strides, tokens, dim, e), a.out[k], out))
+        return fail(FBGEMM_AMD_E_ARG, "the results must not overlap each other");
+    }
+  a.dim = dim;
+  a.pairs = pairs;
+  a.tokens = tokens;
+  a.positions = d_positions;
+  a.idx64 = index_bits == 64;
+  a.interleaved = interleaved != 0;
+  a.frequencies = d_frequencies;
+  a.magnitude = magnitude;
+  a.sine = inverse ? -magnitude : magnitude;
+  HIP_TRY(launch_rotate_positions(a, ty, aligned16, (hipStream_t)stream));
+  return 0;
+}
+
 int64_t fbgemm_amd_paged_attention_workspace(const fbgemm_amd_paged_cache* cache, int64_t requests, int32_t query_heads, int64_t table_width) {
   if (int rc = check_attention(cache, requests, query_heads, table_width)) return rc;
   if (requests == 0) return 0;
@@ -252,9 +397,9 @@ int fbgemm_amd_paged_attention(
     const int32_t* d_block_tables, int64_t table_stride, int64_t table_width, const void* d_lengths, int32_t index_bits,
     float scale, int64_t window, float softcap, void* d_output, float* d_lse, void* d_workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = check_attention(cache, requests, query_heads, table_width)) return rc;
-  const bool rows8 = cache->row_ty == ST_INT8;
+  const bool codes = coded(cache->row_ty);
   if (query_ty != ST_FP16 && query_ty != ST_BF16) return fail(FBGEMM_AMD_E_UNSUPPORTED, "queries are FP16 or BF16");
-  if (!rows8 && query_ty != cache->row_ty) return fail(FBGEMM_AMD_E_ARG, "16-bit rows must have the queries' type");
+  if (!codes && query_ty != cache->row_ty) return fail(FBGEMM_AMD_E_ARG, "16-bit rows must have the queries' type");
   if (index_bits != 32 && index_bits != 64) return fail(FBGEMM_AMD_E_ARG, "index_bits must be 32 or 64");
   if (window < 0) return fail(FBGEMM_AMD_E_ARG, "window must not be negative");
   if (!std::isfinite(scale)) return fail(FBGEMM_AMD_E_ARG, "scale must be finite");
@@ -269,12 +414,12 @@ int fbgemm_amd_paged_attention(
   a.query_head_stride = query_head_stride * 2;
   a.key = rows_of(const_cast<void*>(d_key_cache), cache->key_strides, cache->row_ty);
   a.value = rows_of(const_cast<void*>(d_value_cache), cache->value_strides, cache->row_ty);
-  const int64_t row_align = rows8 ? 4 : 16;
+  const int64_t row_align = codes ? 4 : 16;
   bool aligned = divides(16, {a.query_request_stride, a.query_head_stride}) && (uintptr_t)d_query % 16 == 0;
   if (a.key.slot_stride >= (1 << 26) || a.value.slot_stride >= (1 << 26)) return fail(FBGEMM_AMD_E_UNSUPPORTED, "tokens of a block must be less than 64 MiB apart");
   for (const CacheRows* r : {&a.key, &a.value})
     aligned = aligned && divides(row_align, {r->block_stride, r->head_stride, r->slot_stride}) && (uintptr_t)r->base % row_align == 0;
-  if (!aligned) return fail(FBGEMM_AMD_E_ARG, "queries and 16-bit rows must begin on 16-byte boundaries, 8-bit rows on 4-byte ones");
+  if (!aligned) return fail(FBGEMM_AMD_E_ARG, "queries and 16-bit rows must begin on 16-byte boundaries, 8-bit and 4-bit rows on 4-byte ones");
   if ((uintptr_t)d_output % 16 || (uintptr_t)d_workspace % 16) return fail(FBGEMM_AMD_E_ARG, "output and workspace must begin on 16-byte boundaries");
   a.tables = d_block_tables;
   a.table_stride = table_stride;
@@ -304,8 +449,12 @@ int fbgemm_amd_paged_attention(
   a.partial = (float*)d_workspace;
   a.partial_ml = (float*)((char*)d_workspace + space.partial);
   a.joins = (int4*)((char*)d_workspace + space.partial + space.ml);
-  if (query_ty == ST_BF16) HIP_TRY(rows8 ? launch_paged_attention_bf16_rows8(a, (hipStream_t)stream) : launch_paged_attention_bf16(a, (hipStream_t)stream));
-  else HIP_TRY(rows8 ? launch_paged_attention_fp16_rows8(a, (hipStream_t)stream) : launch_paged_attention_fp16(a, (hipStream_t)stream));
+  const bool bf16 = query_ty == ST_BF16;
+  hipError_t (*const launch)(const AttentionArgs&, hipStream_t) =
+      cache->row_ty == ST_INT8 ? (bf16 ? launch_paged_attention_bf16_rows8 : launch_paged_attention_fp16_rows8)
+      : cache->row_ty == ST_CACHE_INT4 ? (bf16 ? launch_paged_attention_bf16_rows4 : launch_paged_attention_fp16_rows4)
+                                       : (bf16 ? launch_paged_attention_bf16 : launch_paged_attention_fp16);
+  HIP_TRY(launch(a, (hipStream_t)stream));
   return 0;
 }
 
@@ -326,7 +475,7 @@ int fbgemm_amd_penalize_logits(
   if (d_mask && rows > 1 && mask_stride != 0 && mask_stride < (vocab + 31) / 32) return fail(FBGEMM_AMD_E_ARG, "a row of the mask has one bit per token of the vocabulary");
   const int64_t e = storage_bytes(logits_ty);
   const bool in_place = d_output == d_logits && (rows == 1 || output_stride == logits_stride);
-  if (!in_place && rows_meet(d_logits, rows > 1 ? logits_stride * e : 0, d_output, rows > 1 ? output_stride * e : 0, rows, vocab * e))
+  if (!in_place && rows_meet(d_logits, rows > 1 ? logits_stride * e : 0, vocab * e, d_output, rows > 1 ? output_stride * e : 0, vocab * e, rows))
     return fail(FBGEMM_AMD_E_ARG, "the result may be the logits themselves, but must not overlap them otherwise");
   LogitsArgs a;
   a.logits = d_logits;
@@ -349,6 +498,32 @@ int fbgemm_amd_penalize_logits(
   a.mask = (const uint32_t*)d_mask;
   a.mask_stride = mask_stride;
   HIP_TRY(launch_penalize_logits(a, logits_ty, index_bits == 64, (hipStream_t)stream));
+  return 0;
+}
+
+int fbgemm_amd_sample_tokens(
+    const void* d_logits, int32_t logits_ty, int64_t rows, int64_t vocab, int64_t logits_stride, const float* d_uniform,
+    const float* d_temperature, const int32_t* d_top_k, const float* d_top_p, const float* d_min_p, int64_t* d_tokens,
+    float* d_log_probability, void* stream) {
+  if (logits_ty != ST_FP32 && logits_ty != ST_FP16 && logits_ty != ST_BF16) return fail(FBGEMM_AMD_E_ARG, "logits are FP32, FP16 or BF16");
+  if (rows < 0 || rows > (1 << 24)) return fail(FBGEMM_AMD_E_ARG, "rows must be in 0..2^24");
+  if (vocab < 1 || vocab > SAMPLE_MOST_VOCAB) return fail(FBGEMM_AMD_E_ARG, "vocab must be in 1..2^20");
+  if (rows == 0) return 0;
+  if (!d_logits || !d_uniform || !d_tokens || !d_log_probability) return fail(FBGEMM_AMD_E_ARG, "null data pointer");
+  if (logits_stride < 0) return fail(FBGEMM_AMD_E_ARG, "strides must not be negative");
+  SampleArgs a;
+  a.logits = d_logits;
+  a.rows = rows;
+  a.stride = rows > 1 ? logits_stride : 0;
+  a.vocab = (int32_t)vocab;
+  a.uniform = d_uniform;
+  a.temperature = d_temperature;
+  a.top_k = d_top_k;
+  a.top_p = d_top_p;
+  a.min_p = d_min_p;
+  a.tokens = d_tokens;
+  a.log_probability = d_log_probability;
+  HIP_TRY(launch_sample_tokens(a, logits_ty, (hipStream_t)stream));
   return 0;
 }
 

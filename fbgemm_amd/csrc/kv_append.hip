@@ -1,7 +1,7 @@
 // New key and value rows into their slots of a paged cache: cache[slot / S][head][slot % S] = row,
-// as they are, or as the framework's 8-bit rows (fp16 scale and bias in front, then the bytes).
+// as they are, or as the framework's 8-bit or 4-bit rows (fp16 scale and bias in front, then the codes).
 //
-// Bound by memory: every byte is read once and written once (8-bit rows: half of it written). A
+// Bound by memory: every byte is read once and written once (8-bit rows: half of it written, 4-bit rows: a quarter). A
 // thread takes a piece of 16 bytes (less where strides or addresses ask for it) of one row of both
 // keys and values, so that two loads are in flight and the slot is looked up once for the two.
 #include "decode.h"
@@ -83,6 +83,10 @@ __device__ __forceinline__ float held(float x) { return x != x ? 0.0f : __builti
 __device__ __forceinline__ uint32_t put_byte(float x, const RowCode& code, uint32_t at, uint32_t word) {
   return __builtin_amdgcn_cvt_pk_u8_f32(__builtin_rintf((x - code.minimum) * code.inverse_scale), at, word);
 }
+// an element's 4 bits
+__device__ __forceinline__ uint32_t code4(float x, const RowCode& code) {
+  return (uint32_t)__builtin_amdgcn_fmed3f(__builtin_rintf((x - code.minimum) * code.inverse_scale), 0.0f, 15.0f);
+}
 template <int CTRL>
 __device__ __forceinline__ float other(float x) { // of the lane that a row's permutation puts here
   const int v = __builtin_bit_cast(int, x);
@@ -102,8 +106,8 @@ __device__ __forceinline__ void extremes_of_group(float& lo, float& hi, int lane
 }
 
 // One row per group of `lanes` lanes (a power of two): rows of any length and alignment, read twice.
-template <typename T>
-__global__ __launch_bounds__(THREADS) void kv_append_rows8_kernel(const AppendArgs a, const int lanes) {
+template <int BITS, typename T>
+__global__ __launch_bounds__(THREADS) void kv_append_coded_kernel(const AppendArgs a, const int lanes) {
   const int sub = threadIdx.x & (lanes - 1);
   const int64_t rows = a.tokens * a.heads;
   const int64_t groups = (int64_t)gridDim.x * (THREADS / lanes);
@@ -124,9 +128,14 @@ __global__ __launch_bounds__(THREADS) void kv_append_rows8_kernel(const AppendAr
         hi = __builtin_fmaxf(hi, x);
       }
       extremes_of_group(lo, hi, lanes);
-      const RowCode code = row_code<8>(lo, hi, 0, 1);
+      const RowCode code = row_code<BITS>(lo, hi, 0, 1);
       if (sub == 0) *reinterpret_cast<uint32_t*>(out) = (code.sb0 & 0xffffu) | (code.sb1 << 16);
-      for (int j = sub; j < a.dim; j += lanes) out[4 + j] = (char)put_byte(held(T::at(in + (int64_t)j * T::BYTES)), code, 0, 0);
+      const auto at = [&](int j) { return held(T::at(in + (int64_t)j * T::BYTES)); };
+      if constexpr (BITS == 8) {
+        for (int j = sub; j < a.dim; j += lanes) out[4 + j] = (char)put_byte(at(j), code, 0, 0);
+      } else { // an even number of elements
+        for (int j = sub; 2 * j < a.dim; j += lanes) out[4 + j] = (char)(code4(at(2 * j), code) | (code4(at(2 * j + 1), code) << 4));
+      }
     }
   }
 }
@@ -135,8 +144,8 @@ __global__ __launch_bounds__(THREADS) void kv_append_rows8_kernel(const AppendAr
 // loaded together and stay in registers between the search for their extremes and the rounding, lane by lane.
 // 8 191 tokens x 5 heads x 128 bf16 (32 MB read and written, 6 us at a copy's rate) take 31.5 us by the kernel above and 12.1
 // here (13.1 with bytes put together by shifts and extremes exchanged through LDS, 13.3 with two pairs in flight a group).
-template <typename T>
-__global__ __launch_bounds__(THREADS) void kv_append_rows8_runs_kernel(const AppendArgs a, const int lanes) {
+template <int BITS, typename T>
+__global__ __launch_bounds__(THREADS) void kv_append_coded_runs_kernel(const AppendArgs a, const int lanes) {
   typedef piece8 __attribute__((aligned(4))) on4_t; // a row begins on 4 bytes
   const int sub = threadIdx.x & (lanes - 1);
   const bool mine = sub * RUN < a.dim;
@@ -165,22 +174,35 @@ __global__ __launch_bounds__(THREADS) void kv_append_rows8_runs_kernel(const App
         hi = mine ? __builtin_fmaxf(hi, x[e]) : hi;
       }
       extremes_of_group(lo, hi, lanes);
-      const RowCode code = row_code<8>(lo, hi, 0, 1);
+      const RowCode code = row_code<BITS>(lo, hi, 0, 1);
       const CacheRows& c = a.cache[k];
       char* out = c.base + p.block * c.block_stride + head * c.head_stride + p.in_block * c.slot_stride;
       if (sub == 0) *reinterpret_cast<uint32_t*>(out) = (code.sb0 & 0xffffu) | (code.sb1 << 16);
-      piece8 q = {0, 0};
+      if constexpr (BITS == 8) {
+        piece8 q = {0, 0};
 #pragma unroll
-      for (int e = 0; e < RUN; ++e) q[e / 4] = put_byte(x[e], code, e % 4, q[e / 4]);
-      if (mine) *reinterpret_cast<on4_t*>(out + 4 + sub * RUN) = q;
+        for (int e = 0; e < RUN; ++e) q[e / 4] = put_byte(x[e], code, e % 4, q[e / 4]);
+        if (mine) *reinterpret_cast<on4_t*>(out + 4 + sub * RUN) = q;
+      } else {
+        uint32_t q = 0;
+#pragma unroll
+        for (int e = 0; e < RUN; ++e) q |= code4(x[e], code) << (4 * e);
+        if (mine) *reinterpret_cast<uint32_t*>(out + 4 + sub * RUN / 2) = q;
+      }
     }
   }
 }
 
-template <typename T>
-void launch_rows8(const AppendArgs& a, int lanes, int grid, bool runs, hipStream_t stream) {
-  if (runs) kv_append_rows8_runs_kernel<T><<<grid, THREADS, 0, stream>>>(a, lanes);
-  else kv_append_rows8_kernel<T><<<grid, THREADS, 0, stream>>>(a, lanes);
+template <int BITS>
+void launch_coded(const AppendArgs& a, int32_t input_ty, int lanes, int grid, bool runs, hipStream_t stream) {
+  const auto launch = [&](auto type) {
+    using T = decltype(type);
+    if (runs) kv_append_coded_runs_kernel<BITS, T><<<grid, THREADS, 0, stream>>>(a, lanes);
+    else kv_append_coded_kernel<BITS, T><<<grid, THREADS, 0, stream>>>(a, lanes);
+  };
+  if (input_ty == ST_FP32) launch(F32());
+  else if (input_ty == ST_FP16) launch(F16());
+  else launch(B16());
 }
 
 int grid_for(int64_t items, int per_block) {
@@ -201,14 +223,13 @@ hipError_t launch_kv_append(const AppendArgs& a, int piece_bytes, hipStream_t st
   return hipGetLastError();
 }
 
-hipError_t launch_kv_append_rows8(const AppendArgs& a, int32_t input_ty, bool aligned16, hipStream_t stream) {
+hipError_t launch_kv_append_coded(const AppendArgs& a, int bits, int32_t input_ty, bool aligned16, hipStream_t stream) {
   int lanes = 1;
   while (lanes < 64 && lanes * RUN < a.dim) lanes <<= 1;
   const int grid = grid_for(a.tokens * a.heads, THREADS / lanes);
   const bool runs = aligned16 && a.dim % RUN == 0 && a.dim <= 64 * RUN;
-  if (input_ty == ST_FP32) launch_rows8<F32>(a, lanes, grid, runs, stream);
-  else if (input_ty == ST_FP16) launch_rows8<F16>(a, lanes, grid, runs, stream);
-  else launch_rows8<B16>(a, lanes, grid, runs, stream);
+  if (bits == 8) launch_coded<8>(a, input_ty, lanes, grid, runs, stream);
+  else launch_coded<4>(a, input_ty, lanes, grid, runs, stream);
   return hipGetLastError();
 }
 

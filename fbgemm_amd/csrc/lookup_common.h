@@ -14,6 +14,7 @@ enum : int32_t {
   ST_INT2 = 4,
   ST_BF16 = 5,
   ST_FP8 = 6, // 8-bit floats (1 sign, e exponent, 7 - e mantissa bits; exponent bias given per call)
+  ST_CACHE_INT4 = 16, // 4-bit rows of a key-value cache
 };
 
 // Bits of the status word a lookup ORs in when it meets an input the reference

@@ -131,9 +131,22 @@ __device__ __forceinline__ uint4 widen(uint32_t a, uint32_t b) {
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+// A word of 4-bit codes as operands of 16 bits, without arithmetic: a code in the low bits of a number is a subnormal one,
+// code * 2^-133 of bf16 (2^-24 of fp16), and 4 bits further up 16 times that. The matrix cores take subnormal numbers
+// exactly. Elements come as (0, 4), (1, 5), (2, 6), (3, 7): the queries' operand has the same order. bf16: odd elements are 16 times
+// larger, which the queries make up for. fp16: all are; sums of codes in the lowest bits, which lie 6 to 10 bits under
+// the products' leading one, came out as 2^-21 of the terms' sizes, those 16 times larger as 2^-26.
+template <bool BF16>
+__device__ __forceinline__ uint4 codes4(uint32_t w) {
+  constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
+  if (BF16) return make_uint4(w & LOW, w & HIGH, (w >> 8) & LOW, (w >> 8) & HIGH);
+  return make_uint4((w << 4) & HIGH, w & HIGH, (w >> 4) & HIGH, (w >> 8) & HIGH);
+}
+
 __device__ __forceinline__ float half_at(uint32_t pair, int i) { return (float)__builtin_bit_cast(f16x2, pair)[i]; }
-// what byte 128 of a row stands for, by its scale and bias
-__device__ __forceinline__ float middle(uint32_t pair) { return __builtin_fmaf(128.0f, half_at(pair, 0), half_at(pair, 1)); }
+// what code 128 of an 8-bit row, or 8 of a 4-bit one, stands for, by its scale and bias
+template <int ROWS = 8>
+__device__ __forceinline__ float middle(uint32_t pair) { return __builtin_fmaf(ROWS == 8 ? 128.0f : 8.0f, half_at(pair, 0), half_at(pair, 1)); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // tanh(x) / x = 1 - x^2/3 + 2 x^4/15 - ..., for |x| < TANH_SMALL to 2^-24 (the next term: 0.0036 x^12)
 constexpr float TANH_SMALL = 0.35f;
@@ -228,36 +241,42 @@ __device__ __forceinline__ uint32_t inclusive_sum(uint32_t v, int lane) {
   return v;
 }
 
-// ROWS8: rows of the 8-bit format. DP: columns the code is laid out for; FULL: dim is DP, else less: lanes that would have the
+// ROWS: bits of an element: 16, or 8 or 4 in rows with a scale and bias. DP: columns the code is laid out for; FULL: dim is DP, else less: lanes that would have the
 // columns behind read the row's first ones in their place, which meet zeros in the queries or make outputs that nobody wants.
-// PAGE16: pages are whole 16-token tiles, whose addresses are then the same for the wave. PACKED (FULL 8-bit rows, PAGE16): the
+// PAGE16: pages are whole 16-token tiles, whose addresses are then the same for the wave. PACKED (FULL rows of codes, PAGE16): the
 // rows of a page's tokens follow each other without gaps. 16 of them are then read as one run of bytes, every line by one
 // load and marked as read once, and go through LDS, where a lane finds its pieces: 262 143 tokens 103 us, 118 with a gap
 // of 4 bytes behind each row (two tiles ahead instead of one: 2 % more); 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, 400 us, 459 with gaps.
-template <bool BF16, bool ROWS8, int DP, bool FULL, bool PAGE16, bool PACKED>
+template <bool BF16, int ROWS, int DP, bool FULL, bool PAGE16, bool PACKED>
 struct Attention {
+  static constexpr bool ROWS8 = ROWS == 8, ROWS4 = ROWS == 4, CODES = ROWS8 || ROWS4;
   static constexpr int KP = DP / 32;                   // products of a key tile
   static constexpr int HALVES = DP > 128 ? 2 : 1;      // pieces of a value row that a lane holds
   static constexpr int VC = DP / 16 / HALVES;          // columns of a piece: 8, or 4 of DP = 64
-  static constexpr int EL = ROWS8 ? 1 : 2;             // bytes of an element
-  static constexpr int HEAD = ROWS8 ? 4 : 0;           // of a row, in front of its elements
-  static constexpr bool PBF16 = ROWS8 ? true : BF16;   // type of the weights: scales go into them, so 8-bit rows take bf16's range
+  static constexpr int bytes_of(int elements) { return elements * ROWS / 8; }
+  static constexpr int HEAD = CODES ? 4 : 0;           // of a row, in front of its elements
+  static constexpr int ROW = HEAD + bytes_of(DP);      // bytes of a FULL row
+  static constexpr bool PBF16 = CODES ? true : BF16;   // type of the weights: scales go into them, so rows of codes take bf16's range
   static constexpr float SHIFT = PBF16 ? 0.0f : 14.0f; // weights are 2^SHIFT times larger
-  static constexpr int VREGS = ROWS8 ? (VC + 3) / 4 : VC / 2; // registers of a value piece
-  static constexpr int KREGS = ROWS8 ? 2 : 4;          // registers of a key piece
+  static constexpr int VREGS = ROWS4 ? 1 : ROWS8 ? (VC + 3) / 4 : VC / 2; // registers of a value piece (4 bits, DP = 64: a word that two lanes share)
+  // Registers of a key piece. A product takes 8 elements of a lane: of 4-bit rows a word, and a lane's words of a row follow each other
+  static constexpr int KREGS = ROWS4 ? (FULL ? (KP < 4 ? KP : 4) : 1) : ROWS8 ? 2 : 4;
+  static constexpr int KPIECES = ROWS4 ? KP / KREGS : KP;
+  static constexpr int KEY_STEP = ROWS4 ? 4 * KREGS : bytes_of(32); // bytes from a lane's piece to its next one
+  static constexpr int WEIGHT_UP = ROWS4 ? 80 : 0;     // 4-bit rows: weights are 2^80 times larger for the products, whose other operands are subnormal
   static constexpr int DEPTH = 1;                      // tiles loaded ahead
-  static constexpr int KEY_AUX = ROWS8 || DP == 64 ? 0 : READ_ONCE, VALUE_AUX = ROWS8 ? 0 : READ_ONCE;
+  static constexpr int KEY_AUX = CODES || DP == 64 ? 0 : READ_ONCE, VALUE_AUX = CODES ? 0 : READ_ONCE;
 
-  static constexpr int RUN = 16 * (DP * EL + HEAD);    // PACKED: bytes of 16 rows
+  static constexpr int RUN = 16 * ROW;                 // PACKED: bytes of 16 rows
   static constexpr int RUN_LOADS = RUN / 1024;         // a wave's loads of one, but for its last 64 bytes
   static_assert(!PACKED || RUN == RUN_LOADS * 1024 + 64, "16 rows of 64, 128 or 256 bytes and a header each");
   static constexpr int STAGE = PACKED ? 4 * RUN : 16;  // bytes of LDS a wave stages a tile in: keys' two runs, values' two
 
   // a lane's part of 32 tokens
   struct Rows {
-    uint32_t k[2][KP][KREGS];
+    uint32_t k[2][KPIECES][KREGS];
     uint32_t v[HALVES][8][VREGS];
-    uint32_t k_pair[ROWS8 ? 8 : 1], v_pair[ROWS8 ? 8 : 1];
+    uint32_t k_pair[CODES ? 8 : 1], v_pair[CODES ? 8 : 1];
   };
   // the same as bytes in a row: keys' runs, values' runs, and the last 64 bytes of the four in lanes 0 .. 15
   struct Runs {
@@ -285,15 +304,17 @@ struct Attention {
 
   __device__ __forceinline__ Attention(const AttentionArgs& args, int lane_, char* stage_)
       : a(args), lane(lane_), n(lane_ & 15), g(lane_ >> 4), stage(stage_) {
-    key_lane = HEAD + 8 * g * EL;
-    value_lane = HEAD + (FULL || n * VC < a.dim ? n * VC * EL : 0);
+    key_lane = HEAD + (ROWS4 ? 4 * KP * g : bytes_of(8 * g));
+    value_lane = HEAD + (FULL || n * VC < a.dim ? bytes_of(n * VC) & ~(ROWS4 ? 3 : 0) : 0);
     key_rows = n * (uint32_t)a.key.slot_stride + key_lane;
     value_rows = 4 * g * (uint32_t)a.value.slot_stride + value_lane;
   }
 
   // bytes from the lane's first piece to the next ones
-  __device__ __forceinline__ uint32_t key_piece(int i) const { return FULL || 32 * i + 8 * g < a.dim ? 32 * i * EL : 0u - 8 * g * EL; }
-  __device__ __forceinline__ uint32_t value_piece(int h) const { return FULL || h == 0 || 128 * h + n * VC < a.dim ? 128 * h * EL : 0u; }
+  __device__ __forceinline__ uint32_t key_piece(int i) const { return FULL || element_of(i) < a.dim ? KEY_STEP * i : HEAD - key_lane; }
+  __device__ __forceinline__ uint32_t value_piece(int h) const { return FULL || h == 0 || 128 * h + n * VC < a.dim ? bytes_of(128 * h) : 0u; }
+  // the first of the lane's 8 elements of product c
+  __device__ __forceinline__ int element_of(int c) const { return ROWS4 ? 8 * (KP * g + c) : 32 * c + 8 * g; }
 
   __device__ __forceinline__ int token_of(int j) const { return (j >> 2) * 16 + 4 * g + (j & 3); } // of this lane's values and scores, in the tile
 
@@ -317,8 +338,8 @@ struct Attention {
   __device__ __forceinline__ void load(Tile& tile, int t0, const Pages& pages, bool any) const {
     typedef __attribute__((ext_vector_type(KREGS))) uint32_t key_t;
     typedef __attribute__((ext_vector_type(VREGS))) uint32_t value_t;
-    typedef key_t __attribute__((aligned(ROWS8 ? 4 : 16))) stored_key; // 8-bit rows begin on 4 bytes
-    typedef value_t __attribute__((aligned(ROWS8 ? 4 : 2 * VC))) stored_value;
+    typedef key_t __attribute__((aligned(CODES ? 4 : 16))) stored_key; // rows of codes begin on 4 bytes
+    typedef value_t __attribute__((aligned(CODES ? 4 : 2 * VC))) stored_value;
     tile.partial = t0 < span.lo || t0 + ATT_TILE > span.end;
     tile.seen = 0xff;
     [[maybe_unused]] const auto key = [&](auto& tile, int h, int i, const char* p) {
@@ -377,16 +398,16 @@ struct Attention {
         const auto vb = rows_at(value_base + (block * a.value.block_stride + in_block * a.value.slot_stride), any);
         const uint32_t ks = (uint32_t)a.key.slot_stride, vs = (uint32_t)a.value.slot_stride;
 #pragma unroll
-        for (int i = 0; i < KP; ++i) fetch<KEY_AUX>(tile.k[h][i], kb, key_rows + (FULL ? 0 : key_piece(i)), 0, FULL ? 32 * i * EL : 0);
-        if (ROWS8) {
+        for (int i = 0; i < KPIECES; ++i) fetch<KEY_AUX>(tile.k[h][i], kb, key_rows + (FULL ? 0 : key_piece(i)), 0, FULL ? KEY_STEP * i : 0);
+        if (CODES) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) tile.k_pair[4 * h + j] = __builtin_amdgcn_raw_buffer_load_b32(kb, 4 * g * ks, j * ks, 0);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
-          for (int c = 0; c < HALVES; ++c) fetch<VALUE_AUX>(tile.v[c][4 * h + j], vb, value_rows + (FULL ? 0 : value_piece(c)), j * vs, FULL ? 128 * c * EL : 0);
-          if (ROWS8) tile.v_pair[4 * h + j] = __builtin_amdgcn_raw_buffer_load_b32(vb, 4 * g * vs, j * vs, 0);
+          for (int c = 0; c < HALVES; ++c) fetch<VALUE_AUX>(tile.v[c][4 * h + j], vb, value_rows + (FULL ? 0 : value_piece(c)), j * vs, FULL ? bytes_of(128 * c) : 0);
+          if (CODES) tile.v_pair[4 * h + j] = __builtin_amdgcn_raw_buffer_load_b32(vb, 4 * g * vs, j * vs, 0);
         }
       }
     } else {
@@ -410,23 +431,23 @@ struct Attention {
       for (int h = 0; h < 2; ++h) {
         const char* p = reinterpret_cast<const char*>((uint64_t)low[h] | ((uint64_t)high[h] << 32)) + key_lane;
 #pragma unroll
-        for (int i = 0; i < KP; ++i) key(tile, h, i, p + (int32_t)key_piece(i));
+        for (int i = 0; i < KPIECES; ++i) key(tile, h, i, p + (int32_t)key_piece(i));
       }
       const bool fours = a.block_size % 4 == 0; // four tokens in a row share a page: the first one's row is enough
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const char *kr = nullptr, *vr;
         if (fours) {
-          if (ROWS8) kr = row(kt, token_of(j & 4)) + (j & 3) * a.key.slot_stride;
+          if (CODES) kr = row(kt, token_of(j & 4)) + (j & 3) * a.key.slot_stride;
           vr = row(vt, token_of(j & 4)) + (j & 3) * a.value.slot_stride;
         } else {
-          if (ROWS8) kr = row(kt, token_of(j));
+          if (CODES) kr = row(kt, token_of(j));
           vr = row(vt, token_of(j));
         }
         if ((bads >> token_of(j)) & 1) tile.seen &= ~(1u << j);
 #pragma unroll
         for (int c = 0; c < HALVES; ++c) value(tile, c, j, vr + value_lane + value_piece(c));
-        if (ROWS8) {
+        if (CODES) {
           tile.k_pair[j] = *reinterpret_cast<const uint32_t*>(kr);
           tile.v_pair[j] = *reinterpret_cast<const uint32_t*>(vr);
         }
@@ -446,22 +467,26 @@ struct Attention {
   float q_sum;
   f32x4 acc[HALVES][VC];
   float m, l, bias;
+  // 4-bit rows: exponent of a sum of codes by queries; and the products of code 8, which is taken off afterwards, at even and at odd columns
+  int q_up;
+  f32x4 eights[2];
 
   __device__ __forceinline__ void begin(int32_t request, int head, int q0, int rows) {
     q_sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < KP; ++c) {
       q[c] = make_uint4(0, 0, 0, 0);
-      const int d = 32 * c + 8 * g;
+      const int d = element_of(c);
       if (n < rows && d < a.dim)
         q[c] = *reinterpret_cast<const uint4*>(a.query + request * a.query_request_stride + (int64_t)(head * a.group + q0 + n) * a.query_head_stride + d * 2);
-      if (ROWS8) {
+      if (CODES) {
         const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) q_sum += unpack16<BF16>(w[i], 0) + unpack16<BF16>(w[i], 1);
       }
     }
-    if (ROWS8) {
+    if constexpr (ROWS4) order_queries();
+    if (CODES) {
       q_sum += __shfl_xor(q_sum, 16, 64);
       q_sum += __shfl_xor(q_sum, 32, 64);
     }
@@ -469,8 +494,41 @@ struct Attention {
     for (int h = 0; h < HALVES; ++h)
 #pragma unroll
       for (int i = 0; i < VC; ++i) acc[h][i] = f32x4{0, 0, 0, 0};
+    eights[0] = eights[1] = f32x4{0, 0, 0, 0};
     m = -__builtin_inff();
     l = bias = 0.0f;
+  }
+
+  // 4-bit rows: the queries' elements in the codes' order. bf16: the largest is brought to 2^100, so that products with subnormal
+  // numbers are normal ones (an exact step, but for elements 2^-220 times smaller), and odd elements are 2^-4 of that
+  __device__ __forceinline__ void order_queries() {
+    q_up = 20; // 16 * 2^-24 a step
+    int e = 0;
+    if constexpr (BF16) {
+      float most = 0.0f;
+#pragma unroll
+      for (int c = 0; c < KP; ++c) {
+        const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = __builtin_fmaxf(most, __builtin_fmaxf(__builtin_fabsf(unpack16<BF16>(w[i], 0)), __builtin_fabsf(unpack16<BF16>(w[i], 1))));
+      }
+      e = 100 - __builtin_amdgcn_frexp_expf(group_max(most)); // (of 0, inf and NaN: 100)
+      q_up = 133 - e;
+    }
+#pragma unroll
+    for (int c = 0; c < KP; ++c) {
+      const uint4 w = q[c];
+      uint32_t t[4] = {__builtin_amdgcn_perm(w.z, w.x, 0x05040100u), __builtin_amdgcn_perm(w.z, w.x, 0x07060302u),
+                       __builtin_amdgcn_perm(w.w, w.y, 0x05040100u), __builtin_amdgcn_perm(w.w, w.y, 0x07060302u)};
+      if constexpr (BF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int up = i & 1 ? e - 4 : e;
+          t[i] = pack_bf16(__builtin_amdgcn_ldexpf(unpack16<BF16>(t[i], 0), up), __builtin_amdgcn_ldexpf(unpack16<BF16>(t[i], 1), up));
+        }
+      }
+      q[c] = make_uint4(t[0], t[1], t[2], t[3]);
+    }
   }
 
   // PACKED: a lane's part of the runs, through LDS, where no other wave looks. Lanes read what others wrote: that the wave's
@@ -494,14 +552,13 @@ struct Attention {
       if (lane < 16)
         *reinterpret_cast<piece_t*>(stage + (n >> 2) * RUN + RUN_LOADS * 1024 + (n & 3) * 16) = piece_t{loaded.last[0], loaded.last[1], loaded.last[2], loaded.last[3]};
       wave_sync();
-      constexpr int ROW = DP * EL + HEAD;
       const char *keys = stage, *values = stage + 2 * RUN;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < KP; ++i)
+        for (int i = 0; i < KPIECES; ++i)
 #pragma unroll
-          for (int r = 0; r < KREGS; ++r) rows.k[h][i][r] = *reinterpret_cast<const uint32_t*>(keys + (16 * h + n) * ROW + HEAD + 32 * i + 8 * g + 4 * r);
+          for (int r = 0; r < KREGS; ++r) rows.k[h][i][r] = *reinterpret_cast<const uint32_t*>(keys + (16 * h + n) * ROW + key_lane + KEY_STEP * i + 4 * r);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         rows.k_pair[j] = *reinterpret_cast<const uint32_t*>(keys + token_of(j) * ROW);
@@ -509,7 +566,7 @@ struct Attention {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-          for (int r = 0; r < VREGS; ++r) rows.v[h][j][r] = *reinterpret_cast<const uint32_t*>(values + token_of(j) * ROW + HEAD + 128 * h + n * VC + 4 * r);
+          for (int r = 0; r < VREGS; ++r) rows.v[h][j][r] = *reinterpret_cast<const uint32_t*>(values + token_of(j) * ROW + value_lane + bytes_of(128 * h) + 4 * r);
       }
     }
   }
@@ -532,13 +589,15 @@ struct Attention {
       f32x4 r = {0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < KP; ++i) {
-        const auto& k = tile.k[h][i];
-        if constexpr (ROWS8) r = product<BF16>(widen<BF16>(k[0], k[1]), q[i], r);
+        const auto& k = tile.k[h][ROWS4 ? i / KREGS : i];
+        if constexpr (ROWS4) r = product<BF16>(codes4<BF16>(k[i % KREGS]), q[i], r);
+        else if constexpr (ROWS8) r = product<BF16>(widen<BF16>(k[0], k[1]), q[i], r);
         else r = product<BF16>(make_uint4(k[0], k[1], k[2], k[3]), q[i], r);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float y = r[j];
+        if (ROWS4) y = __builtin_fmaf(half_at(tile.k_pair[4 * h + j], 0), __builtin_amdgcn_ldexpf(y, q_up), half_at(tile.k_pair[4 * h + j], 1) * q_sum);
         if (ROWS8) y = __builtin_fmaf(half_at(tile.k_pair[4 * h + j], 0), y, (BF16 ? half_at(tile.k_pair[4 * h + j], 1) : middle(tile.k_pair[4 * h + j])) * q_sum);
         s[4 * h + j] = y * a.scale;
       }
@@ -558,7 +617,7 @@ struct Attention {
         const uint32_t keep = (uint32_t)((int32_t)(seen << (31 - j)) >> 31); // all bits or none
         s[j] = keep ? s[j] : -__builtin_inff();
         // what a row without a token holds may be anything: its weight of 0 would not hide it
-        if (ROWS8) {
+        if (CODES) {
           tile.v_pair[j] &= keep;
         } else {
 #pragma unroll
@@ -583,6 +642,10 @@ struct Attention {
       for (int h = 0; h < HALVES; ++h)
 #pragma unroll
         for (int i = 0; i < VC; ++i) acc[h][i] *= f;
+      if (ROWS4) {
+        eights[0] *= f;
+        eights[1] *= f;
+      }
     }
     const float ref = m == -__builtin_inff() ? 0.0f : m - SHIFT; // nothing seen yet: all weights 0
     float p[8];
@@ -591,16 +654,21 @@ struct Attention {
       p[j] = exp2_fast(s[j] - ref);
       l += p[j];
     }
-    if (ROWS8) {
+    if (CODES) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        bias = __builtin_fmaf(p[j], middle(tile.v_pair[j]), bias);
+        bias = __builtin_fmaf(p[j], middle<ROWS>(tile.v_pair[j]), bias);
         p[j] *= half_at(tile.v_pair[j], 0);
+        if (ROWS4) p[j] = __builtin_amdgcn_ldexpf(p[j], WEIGHT_UP);
       }
     }
     uint4 hi, lo;
     split<PBF16>(p, hi, lo);
     // ---- values ----
+    if constexpr (ROWS4) {
+      add_codes4(tile, hi, lo);
+      return;
+    }
     if constexpr (ROWS8) {
 #pragma unroll
       for (int h = 0; h < HALVES; ++h)
@@ -627,6 +695,45 @@ struct Attention {
         acc[h][i] = product<PBF16>(col, hi, acc[h][i]);
         acc[h][i] = product<PBF16>(col, lo, acc[h][i]);
       }
+  }
+
+  // 4-bit values: a byte holds two neighbouring columns. The bytes of two tokens go side by side, the low codes are the even column's
+  // operand and the high ones the odd column's, 16 times larger
+  __device__ __forceinline__ void add_codes4(Rows& tile, uint4 hi, uint4 lo) {
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+      for (int i = 0; i < VC; i += 2) {
+        uint32_t even[4], odd[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a0 = tile.v[h][2 * j][0], a1 = tile.v[h][2 * j + 1][0];
+          if (VC == 4) { // two lanes share a word
+            a0 >>= 16 * (n & 1);
+            a1 >>= 16 * (n & 1);
+          }
+          const uint32_t both = __builtin_amdgcn_perm(a1, a0, 0x0c040c00u + 0x00010001u * (i / 2)); // (0x0c: a zero)
+          even[j] = both & 0x000f000fu;
+          odd[j] = both & 0x00f000f0u;
+        }
+        const uint4 c0 = make_uint4(even[0], even[1], even[2], even[3]), c1 = make_uint4(odd[0], odd[1], odd[2], odd[3]);
+        acc[h][i] = product_bf16(c0, hi, acc[h][i]);
+        acc[h][i] = product_bf16(c0, lo, acc[h][i]);
+        acc[h][i + 1] = product_bf16(c1, hi, acc[h][i + 1]);
+        acc[h][i + 1] = product_bf16(c1, lo, acc[h][i + 1]);
+      }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t eight = k ? 0x00800080u : 0x00080008u;
+      const uint4 column = make_uint4(eight, eight, eight, eight);
+      eights[k] = product_bf16(column, hi, eights[k]);
+      eights[k] = product_bf16(column, lo, eights[k]);
+    }
+  }
+  // what has come together at a column, but for the common bias
+  __device__ __forceinline__ float sum_at(int h, int i, int r) const {
+    if constexpr (ROWS4) return __builtin_amdgcn_ldexpf(acc[h][i][r] - eights[i & 1][r], 133 - WEIGHT_UP - 4 * (i & 1));
+    return acc[h][i][r];
   }
 
   // Tiles first, first + STEP, ... up to last. The rows of the DEPTH next ones are on their way while one is added, and the pages of
@@ -682,9 +789,9 @@ __device__ __forceinline__ void write_out(const AttentionArgs& a, int64_t at, in
   if (d == 0) a.lse[at] = s.l == 0.0f ? -__builtin_inff() : (s.m - shift + __builtin_amdgcn_logf(s.l)) * (1.0f / ATT_LOG2E);
 }
 
-template <bool BF16, bool ROWS8, int DP, bool FULL, bool PAGE16, bool PACKED>
+template <bool BF16, int ROWS, int DP, bool FULL, bool PAGE16, bool PACKED>
 __global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP)) void paged_attention_kernel(const AttentionArgs a) {
-  using A = Attention<BF16, ROWS8, DP, FULL, PAGE16, PACKED>;
+  using A = Attention<BF16, ROWS, DP, FULL, PAGE16, PACKED>;
   constexpr int THREADS = 64 * ATT_WAVES;
   __shared__ __attribute__((aligned(16))) float s_acc[ATT_WAVES][ATTENTION_ROWS][DP + 4];
   __shared__ float s_ml[ATT_WAVES][ATTENTION_ROWS][2];
@@ -768,7 +875,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP)) void paged
     const int n = x.n, g = x.g;
     x.l += __shfl_xor(x.l, 16, 64);
     x.l += __shfl_xor(x.l, 32, 64);
-    if (ROWS8) {
+    if (A::CODES) {
       x.bias += __shfl_xor(x.bias, 16, 64);
       x.bias += __shfl_xor(x.bias, 32, 64);
     }
@@ -781,7 +888,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP)) void paged
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < A::VC; ++i) s_acc[wave][n][h * 128 + (4 * g + r) * A::VC + i] = x.acc[h][i][r] + x.bias;
+        for (int i = 0; i < A::VC; ++i) s_acc[wave][n][h * 128 + (4 * g + r) * A::VC + i] = x.sum_at(h, i, r) + x.bias;
     const bool whole = s.c0 == 0 && s.c1 == s.steps;
     __syncthreads();
     const auto each_four = [&](auto&& f) { // f(query, first of four columns)
@@ -856,38 +963,39 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const Attenti
   write_out<BF16>(a, first + row, d, sum, shift);
 }
 
-template <bool BF16, bool ROWS8, int DP, bool FULL>
+template <bool BF16, int ROWS, int DP, bool FULL>
 void launch_kernel(const AttentionArgs& a, hipStream_t stream) {
   const dim3 grid(a.workers), block(64 * ATT_WAVES);
   if (a.block_size % 16) {
-    paged_attention_kernel<BF16, ROWS8, DP, FULL, false, false><<<grid, block, 0, stream>>>(a);
+    paged_attention_kernel<BF16, ROWS, DP, FULL, false, false><<<grid, block, 0, stream>>>(a);
     return;
   }
-  if constexpr (ROWS8 && FULL) {
-    if (a.key.slot_stride == DP + 4 && a.value.slot_stride == DP + 4) {
-      paged_attention_kernel<BF16, ROWS8, DP, FULL, true, true><<<grid, block, 0, stream>>>(a);
+  if constexpr (ROWS < 16 && FULL && !(ROWS == 4 && DP == 64)) {
+    constexpr int ROW = DP * ROWS / 8 + 4;
+    if (a.key.slot_stride == ROW && a.value.slot_stride == ROW) {
+      paged_attention_kernel<BF16, ROWS, DP, FULL, true, true><<<grid, block, 0, stream>>>(a);
       return;
     }
   }
-  paged_attention_kernel<BF16, ROWS8, DP, FULL, true, false><<<grid, block, 0, stream>>>(a);
+  paged_attention_kernel<BF16, ROWS, DP, FULL, true, false><<<grid, block, 0, stream>>>(a);
 }
 
-template <bool BF16, bool ROWS8, int DP>
+template <bool BF16, int ROWS, int DP>
 hipError_t launch_dp(const AttentionArgs& a, hipStream_t stream) {
-  if (a.dim == DP) launch_kernel<BF16, ROWS8, DP, true>(a, stream);
-  else launch_kernel<BF16, ROWS8, DP, false>(a, stream);
+  if (a.dim == DP) launch_kernel<BF16, ROWS, DP, true>(a, stream);
+  else launch_kernel<BF16, ROWS, DP, false>(a, stream);
   if (hipError_t e = hipGetLastError()) return e;
   if (a.max_tokens <= ATT_STEP - 15) return hipSuccess; // a pair is one step: nobody shares it
   const int rows = a.group < ATTENTION_ROWS ? a.group : ATTENTION_ROWS, groups = (rows + 256 / DP - 1) / (256 / DP);
-  paged_attention_join_kernel<BF16, DP><<<a.workers * groups, 256, 0, stream>>>(a, groups, ROWS8 || BF16 ? 0.0f : 14.0f);
+  paged_attention_join_kernel<BF16, DP><<<a.workers * groups, 256, 0, stream>>>(a, groups, ROWS < 16 || BF16 ? 0.0f : 14.0f);
   return hipGetLastError();
 }
 
-template <bool BF16, bool ROWS8>
+template <bool BF16, int ROWS>
 hipError_t launch_any(const AttentionArgs& a, hipStream_t stream) {
-  if (a.dim <= 64) return launch_dp<BF16, ROWS8, 64>(a, stream);
-  if (a.dim <= 128) return launch_dp<BF16, ROWS8, 128>(a, stream);
-  return launch_dp<BF16, ROWS8, 256>(a, stream);
+  if (a.dim <= 64) return launch_dp<BF16, ROWS, 64>(a, stream);
+  if (a.dim <= 128) return launch_dp<BF16, ROWS, 128>(a, stream);
+  return launch_dp<BF16, ROWS, 256>(a, stream);
 }
 
 } // namespace attention

@@ -2,5 +2,5 @@
 #include "paged_attention.h"
 
 namespace fbgemm_amd {
-hipError_t launch_paged_attention_bf16(const AttentionArgs& a, hipStream_t stream) { return attention::launch_any<true, false>(a, stream); }
+hipError_t launch_paged_attention_bf16(const AttentionArgs& a, hipStream_t stream) { return attention::launch_any<true, 16>(a, stream); }
 } // namespace fbgemm_amd

@@ -1,0 +1,221 @@
+// Rotary positions: a head's first 2 * pairs elements as pairs (a, b), elements (p, p + pairs) or
+// neighbours (2 p, 2 p + 1), turned by the angle  position * frequency_p:
+//
+//   a' = m (a cos - b sin),  b' = m (b cos + a sin)
+//
+// and the rest of the head as it is. In fp32, rounded once.
+//
+// Angles are taken in fp64, as quarters of a turn: what is left of a far position's angle behind its whole
+// quarters is off by 2^-53 of the angle, in fp32 it would be 2^-24 of it (262 143 radians: 0.02). Sine and
+// cosine of the rest, at most pi/4, are their series.
+//
+// Bound by memory: every element is read once and written once. A workgroup has one or a few tokens: it
+// makes their sines once, in LDS, and turns all heads of queries and keys by them, 16 bytes (two of them,
+// where a pair's elements are apart) a thread at a time.
+#include "decode.h"
+
+namespace fbgemm_amd {
+
+namespace {
+
+constexpr int THREADS = 256;
+typedef __attribute__((ext_vector_type(4))) uint32_t piece16;
+
+struct Turn {
+  float cosine, sine;
+};
+// of position * frequency
+__device__ __forceinline__ Turn turn_of(double position, double frequency, float magnitude, float sine_magnitude) {
+  const double quarters = position * (frequency * 0.63661977236758134308); // 2 / pi
+  const double whole = __builtin_rint(quarters);
+  const int quadrant = (int)(int64_t)(whole - 4.0 * __builtin_floor(whole * 0.25));
+  const float x = (float)(quarters - whole) * 1.5707963267948966f, z = x * x;
+  // to z^4 and z^5: the next terms are below 2^-29 at pi/4
+  float s = 1.0f / 362880.0f, c = -1.0f / 3628800.0f;
+  s = __builtin_fmaf(s, z, -1.0f / 5040.0f);
+  s = __builtin_fmaf(s, z, 1.0f / 120.0f);
+  s = __builtin_fmaf(s, z, -1.0f / 6.0f);
+  s = __builtin_fmaf(s * z, x, x);
+  c = __builtin_fmaf(c, z, 1.0f / 40320.0f);
+  c = __builtin_fmaf(c, z, -1.0f / 720.0f);
+  c = __builtin_fmaf(c, z, 1.0f / 24.0f);
+  c = __builtin_fmaf(c, z, -0.5f);
+  c = __builtin_fmaf(c, z, 1.0f);
+  const float sine = quadrant & 1 ? c : s, cosine = quadrant & 1 ? s : c;
+  return Turn{(quadrant == 1 || quadrant == 2 ? -cosine : cosine) * magnitude, (quadrant & 2 ? -sine : sine) * sine_magnitude};
+}
+
+// the sines of a workgroup's tokens
+__device__ __forceinline__ void make_turns(const RotateArgs& a, int64_t first, int tokens, Turn* turns) {
+  for (int i = threadIdx.x; i < tokens * a.pairs; i += THREADS) {
+    const int t = i / a.pairs;
+    const int64_t position = a.idx64 ? reinterpret_cast<const int64_t*>(a.positions)[first + t] : reinterpret_cast<const int32_t*>(a.positions)[first + t];
+    turns[i] = turn_of((double)position, a.frequencies[i - t * a.pairs], a.magnitude, a.sine);
+  }
+  __syncthreads();
+}
+
+// Elements of 16 bytes as fp32, and back
+template <int TY>
+struct Chunk {
+  static constexpr int N = TY == ST_FP32 ? 4 : 8;
+  static constexpr int BYTES = 16 / N;
+  static __device__ __forceinline__ float get(const piece16& w, int e) {
+    if constexpr (TY == ST_FP32) return __builtin_bit_cast(float, (uint32_t)w[e]);
+    else if constexpr (TY == ST_BF16) return __builtin_bit_cast(float, e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e / 2] >> (e % 2 * 16)));
+  }
+  // elements e and e + 1
+  static __device__ __forceinline__ void put(piece16& w, int e, float x, float y) {
+    if constexpr (TY == ST_FP32) {
+      w[e] = __builtin_bit_cast(uint32_t, x);
+      w[e + 1] = __builtin_bit_cast(uint32_t, y);
+    } else if constexpr (TY == ST_BF16) {
+      typedef __attribute__((ext_vector_type(2))) __bf16 pair_t;
+      const pair_t v = {(__bf16)x, (__bf16)y};
+      w[e / 2] = __builtin_bit_cast(uint32_t, v);
+    } else {
+      typedef __attribute__((ext_vector_type(2))) _Float16 pair_t;
+      const pair_t v = {(_Float16)x, (_Float16)y};
+      w[e / 2] = __builtin_bit_cast(uint32_t, v);
+    }
+  }
+  static __device__ __forceinline__ float at(const char* p) {
+    if constexpr (TY == ST_FP32) return *reinterpret_cast<const float*>(p);
+    else if constexpr (TY == ST_BF16) return __builtin_bit_cast(float, (uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16);
+    else return (float)*reinterpret_cast<const _Float16*>(p);
+  }
+  static __device__ __forceinline__ void set(char* p, float x) {
+    if constexpr (TY == ST_FP32) *reinterpret_cast<float*>(p) = x;
+    else if constexpr (TY == ST_BF16) *reinterpret_cast<__bf16*>(p) = (__bf16)x;
+    else *reinterpret_cast<_Float16*>(p) = (_Float16)x;
+  }
+};
+// (fp32 numbers, said to the compiler: it would else round some, not all, products of fp16 numbers to fp16 at once, and
+// results would go by how rows are aligned)
+__device__ __forceinline__ float rounded(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ float first_of(float a, float b, Turn t) { return rounded(__builtin_fmaf(a, t.cosine, -(b * t.sine))); }
+__device__ __forceinline__ float second_of(float a, float b, Turn t) { return rounded(__builtin_fmaf(b, t.cosine, a * t.sine)); }
+
+// where a unit's head is, and its number in it
+struct Place {
+  const char* in;
+  char* out;
+  int token, unit;
+  bool same; // out is in
+};
+__device__ __forceinline__ Place place_of(const RotateArgs& a, int64_t first, uint32_t item) {
+  Place p;
+  const uint32_t row = divide(item, a.units);
+  p.unit = (int)(item - row * a.units.d);
+  p.token = (int)divide(row, a.all_heads);
+  int head = (int)(row - p.token * a.all_heads.d);
+  const int k = head >= a.heads[0];
+  if (k) head -= a.heads[0];
+  p.in = a.in[k] + (first + p.token) * a.in_token[k] + head * a.in_head[k];
+  p.out = a.out[k] + (first + p.token) * a.out_token[k] + head * a.out_head[k];
+  p.same = p.in == p.out;
+  return p;
+}
+
+// Rows of whole 16-byte pieces on 16-byte boundaries, and pairs that fill whole pieces
+template <int TY, bool INTERLEAVED>
+__device__ __forceinline__ void turn_piece(const RotateArgs& a, const Place& p, const Turn* turns) {
+  using C = Chunk<TY>;
+  constexpr int N = C::N;
+  const int turning = INTERLEAVED ? 2 * a.pairs / N : a.pairs / N; // units; the others are pieces of the rest, behind all pairs
+  if (p.unit >= turning) {
+    if (p.same) return;
+    const int at = 2 * a.pairs * C::BYTES + (p.unit - turning) * 16;
+    *reinterpret_cast<piece16*>(p.out + at) = *reinterpret_cast<const piece16*>(p.in + at);
+  } else if constexpr (INTERLEAVED) {
+    const Turn* turn = turns + p.token * a.pairs + p.unit * (N / 2);
+    piece16 w = *reinterpret_cast<const piece16*>(p.in + p.unit * 16);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const float x = C::get(w, e), y = C::get(w, e + 1);
+      C::put(w, e, first_of(x, y, turn[e / 2]), second_of(x, y, turn[e / 2]));
+    }
+    *reinterpret_cast<piece16*>(p.out + p.unit * 16) = w;
+  } else {
+    const Turn* turn = turns + p.token * a.pairs + p.unit * N;
+    const int other = a.pairs * C::BYTES;
+    piece16 v = *reinterpret_cast<const piece16*>(p.in + p.unit * 16), w = *reinterpret_cast<const piece16*>(p.in + p.unit * 16 + other);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const float x0 = C::get(v, e), x1 = C::get(v, e + 1), y0 = C::get(w, e), y1 = C::get(w, e + 1);
+      C::put(v, e, first_of(x0, y0, turn[e]), first_of(x1, y1, turn[e + 1]));
+      C::put(w, e, second_of(x0, y0, turn[e]), second_of(x1, y1, turn[e + 1]));
+    }
+    *reinterpret_cast<piece16*>(p.out + p.unit * 16) = v;
+    *reinterpret_cast<piece16*>(p.out + p.unit * 16 + other) = w;
+  }
+}
+
+// Any others: a pair, or an element of the rest
+template <int TY>
+__device__ __forceinline__ void turn_element(const RotateArgs& a, const Place& p, const Turn* turns) {
+  using C = Chunk<TY>;
+  if (p.unit < a.pairs) {
+    const int e = (a.interleaved ? 2 * p.unit : p.unit) * C::BYTES, f = e + (a.interleaved ? 1 : a.pairs) * C::BYTES;
+    const float x = C::at(p.in + e), y = C::at(p.in + f);
+    const Turn turn = turns[p.token * a.pairs + p.unit];
+    C::set(p.out + e, first_of(x, y, turn));
+    C::set(p.out + f, second_of(x, y, turn));
+  } else if (!p.same) {
+    const int e = (p.unit + a.pairs) * C::BYTES; // behind the pairs' second elements
+    if constexpr (TY == ST_FP32) *reinterpret_cast<uint32_t*>(p.out + e) = *reinterpret_cast<const uint32_t*>(p.in + e);
+    else *reinterpret_cast<uint16_t*>(p.out + e) = *reinterpret_cast<const uint16_t*>(p.in + e);
+  }
+}
+
+enum { ELEMENTS, HALVES, NEIGHBOURS };
+template <int TY, int FORM>
+__global__ __launch_bounds__(THREADS) void rotate_positions_kernel(const RotateArgs a) {
+  extern __shared__ Turn s_turns[];
+  for (int64_t first = (int64_t)blockIdx.x * a.token_group; first < a.tokens; first += (int64_t)gridDim.x * a.token_group) {
+    const int tokens = (int)(a.tokens - first < a.token_group ? a.tokens - first : a.token_group);
+    __syncthreads(); // the last group's turns have been read
+    make_turns(a, first, tokens, s_turns);
+    const uint32_t items = (uint32_t)tokens * a.all_heads.d * a.units.d;
+    for (uint32_t i = threadIdx.x; i < items; i += THREADS) {
+      const Place p = place_of(a, first, i);
+      if constexpr (FORM == ELEMENTS) turn_element<TY>(a, p, s_turns);
+      else turn_piece<TY, FORM == NEIGHBOURS>(a, p, s_turns);
+    }
+  }
+}
+
+template <int TY>
+void launch(RotateArgs a, bool aligned16, hipStream_t stream) {
+  constexpr int N = Chunk<TY>::N;
+  // queries and keys share a piece's place in a head
+  const bool pieces = aligned16 && a.dim % N == 0 && (a.interleaved ? 2 * a.pairs : a.pairs) % N == 0;
+  const int rest = a.dim - 2 * a.pairs;
+  const int units = pieces ? (a.interleaved ? 2 * a.pairs / N : a.pairs / N) + rest / N : a.pairs + rest;
+  const int heads = a.heads[0] + a.heads[1];
+  a.units = make_divisor((uint32_t)units);
+  a.all_heads = make_divisor((uint32_t)heads);
+  // Four tokens a workgroup where the device is full all the same
+  a.token_group = a.tokens >= 8192 ? 4 : 1;
+  const int64_t groups = (a.tokens + a.token_group - 1) / a.token_group;
+  const unsigned grid = (unsigned)(groups < (1 << 22) ? groups : 1 << 22);
+  const size_t lds = (size_t)a.token_group * a.pairs * sizeof(Turn);
+  if (!pieces) rotate_positions_kernel<TY, ELEMENTS><<<grid, THREADS, lds, stream>>>(a);
+  else if (a.interleaved) rotate_positions_kernel<TY, NEIGHBOURS><<<grid, THREADS, lds, stream>>>(a);
+  else rotate_positions_kernel<TY, HALVES><<<grid, THREADS, lds, stream>>>(a);
+}
+
+} // namespace
+
+hipError_t launch_rotate_positions(const RotateArgs& a, int32_t ty, bool aligned16, hipStream_t stream) {
+  if (ty == ST_FP32) launch<ST_FP32>(a, aligned16, stream);
+  else if (ty == ST_FP16) launch<ST_FP16>(a, aligned16, stream);
+  else launch<ST_BF16>(a, aligned16, stream);
+  return hipGetLastError();
+}
+
+} // namespace fbgemm_amd

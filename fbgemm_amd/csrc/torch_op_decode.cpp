@@ -2,86 +2,14 @@
 // the reference's operators of the quantized-embedding path: namespace fbgemm_amd. torch owns
 // tensors and streams; all work goes through the C ABI of include/fbgemm_amd.h. What a call
 // returns and its scratch come from torch's allocator, for the current stream.
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/library.h>
-
 #include <algorithm>
 #include <cmath>
 #include <limits>
-#include <optional>
 #include <tuple>
 
-#include "../../include/fbgemm_amd.h"
+#include "torch_op_decode.h"
 
 namespace {
-
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-
-void* current_stream(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-
-#define CHECK_CALL(call)                                              \
-  do {                                                                \
-    const int rc_ = (int)(call);                                      \
-    TORCH_CHECK(rc_ == 0, "fbgemm_amd: ", fbgemm_amd_last_error());   \
-  } while (0)
-
-void on_device(const Tensor& t, const Tensor& like, const char* name) {
-  TORCH_CHECK(t.device() == like.device(), "fbgemm_amd: ", name, " must be on ", like.device(), ", got ", t.device());
-}
-int32_t index_bits(const Tensor& t, const char* name) {
-  TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, "fbgemm_amd: ", name, " must be int32 or int64");
-  return t.scalar_type() == at::kLong ? 64 : 32;
-}
-void list_of(const Tensor& t, int64_t numel, const Tensor& like, at::ScalarType type, const char* name) {
-  on_device(t, like, name);
-  TORCH_CHECK(t.scalar_type() == type, "fbgemm_amd: ", name, " must be ", type, ", got ", t.scalar_type());
-  TORCH_CHECK(t.dim() == 1 && t.size(0) == numel, "fbgemm_amd: ", name, " must hold ", numel, " entries, got ", t.sizes());
-  TORCH_CHECK(t.is_contiguous(), "fbgemm_amd: ", name, " must be contiguous");
-}
-int32_t float_type(at::ScalarType t, const char* name) {
-  TORCH_CHECK(t == at::kFloat || t == at::kHalf || t == at::kBFloat16, "fbgemm_amd: ", name, " must be float32, float16 or bfloat16, got ", t);
-  return t == at::kFloat ? FBGEMM_AMD_FP32 : t == at::kHalf ? FBGEMM_AMD_FP16 : FBGEMM_AMD_BF16;
-}
-// a dimension of one entry (or none) has no stride worth looking at
-int64_t stride_of(const Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
-void rows_dense(const Tensor& t, const char* name) {
-  TORCH_CHECK(t.numel() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1, "fbgemm_amd: the elements of a row of ", name, " must be next to each other");
-}
-void* status_pointer(const OptTensor& status, const Tensor& like) {
-  if (!status.has_value()) return nullptr;
-  on_device(*status, like, "status");
-  TORCH_CHECK(status->is_contiguous() && status->nbytes() >= FBGEMM_AMD_STATUS_BYTES, "fbgemm_amd: status must be a block of ", FBGEMM_AMD_STATUS_BYTES, " bytes");
-  return status->data_ptr();
-}
-void* pointer(const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; }
-
-fbgemm_amd_paged_cache cache_of(const Tensor& key_cache, const Tensor& value_cache, int64_t dim) {
-  TORCH_CHECK(key_cache.dim() == 4 && value_cache.dim() == 4, "fbgemm_amd: a cache is [blocks, heads, block_size, row], got ", key_cache.sizes(),
-              " and ", value_cache.sizes());
-  TORCH_CHECK(key_cache.sizes() == value_cache.sizes() && key_cache.scalar_type() == value_cache.scalar_type(),
-              "fbgemm_amd: keys and values must have caches of the same shape and type");
-  on_device(value_cache, key_cache, "value_cache");
-  rows_dense(key_cache, "key_cache");
-  rows_dense(value_cache, "value_cache");
-  const bool rows8 = key_cache.scalar_type() == at::kByte;
-  TORCH_CHECK(key_cache.size(3) == (rows8 ? dim + 4 : dim) || (rows8 && key_cache.size(3) > dim + 4), "fbgemm_amd: rows of ", key_cache.size(3),
-              " do not hold ", dim, " elements", rows8 ? " and a scale and bias" : "");
-  TORCH_CHECK(key_cache.size(1) <= 0x7fffffff && key_cache.size(2) <= 0x7fffffff && dim <= 0x7fffffff, "fbgemm_amd: cache too large");
-  fbgemm_amd_paged_cache c;
-  c.row_ty = rows8 ? FBGEMM_AMD_INT8 : float_type(key_cache.scalar_type(), "a cache that is not uint8");
-  c.blocks = key_cache.size(0);
-  c.heads = (int32_t)key_cache.size(1);
-  c.block_size = (int32_t)key_cache.size(2);
-  c.dim = (int32_t)dim;
-  for (int k = 0; k < 3; ++k) {
-    c.key_strides[k] = stride_of(key_cache, k);
-    c.value_strides[k] = stride_of(value_cache, k);
-  }
-  return c;
-}
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> kv_block_tables(
     const Tensor& lengths, const Tensor& new_tokens, Tensor block_tables, const Tensor& free_blocks, const Tensor& free_start,
@@ -111,7 +39,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> kv_block_tables(
   return {slots, positions, offsets, total, next};
 }
 
-void kv_cache_append(const Tensor& key, const Tensor& value, Tensor key_cache, Tensor value_cache, const Tensor& slots, const OptTensor& status) {
+void kv_cache_append(const Tensor& key, const Tensor& value, Tensor key_cache, Tensor value_cache, const Tensor& slots, const OptTensor& status,
+                     int64_t row_bits) {
   TORCH_CHECK(key.dim() == 3 && key.sizes() == value.sizes() && key.scalar_type() == value.scalar_type(),
               "fbgemm_amd: key and value must be [tokens, heads, dim] of one type, got ", key.sizes(), " and ", value.sizes());
   on_device(value, key, "value");
@@ -119,7 +48,7 @@ void kv_cache_append(const Tensor& key, const Tensor& value, Tensor key_cache, T
   rows_dense(key, "key");
   rows_dense(value, "value");
   list_of(slots, key.size(0), key, at::kLong, "slots");
-  const fbgemm_amd_paged_cache cache = cache_of(key_cache, value_cache, key.size(2));
+  const fbgemm_amd_paged_cache cache = cache_of(key_cache, value_cache, key.size(2), row_bits);
   TORCH_CHECK(key.size(1) == cache.heads, "fbgemm_amd: key has ", key.size(1), " heads, its cache ", cache.heads);
   const int64_t ks[2] = {stride_of(key, 0), stride_of(key, 1)}, vs[2] = {stride_of(value, 0), stride_of(value, 1)};
   const c10::OptionalDeviceGuard guard(key.device());
@@ -130,13 +59,13 @@ void kv_cache_append(const Tensor& key, const Tensor& value, Tensor key_cache, T
 
 std::tuple<Tensor, Tensor> paged_attention(
     const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& block_tables, const Tensor& lengths,
-    std::optional<double> scale, int64_t window, double softcap) {
+    std::optional<double> scale, int64_t window, double softcap, int64_t row_bits) {
   TORCH_CHECK(query.dim() == 3, "fbgemm_amd: query must be [requests, heads, dim], got ", query.sizes());
   rows_dense(query, "query");
   const int64_t B = query.size(0), heads = query.size(1), dim = query.size(2);
   TORCH_CHECK(dim > 0, "fbgemm_amd: dim must be positive");
   on_device(key_cache, query, "key_cache");
-  const fbgemm_amd_paged_cache cache = cache_of(key_cache, value_cache, dim);
+  const fbgemm_amd_paged_cache cache = cache_of(key_cache, value_cache, dim, row_bits);
   list_of(lengths, B, query, lengths.scalar_type(), "lengths");
   on_device(block_tables, query, "block_tables");
   TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.size(0) == B,
@@ -213,9 +142,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> kv_block_tables_meta(
   return {at::empty({num_tokens}, wide), at::empty({num_tokens}, wide), at::empty({lengths.size(0) + 1}, narrow), at::empty_like(lengths),
           at::empty({1}, narrow)};
 }
-void kv_cache_append_meta(const Tensor&, const Tensor&, Tensor, Tensor, const Tensor&, const OptTensor&) {}
+void kv_cache_append_meta(const Tensor&, const Tensor&, Tensor, Tensor, const Tensor&, const OptTensor&, int64_t) {}
 std::tuple<Tensor, Tensor> paged_attention_meta(
-    const Tensor& query, const Tensor&, const Tensor&, const Tensor&, const Tensor&, std::optional<double>, int64_t, double) {
+    const Tensor& query, const Tensor&, const Tensor&, const Tensor&, const Tensor&, std::optional<double>, int64_t, double, int64_t) {
   return {at::empty(query.sizes(), query.options()), at::empty({query.size(0), query.size(1)}, query.options().dtype(at::kFloat))};
 }
 Tensor penalize_logits_new(
@@ -248,9 +177,9 @@ TORCH_LIBRARY_FRAGMENT(fbgemm_amd, m) {
   m.def(
       "kv_block_tables(Tensor lengths, Tensor new_tokens, Tensor(a!) block_tables, Tensor free_blocks, Tensor free_start, int block_size, int num_tokens, Tensor(b!)? status=None) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def(
-      "kv_cache_append(Tensor key, Tensor value, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor slots, Tensor(c!)? status=None) -> ()");
+      "kv_cache_append(Tensor key, Tensor value, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor slots, Tensor(c!)? status=None, int row_bits=8) -> ()");
   m.def(
-      "paged_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_tables, Tensor lengths, float? scale=None, int window=0, float softcap=0.0) -> (Tensor, Tensor)");
+      "paged_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_tables, Tensor lengths, float? scale=None, int window=0, float softcap=0.0, int row_bits=8) -> (Tensor, Tensor)");
   m.def(
       "penalize_logits(Tensor logits, Tensor? tokens=None, Tensor? offsets=None, Tensor? prompt_lengths=None, Tensor? repetition=None, Tensor? frequency=None, Tensor? presence=None, Tensor? bias_ids=None, Tensor? bias_values=None, Tensor? bias_offsets=None, Tensor? mask=None) -> Tensor");
   m.def(

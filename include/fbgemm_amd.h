@@ -605,9 +605,12 @@ int fbgemm_amd_kv_block_tables(
 /* Keys and values are two arrays [blocks][heads][block_size][row]; strides (blocks,
  * heads, slots) in elements of storage (INT8: bytes), a row's elements next to each
  * other. INT8 rows are the table-batched operator's: fp16 scale, fp16 bias, dim bytes
- * (dim + 4 bytes, on 4-byte boundaries). */
+ * (dim + 4 bytes, on 4-byte boundaries). CACHE_INT4 rows are its 4-bit ones: scale and
+ * bias, then two elements a byte, the first in the low bits (dim / 2 + 4 bytes, strides
+ * in bytes, on 4-byte boundaries too; dim is even). */
+enum { FBGEMM_AMD_CACHE_INT4 = 16 }; /* a cache's row_ty alone: a table's type is no cache's */
 typedef struct fbgemm_amd_paged_cache {
-  int32_t row_ty;     /* FBGEMM_AMD_FP32/FP16/BF16/INT8 */
+  int32_t row_ty;     /* FBGEMM_AMD_FP32/FP16/BF16/INT8, FBGEMM_AMD_CACHE_INT4 */
   int32_t block_size; /* tokens of a block */
   int32_t heads, dim; /* of keys and values */
   int64_t blocks;
@@ -617,8 +620,8 @@ typedef struct fbgemm_amd_paged_cache {
 /* New rows into their slots: cache[slot / block_size][head][slot % block_size] = row.
  * d_key and d_value are [tokens][heads][dim] with the strides (tokens, heads) given in
  * elements. A cache of FP32 / FP16 / BF16 rows takes rows of its own type as they are;
- * an INT8 cache takes any of the three and stores what fbgemm_amd_quantize_rowwise
- * (bit_rate 8, sb_float 0, FBGEMM_AMD_QLAYOUT_TBE) makes of them, with elements beyond
+ * an INT8 or CACHE_INT4 cache takes any of the three and stores what fbgemm_amd_quantize_rowwise
+ * (bit_rate 8 or 4, sb_float 0, FBGEMM_AMD_QLAYOUT_TBE) makes of them, with elements beyond
  * fp16's range at its end and NaN as 0 (a zero bias may have either sign). Slot -1 is
  * skipped; another slot outside the cache too, and is recorded in d_status (may be
  * NULL) as INDEX_OUT_OF_RANGE with the token's number. Slots differ from each other
@@ -629,6 +632,41 @@ int fbgemm_amd_kv_cache_append(
     const fbgemm_amd_paged_cache* cache, const void* d_key, const void* d_value, int32_t input_ty, int64_t tokens,
     const int64_t* key_strides, const int64_t* value_strides, const int64_t* d_slots, void* d_key_cache, void* d_value_cache,
     void* d_status, void* stream);
+
+/* Rows of requests' tokens, out of their pages into dense arrays d_key and d_value
+ * [tokens][heads][dim] on 16-byte boundaries: what attention of a prompt's later part
+ * reads of its earlier one. Token i belongs to the request r with d_offsets[r] <= i <
+ * d_offsets[r + 1] (requests + 1 entries, ascending, int32 or int64 by index_bits) and is at position
+ * d_starts[r] + i - d_offsets[r] of it (d_starts NULL: 0). Rows come as they are, in the cache's type;
+ * INT8 and CACHE_INT4 rows as the values they stand for, scale * code + bias, in
+ * FP32, FP16 or BF16. A token whose block the table or the cache does not have is zeros, and is
+ * recorded in d_status (may be NULL) as INDEX_OUT_OF_RANGE with its number; tokens
+ * from d_offsets[requests] on are zeros. table_width * block_size is below 2^31. */
+int fbgemm_amd_kv_cache_read(
+    const fbgemm_amd_paged_cache* cache, const void* d_key_cache, const void* d_value_cache, const int32_t* d_block_tables,
+    int64_t table_stride, int64_t table_width, const void* d_offsets, const void* d_starts, int32_t index_bits, int64_t requests,
+    int64_t tokens, int32_t output_ty, void* d_key, void* d_value, void* d_status, void* stream);
+
+/* Rows [tokens][heads][dim] that go in and come out; strides (tokens, heads) in elements */
+typedef struct fbgemm_amd_head_rows {
+  const void* in;
+  void* out; /* may be in, with the same strides */
+  int64_t in_strides[2], out_strides[2];
+  int32_t heads;
+} fbgemm_amd_head_rows;
+
+/* Queries and keys turned by their positions (rotary positions). Of the first 2 * pairs
+ * elements of a head pair p is (p, p + pairs), or with `interleaved` (2 p, 2 p + 1):
+ *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin) of position * d_frequencies[p]
+ * (radians, fp64); the elements behind them stay as they are. With `inverse` the other
+ * way round, with the same magnitude: the way a gradient takes. d_positions [tokens],
+ * int32 or int64 by index_bits; FP32, FP16 or BF16 rows, in fp32 and rounded once;
+ * angles in fp64. pairs: at most 1024; `key` may be NULL. What is written must not
+ * overlap what else is read or written. */
+int fbgemm_amd_rotate_positions(
+    const fbgemm_amd_head_rows* query, const fbgemm_amd_head_rows* key, int32_t ty, int64_t tokens, int32_t dim,
+    const void* d_positions, int32_t index_bits, const double* d_frequencies, int32_t pairs, int32_t interleaved,
+    float magnitude, int32_t inverse, void* stream);
 
 /* Attention of one new token per request. d_query [requests][query_heads][dim] (FP16
  * or BF16; strides in elements, rows on 16-byte boundaries), query head h reads key
@@ -644,7 +682,7 @@ int fbgemm_amd_kv_cache_append(
  * outputs not finite; a score of -inf weighs 0. Tokens of a block are less than 64 MiB
  * apart. A
  * cache of FP16 / BF16 rows must have the queries' type and rows on 16-byte boundaries,
- * one of INT8 rows goes with either. dim: a multiple of 8, at most 256;
+ * one of INT8 or CACHE_INT4 rows goes with either. dim: a multiple of 8, at most 256;
  * requests * heads * table_width * block_size below some 2^37. Scores, weights
  * and sums are fp32 (weights go to the matrix cores as two 16-bit numbers); results do
  * not depend on the order in which workgroups run. d_workspace: scratch of
@@ -674,6 +712,26 @@ int fbgemm_amd_penalize_logits(
     int64_t tokens_numel, const void* d_offsets, const void* d_prompt_lengths, int32_t index_bits, const float* d_repetition,
     const float* d_frequency, const float* d_presence, const void* d_bias_ids, const float* d_bias_values, int64_t bias_numel,
     const void* d_bias_offsets, const int32_t* d_mask, int64_t mask_stride, void* d_output, int64_t output_stride, void* stream);
+
+/* A token of every row of logits [rows][vocab] (FP32, FP16 or BF16), drawn by a number
+ * d_uniform[row] in [0, 1). With tokens in order, larger logits first, equal ones by
+ * number, and w = exp((x - max) / temperature), those that may be drawn are the first
+ * top_k; of these the fewest first ones whose w add up to top_p times the sum of all of
+ * these (one at least); of these the ones with w >= min_p. d_tokens[row] is the
+ * first of them, by number, where the running sum of w is above uniform times the whole
+ * (or the last one), d_log_probability[row] the logarithm of its w over the whole. Of
+ * the four lists, one number per row, each may be NULL: temperature 1, top_k and min_p
+ * 0, top_p 1. top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 leave every token (min_p
+ * >= 1: those of the largest logit); with a temperature or top_p that is not above 0 it
+ * is the first of the largest ones, of probability 1. NaN and -inf are never drawn,
+ * +inf counts as the largest finite fp32 number; a row with nothing else gives -1 and
+ * -inf. Sums are of whole numbers, w in units of 2^-(62 - bits of vocab) at most: a draw
+ * is that of exact sums but within some 2^-40 of a border of two tokens. vocab: 1..2^20,
+ * rows up to 2^24; a row stride of 0 shares the logits. */
+int fbgemm_amd_sample_tokens(
+    const void* d_logits, int32_t logits_ty, int64_t rows, int64_t vocab, int64_t logits_stride, const float* d_uniform,
+    const float* d_temperature, const int32_t* d_top_k, const float* d_top_p, const float* d_min_p, int64_t* d_tokens,
+    float* d_log_probability, void* stream);
 
 /* Wait for everything enqueued on `stream` (hipStreamSynchronize), for callers
  * of the asynchronous entry points that hold no HIP headers. */
