@@ -13,14 +13,19 @@
 // A large vocabulary has a border of two tokens within 1e-6 of almost every u, so sums in fp32 would often draw a
 // neighbour. w is a whole number here, 2^fraction times larger and rounded (fraction: 45 bits for
 // 131 071 tokens): sums of whole numbers are the same in any order, so lanes, waves and LDS atomics add them as they come,
-// and a running sum is off by no more than the w's own roundings, some 2^-46 of the largest each. exp is made in fp64 (2^-52).
+// and a running sum is off by no more than the w's own roundings, some 2^-46 of the largest each. exp is made in fp64 (2^-48).
 //
-// A workgroup has a row, a wave a run of its tokens, in their order. Passes over the row: the largest logit; then the tokens that
-// can matter at all (top-k: the k-th largest of the threads' largest logits is a bound that few others pass; else weights that
-// are not 0, or min-p) are put in a list in LDS, if it holds them, and what follows are passes over the list, else over
-// the row again, out of the caches. Where the order matters (which of equal ones is within top-k, top-p's sum) the first part
-// is found by counting: bins of keys (fp32 bits in ascending order), the bin where the count or sum is reached, bins of that
-// bin's keys, until a bin is one key; then the last token of that key that is within.
+// A workgroup has a row. It reads it once to keep the largest logit of every few pieces of 16 bytes, in LDS. Few of these groups
+// hold a token that can matter: with top-k those whose largest is above the k-th largest of the groups' largest, without those with a
+// weight that is not 0, or enough for min-p. Where a list in LDS takes the tokens of those groups, everything else is done there:
+// up to SMALL of them are ranked against each other, more are counted into bins (below). Else (top-p of a flat row) the whole
+// row is weighed once, a wave a run of its tokens, into bins of logits of its own, which say the bin where top-p's sum is reached
+// and the run where the draw falls; only that bin's tokens and that run are looked at again.
+//
+// Finding where a count or a sum is reached, going down from the largest, by bins: of keys (fp32 bits in ascending order), then of
+// the keys of the bin that has it, until they are one; then the last token of that key that is within.
+#include <type_traits>
+
 #include "decode.h"
 #include "logits_piece.h"
 
@@ -41,144 +46,287 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ float logit_of(uint32_t key) { return __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
+// 2^(i / 32)
+constexpr int STEPS = 32;
+__device__ const double ROOTS[STEPS] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+};
+
 // exp((x - most) / temperature) in units of 2^-fraction
 struct Weights {
   double most, per_logit; // per_logit: log2(e) / temperature
   int fraction;
+  const double* roots;    // ROOTS, in LDS: 32 entries lie in different banks
+  // x: not +inf; of NaN and -inf: 0
   __device__ __forceinline__ u64 operator()(float x) const {
-    const double t = ((double)__builtin_fminf(x, FLT_BIG) - most) * per_logit;
-    if (!(t > -(double)(fraction + 2))) return 0;
-    const double whole = __builtin_rint(t), f = t - whole;
-    // 2^f, |f| <= 1/2, by its series: the next term is below 2^-52
-    constexpr double C[12] = {0.6931471805599453094,  0.2402265069591007123,  0.05550410866482157995, 0.009618129107628477162, 0.001333355814642844342, 1.540353039338160995e-4,
-                              1.525273380405984028e-5, 1.321548679014430949e-6, 1.017808600923969973e-7, 7.054911620801123329e-9, 4.445538271870811498e-10, 2.567843599348820514e-11};
-    double p = C[11];
-#pragma unroll
-    for (int i = 10; i >= 0; --i) p = __builtin_fma(p, f, C[i]);
-    p = __builtin_fma(p, f, 1.0);
+    // (no branches: weights next to each other are made together)
+    const double t = fmax(((double)x - most) * per_logit, -(double)(fraction + 2));
+    // a sum with 1.5 * 2^47 is rounded to 32nds, and holds their number in its low bits
+    constexpr double ROUND = 211106232532992.0;
+    const double steps = t + ROUND, f = t - (steps - ROUND);
+    const int n = (int)(uint32_t)__builtin_bit_cast(u64, steps);
+    // 2^f, |f| <= 1/64, by its series: the next term is below 2^-48
+    double p = 0.0013333558146428443;
+    p = __builtin_fma(p, f, 0.009618129107628477);
+    p = __builtin_fma(p, f, 0.0555041086648215799);
+    p = __builtin_fma(p, f, 0.2402265069591007123);
+    p = __builtin_fma(p, f, 0.6931471805599453094);
+    const double root = roots[n & (STEPS - 1)];
+    p = __builtin_fma(p * f, root, root);
+    // times 2^(whole steps + fraction), in the exponent's bits (0.9 < p < 2.1, and the exponent stays that of a normal number)
+    u64 bits = __builtin_bit_cast(u64, p);
+    bits += (u64)(uint32_t)(((n >> 5) + fraction) << 20) << 32;
     // a double of 2^52 and more holds whole numbers: adding that rounds, and leaves the number in the low bits
-    const double w = __builtin_ldexp(p, (int)whole + fraction) + 4503599627370496.0;
-    return __builtin_bit_cast(u64, w) & 0xfffffffffffffull;
+    return __builtin_bit_cast(u64, __builtin_bit_cast(double, bits) + 4503599627370496.0) & 0xfffffffffffffull;
   }
 };
 
-__device__ __forceinline__ u64 shfl_up64(u64 v, int d) {
-  return (u64)__shfl_up((uint32_t)v, d, 64) | ((u64)__shfl_up((uint32_t)(v >> 32), d, 64) << 32);
+// Running sums and maxima over a wave by its rows' permutations, which take an instruction each, not a way through LDS: over rows of 16,
+// then a row's last lane into the next row, then the first half's into the second
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) { // 0 where nothing comes
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ u64 shfl_xor64(u64 v, int d) {
-  return (u64)__shfl_xor((uint32_t)v, d, 64) | ((u64)__shfl_xor((uint32_t)(v >> 32), d, 64) << 32);
+template <typename T, typename F>
+__device__ __forceinline__ T wave_running(T v, F&& with) {
+  v = with(v, std::integral_constant<int, 0x111>(), std::integral_constant<int, 0xf>()); // row_shr 1, 2, 4, 8
+  v = with(v, std::integral_constant<int, 0x112>(), std::integral_constant<int, 0xf>());
+  v = with(v, std::integral_constant<int, 0x114>(), std::integral_constant<int, 0xf>());
+  v = with(v, std::integral_constant<int, 0x118>(), std::integral_constant<int, 0xf>());
+  v = with(v, std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>()); // row_bcast 15 into rows 1 and 3
+  return with(v, std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>()); // row_bcast 31 into rows 2 and 3
 }
-__device__ __forceinline__ u64 wave_sum(u64 v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += shfl_xor64(v, d);
-  return v;
+__device__ __forceinline__ u64 wave_inclusive(u64 v) {
+  return wave_running(v, [](u64 x, auto ctrl, auto rows) {
+    return x + ((u64)moved<decltype(ctrl)::value, decltype(rows)::value>((uint32_t)x) | ((u64)moved<decltype(ctrl)::value, decltype(rows)::value>((uint32_t)(x >> 32)) << 32));
+  });
 }
-__device__ __forceinline__ u64 wave_inclusive(u64 v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const u64 o = shfl_up64(v, d);
-    v += lane >= d ? o : 0;
-  }
-  return v;
+__device__ __forceinline__ uint32_t wave_inclusive32(uint32_t v) {
+  return wave_running(v, [](uint32_t x, auto ctrl, auto rows) { return x + moved<decltype(ctrl)::value, decltype(rows)::value>(x); });
 }
-__device__ __forceinline__ u64 last_lane(u64 v) { // (readlane gives an int)
-  return (u64)(uint32_t)__builtin_amdgcn_readlane((uint32_t)v, 63) | ((u64)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), 63) << 32);
-}
+// (readlane gives an int)
+__device__ __forceinline__ uint32_t last_lane32(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
+__device__ __forceinline__ u64 last_lane(u64 v) { return (u64)last_lane32((uint32_t)v) | ((u64)last_lane32((uint32_t)(v >> 32)) << 32); }
+__device__ __forceinline__ u64 wave_sum(u64 v) { return last_lane(wave_inclusive(v)); }
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t o = __shfl_xor(v, d, 64);
-    v = v > o ? v : o;
-  }
-  return v;
+  return last_lane32(wave_running(v, [](uint32_t x, auto ctrl, auto rows) {
+    const uint32_t o = moved<decltype(ctrl)::value, decltype(rows)::value>(x);
+    return x > o ? x : o;
+  }));
 }
 
-// What may be drawn: keys above `key`, and of that key the tokens up to `last`
+// Orders of numbers of a type: keys of different ones are more than 2^GRAIN apart
+template <int TY>
+constexpr int GRAIN = TY == ST_FP32 ? 0 : TY == ST_BF16 ? 15 : 12;
+
+// What may be drawn: keys above `hi`, and of those in [lo, hi], which are one, the tokens up to `last`
 struct Part {
-  uint32_t key;
+  uint32_t lo, hi;
   int32_t last;
-  __device__ __forceinline__ bool has(uint32_t k, int32_t token) const { return k > key || (k == key && token <= last); }
+  __device__ __forceinline__ bool has(uint32_t k, int32_t token) const { return k > hi || (k >= lo && token <= last); }
 };
 
-constexpr int THREADS = 1024, WAVES = THREADS / 64;
-constexpr int LIST = 448; // entries of a wave's part of the list
-struct Shared {
-  u64 weight[BINS];
-  uint32_t count[BINS];
+constexpr int GROUPS = 8192; // at most
+constexpr int RUN_BINS = 512;
+constexpr int FIRST_AHEAD = 8; // pieces that a thread loads together, where they come from memory
+
+template <int THREADS>
+struct alignas(16) Shared {
+  static constexpr int WAVES = THREADS / 64;
+  static constexpr int LIST = THREADS == 1024 ? 320 : 512; // entries of a wave's part of the list
+  static constexpr int MOST_GROUPS = THREADS == 1024 ? GROUPS : 1024;
+  static constexpr int SMALL = 512; // entries that are ranked
+  union {
+    struct {
+      u64 weight[BINS];
+      uint32_t count[BINS];
+    };
+    u64 run[WAVES][RUN_BINS]; // a run's weights, by bins of logits
+    struct {
+      u64 ranked[SMALL], amount[SMALL];
+      uint32_t small_key[SMALL];
+      int32_t small_token[SMALL], rank[SMALL];
+    };
+  };
+  uint32_t group[MOST_GROUPS]; // the largest key of each
+  uint16_t chosen[MOST_GROUPS];
+  double roots[STEPS];
   u64 sums[WAVES], wave[WAVES];
-  uint32_t wave32[WAVES];
+  uint32_t wave32[WAVES], low32[WAVES];
   u64 found;    // an amount
   uint32_t bin; // a place
+  uint32_t found_key;
   int32_t listed[WAVES];
   uint32_t key[WAVES * LIST];
   int32_t token[WAVES * LIST];
 };
 
-// The row in memory. A wave's tokens follow each other: `steps` times 64 pieces.
+__device__ __forceinline__ uint32_t group_lanes_max(uint32_t v, int lanes) { // over 1, 2, 4, 8, 16 or 32 lanes
+  const auto with = [&](uint32_t o) { v = v > o ? v : o; };
+  if (lanes > 1) with(__builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true));
+  if (lanes > 2) with(__builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true));
+  if (lanes > 4) with(__builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));
+  if (lanes > 8) with(__builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));
+  if (lanes > 16) with(__shfl_xor(v, 16, 64));
+  return v;
+}
+
+// The largest key of a piece. 16-bit numbers as whole numbers of the same order, two at a time; the order puts NaN behind infinity
+// (or below its negative): a piece with one such is looked at number by number.
 template <int TY>
+__device__ __forceinline__ uint32_t largest_of(const Piece<TY>& p) {
+  using P = Piece<TY>;
+  bool nan;
+  float x;
+  if constexpr (TY == ST_FP32) {
+    int32_t m = INT32_MIN;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int32_t b = (int32_t)p.raw[i], o = b ^ ((b >> 31) & 0x7fffffff);
+      m = m > o ? m : o;
+    }
+    nan = m > 0x7f800000;
+    x = __builtin_bit_cast(float, m ^ ((m >> 31) & 0x7fffffff));
+  } else {
+    typedef __attribute__((ext_vector_type(2))) int16_t pair_t;
+    pair_t m = {INT16_MIN, INT16_MIN};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const pair_t b = __builtin_bit_cast(pair_t, (uint32_t)p.raw[i]);
+      const uint32_t flip = __builtin_bit_cast(uint32_t, (pair_t)(b >> 15)) & 0x7fff7fffu;
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(pair_t, (uint32_t)p.raw[i] ^ flip));
+    }
+    const int16_t o = m[0] > m[1] ? m[0] : m[1];
+    nan = o > (TY == ST_BF16 ? 0x7f80 : 0x7c00);
+    const uint16_t b = (uint16_t)(o ^ ((o >> 15) & 0x7fff));
+    x = TY == ST_BF16 ? __builtin_bit_cast(float, (uint32_t)b << 16) : (float)__builtin_bit_cast(_Float16, b);
+  }
+  uint32_t k = key_of(x);
+  if (nan) {
+    k = 0;
+#pragma unroll 1
+    for (int i = 0; i < P::N; ++i) {
+      const uint32_t o = key_of(p.get(i));
+      k = k > o ? k : o;
+    }
+  }
+  return k;
+}
+
+// Pieces [first, first + pieces) of a row, a wave a run of `steps` times 64 of them
+template <int TY, int THREADS>
 struct Row {
   using P = Piece<TY>;
-  static constexpr int N = P::N, AHEAD = 4; // pieces that are loaded together
+  static constexpr int N = P::N, WAVES = THREADS / 64;
   const char* logits;
-  int32_t vocab;
+  int32_t vocab, first, pieces;
   int steps, lane, wave;
-  __device__ __forceinline__ Row(const SampleArgs& a, int64_t row)
-      : logits(reinterpret_cast<const char*>(a.logits) + row * a.stride * P::BYTES), vocab(a.vocab), lane(threadIdx.x & 63),
-        wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
-    steps = ((vocab + N - 1) / N + THREADS - 1) / THREADS;
+  __device__ __forceinline__ Row(const char* row, int32_t vocab_, int32_t first_, int32_t pieces_)
+      : logits(row), vocab(vocab_), first(first_), pieces(pieces_), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
+    steps = (pieces + THREADS - 1) / THREADS;
   }
-  // the first token of a lane's piece
-  __device__ __forceinline__ int32_t at(int step) const { return ((wave * steps + step) * 64 + lane) * N; }
+  __device__ __forceinline__ Row run(int w) const { // a wave's run, for all waves
+    const int32_t at = w * steps * 64, n = pieces - at;
+    return Row(logits, vocab, first + at, n < 0 ? 0 : n < steps * 64 ? n : steps * 64);
+  }
+  // a lane's piece
+  __device__ __forceinline__ int32_t piece_at(int step) const { return (wave * steps + step) * 64 + lane; }
+  __device__ __forceinline__ int32_t token_at(int step) const { return (first + piece_at(step)) * N; }
+  static __device__ __forceinline__ void load(P& p, const char* logits, int32_t v, int32_t vocab) {
+    if (v + N <= vocab) {
+      p.load(logits + (int64_t)v * P::BYTES);
+    } else { // behind the end: NaN, no token
+      p.raw[0] = p.raw[1] = p.raw[2] = p.raw[3] = 0xffffffffu;
+      if (v < vocab) {
+        const P some = [&] {
+          P q;
+          q.load_some(logits + (int64_t)v * P::BYTES, vocab - v);
+          return q;
+        }();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (TY == ST_FP32) p.raw[i] = i < vocab - v ? some.raw[i] : 0xffffffffu;
+          else p.raw[i] = (2 * i < vocab - v ? some.raw[i] & 0xffffu : 0xffffu) | (2 * i + 1 < vocab - v ? some.raw[i] & 0xffff0000u : 0xffff0000u);
+        }
+      }
+    }
+  }
   __device__ __forceinline__ void load(P& p, int step) const {
-    const int32_t v = at(step);
-    if (step < steps && v + N <= vocab) p.load(logits + (int64_t)v * P::BYTES);
-    else p.load_some(logits + (int64_t)v * P::BYTES, step < steps && v < vocab ? vocab - v : 0);
+    const int32_t i = piece_at(step);
+    load(p, logits, step < steps && i < pieces ? (first + i) * N : vocab, vocab);
   }
-  // f(logit, its token) for those of a lane's piece, in their order
+  // f(logit, its token) for those of a piece, in their order (two numbers' code: the piece is turned past them)
   template <typename F>
-  __device__ __forceinline__ void each_of(P p, int32_t v, F&& f) const {
+  static __device__ __forceinline__ void each_of(P p, int32_t v, F&& f) {
 #pragma unroll 1
-    for (int i = 0; i < N; i += 2) { // (two elements' code: the piece is turned past them)
-      if (v + i < vocab) f(p.get(0), v + i);
-      if (v + i + 1 < vocab) f(p.get(1), v + i + 1);
+    for (int i = 0; i < N; i += 2) {
+      f(p.get(0), v + i);
+      f(p.get(1), v + i + 1);
       if constexpr (TY == ST_FP32) p.raw[0] = p.raw[2], p.raw[1] = p.raw[3];
       else p.raw[0] = p.raw[1], p.raw[1] = p.raw[2], p.raw[2] = p.raw[3];
     }
   }
-  // f(piece, its first token), step by step; f may end it
-  template <typename F>
+  // f(piece, its first token, its number), step by step; several loads on their way, as long as all lanes have whole pieces
+  // (a load that goes to a register by one of two ways is waited for where they meet)
+  template <int AHEAD = 4, typename F>
   __device__ __forceinline__ void each_piece(F&& f) const {
-    for (int k = 0; k < steps; k += AHEAD) {
+    int whole = (vocab / N - first < pieces ? vocab / N - first : pieces) / 64 - wave * steps; // steps
+    whole = __builtin_amdgcn_readfirstlane(whole < steps ? whole : steps);
+    int k = 0;
+    for (; k + AHEAD <= whole; k += AHEAD) {
       P x[AHEAD];
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) load(x[j], k + j);
+      for (int j = 0; j < AHEAD; ++j) x[j].load(logits + (int64_t)token_at(k + j) * P::BYTES);
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j)
-        if (k + j < steps && !f(x[j], at(k + j))) return;
+      for (int j = 0; j < AHEAD; ++j) f(x[j], token_at(k + j), piece_at(k + j));
+    }
+    if constexpr (AHEAD > 4) {
+      for (; k + 4 <= whole; k += 4) {
+        P x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j].load(logits + (int64_t)token_at(k + j) * P::BYTES);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f(x[j], token_at(k + j), piece_at(k + j));
+      }
+    }
+    for (; k < steps; ++k) {
+      P x;
+      load(x, k);
+      f(x, token_at(k), piece_at(k));
     }
   }
-  // f(key, token, step) for a thread's tokens
+  // f(logit, token) for a thread's tokens (and NaN for what is none)
+  template <typename F>
+  __device__ __forceinline__ void each_logit(F&& f) const {
+    each_piece([&](const P& p, int32_t v, int32_t) { each_of(p, v, f); });
+  }
+  // f(key, token) for a thread's tokens (and key 0 for what is none)
   template <typename F>
   __device__ __forceinline__ void each(F&& f) const {
-    each_piece([&](const P& p, int32_t v) {
-      each_of(p, v, [&](float x, int32_t token) { f(key_of(x), token); });
-      return true;
-    });
+    each_piece([&](const P& p, int32_t v, int32_t) { each_of(p, v, [&](float x, int32_t token) { f(key_of(x), token); }); });
   }
   template <typename F>
   __device__ __forceinline__ void each_of_step(int step, F&& f) const {
     P p;
     load(p, step);
-    each_of(p, at(step), [&](float x, int32_t token) { f(key_of(x), token); });
+    each_of(p, token_at(step), [&](float x, int32_t token) { f(key_of(x), token); });
   }
 };
 
 // The list: a wave's entries, in their tokens' order
+template <int THREADS>
 struct List {
-  const Shared& s;
+  static constexpr int LIST = Shared<THREADS>::LIST;
+  const Shared<THREADS>& s;
   int steps, lane, wave, n;
-  __device__ __forceinline__ List(const Shared& shared)
-      : s(shared), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
+  __device__ __forceinline__ List(const Shared<THREADS>& shared) : s(shared), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
     n = __builtin_amdgcn_readfirstlane(s.listed[wave]);
     steps = (n + 63) / 64;
   }
@@ -193,80 +341,62 @@ struct List {
   }
 };
 
-// The tokens of keys >= lo, into the list; false: it does not hold them
-template <int TY>
-__device__ __forceinline__ bool make_list(const Row<TY>& row, Shared& s, uint32_t lo) {
-  int n = 0; // the same for the wave
-  row.each_piece([&](const auto& p, int32_t v) {
-    int mine = 0;
-    row.each_of(p, v, [&](float x, int32_t) { mine += key_of(x) >= lo; });
-    if (__builtin_amdgcn_ballot_w64(mine > 0) == 0) return true;
-    int to = mine;
+// A wave puts those of its 64 pieces' tokens with lo <= logit <= hi for which also(logit) into its part of the list, behind the n that are
+// there; the new n, or more than there is room for
+template <int TY, int THREADS, typename F>
+__device__ __forceinline__ int list_pieces(Shared<THREADS>& s, const Piece<TY>& p, int32_t v, int n, float lo, float hi, F&& also) {
+  constexpr int LIST = Shared<THREADS>::LIST, N = Piece<TY>::N;
+  const int wave = threadIdx.x >> 6;
+  uint32_t in = 0; // few are
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(to, d, 64);
-      to += row.lane >= d ? o : 0;
-    }
-    const int all = __builtin_amdgcn_readlane(to, 63);
-    if (n + all > LIST) {
-      n = LIST + 1;
-      return false;
-    }
-    int at = row.wave * LIST + n + to - mine;
-    if (mine > 0)
-      row.each_of(p, v, [&](float x, int32_t token) {
-        const uint32_t k = key_of(x);
-        if (k >= lo) {
-          s.key[at] = k;
-          s.token[at] = token;
-          ++at;
-        }
-      });
-    n += all;
-    return true;
-  });
-  if (row.lane == 0) s.listed[row.wave] = n;
-  return !__syncthreads_or(n > LIST);
-}
-
-__device__ __forceinline__ uint32_t block_max(Shared& s, uint32_t v) {
-  v = wave_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.wave32[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = s.wave32[0];
+  for (int e = 0; e < N; ++e) {
+    const float x = p.get(e);
+    in |= x >= lo && x <= hi ? 1u << e : 0u;
+  }
+  if (__builtin_amdgcn_ballot_w64(in != 0) == 0) return n;
+  const auto at = [&](int e) {
+    float x = p.get(0);
 #pragma unroll
-  for (int w = 1; w < WAVES; ++w) v = v > s.wave32[w] ? v : s.wave32[w];
-  return v;
+    for (int i = 1; i < N; ++i) x = e == i ? p.get(i) : x;
+    return x;
+  };
+  for (uint32_t left = in; left; left &= left - 1) {
+    const int e = __builtin_ctz(left);
+    if (!also(at(e))) in &= ~(1u << e);
+  }
+  const int mine = __builtin_popcount(in), to = (int)wave_inclusive32((uint32_t)mine), all = (int)last_lane32((uint32_t)to);
+  if (n + all > LIST) return LIST + 1;
+  int place = wave * LIST + n + to - mine;
+  for (; in; in &= in - 1) {
+    const int e = __builtin_ctz(in);
+    s.key[place] = key_of(at(e));
+    s.token[place] = v + e;
+    ++place;
+  }
+  return n + all;
 }
 
 // The first token, by number, where the running sum of amount(key, token) is above a target, which is asked for by the whole sum;
 // where that is the whole or more, the last one that has an amount. One has at least.
 struct Found {
   int32_t token;
+  uint32_t key;
   u64 amount, whole;
 };
-template <typename Source, typename F, typename T>
-__device__ __forceinline__ Found locate(const Source& from, Shared& s, F&& amount, T&& target_of) {
-  u64 mine = 0;
-  from.each([&](uint32_t k, int32_t v) { mine += amount(k, v); });
-  mine = wave_sum(mine);
-  __syncthreads();
-  if (from.lane == 0) s.sums[from.wave] = mine;
-  __syncthreads();
-  u64 whole = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) whole += s.sums[w];
-  u64 target = target_of(whole);
-  target = target < whole ? target : whole - 1;
+// of `from`, by its waves' sums
+template <typename Source, int THREADS, typename F>
+__device__ __forceinline__ Found locate_by(const Source& from, Shared<THREADS>& s, F&& amount, u64 mine, u64 whole, u64 target) {
   int in = 0;
   u64 before = 0;
-  for (; in < WAVES - 1 && before + s.sums[in] <= target; ++in) before += s.sums[in];
+  for (; in < THREADS / 64 - 1 && before + s.sums[in] <= target; ++in) before += s.sums[in];
   if (from.wave == in) {
     for (int k = 0; k < from.steps; ++k) {
-      u64 of_step = 0;
-      from.each_of_step(k, [&](uint32_t key, int32_t v) { of_step += amount(key, v); });
-      const u64 to = before + wave_inclusive(of_step, from.lane);
+      u64 of_step = mine; // of a single step they are known
+      if (from.steps > 1) {
+        of_step = 0;
+        from.each_of_step(k, [&](uint32_t key, int32_t v) { of_step += amount(key, v); });
+      }
+      const u64 to = before + wave_inclusive(of_step);
       const u64 above = __builtin_amdgcn_ballot_w64(target < to);
       if (above) {
         if (from.lane == __builtin_ctzll(above)) {
@@ -278,6 +408,7 @@ __device__ __forceinline__ Found locate(const Source& from, Shared& s, F&& amoun
             if (open && target < sum) {
               s.bin = (uint32_t)v;
               s.found = n;
+              s.found_key = key;
               open = false;
             }
           });
@@ -288,15 +419,44 @@ __device__ __forceinline__ Found locate(const Source& from, Shared& s, F&& amoun
     }
   }
   __syncthreads();
-  const Found r{(int32_t)s.bin, s.found, whole};
+  const Found r{(int32_t)s.bin, s.found_key, s.found, whole};
   __syncthreads();
+  return r;
+}
+// the waves' sums, and their whole
+template <int THREADS>
+__device__ __forceinline__ u64 sum_up(Shared<THREADS>& s, u64 mine) {
+  mine = wave_sum(mine);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s.sums[threadIdx.x >> 6] = mine;
+  __syncthreads();
+  u64 whole = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) whole += s.sums[w];
+  return whole;
+}
+template <typename Source, int THREADS, typename F, typename T>
+__device__ __forceinline__ Found locate(const Source& from, Shared<THREADS>& s, F&& amount, T&& target_of) {
+  u64 mine = 0;
+  from.each([&](uint32_t k, int32_t v) { mine += amount(k, v); });
+  const u64 whole = sum_up(s, mine);
+  const u64 target = target_of(whole);
+  return locate_by(from, s, amount, mine, whole, target < whole ? target : whole - 1);
+}
+// of a row, by its waves' sums in s.sums: the wave's run once more, by all waves
+template <int TY, int THREADS, typename F>
+__device__ __forceinline__ Found locate_in_run(const Row<TY, THREADS>& row, Shared<THREADS>& s, F&& amount, u64 whole, u64 target) {
+  int in = 0;
+  for (; in < THREADS / 64 - 1 && s.sums[in] <= target; ++in) target -= s.sums[in];
+  Found r = locate(row.run(in), s, amount, [&](u64) { return target; });
+  r.whole = whole;
   return r;
 }
 
 // s.bin: the first bin where the running sum reaches `target` (asked for by the whole; none does: the last one that is not empty); s.found: the sum
 // before it. The target.
-template <bool WEIGHTS, typename T>
-__device__ __forceinline__ u64 find_bin(Shared& s, T&& target_of) {
+template <bool WEIGHTS, int THREADS, typename T>
+__device__ __forceinline__ u64 find_bin(Shared<THREADS>& s, T&& target_of) {
   constexpr int EACH = BINS / THREADS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   u64 n[EACH], mine = 0;
@@ -305,11 +465,12 @@ __device__ __forceinline__ u64 find_bin(Shared& s, T&& target_of) {
     n[i] = WEIGHTS ? s.weight[threadIdx.x * EACH + i] : (u64)s.count[threadIdx.x * EACH + i];
     mine += n[i];
   }
-  const u64 to = wave_inclusive(mine, lane);
+  const u64 to = wave_inclusive(mine);
   if (lane == 63) s.wave[wave] = to;
   __syncthreads();
   u64 before = to - mine, whole = 0;
-  for (int w = 0; w < WAVES; ++w) {
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
     if (w < wave) before += s.wave[w];
     whole += s.wave[w];
   }
@@ -326,25 +487,33 @@ __device__ __forceinline__ u64 find_bin(Shared& s, T&& target_of) {
   __syncthreads();
   return target;
 }
+template <bool WEIGHTS, int THREADS>
+__device__ __forceinline__ void clear_bins(Shared<THREADS>& s) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < BINS; i += THREADS) {
+    if (WEIGHTS) s.weight[i] = 0;
+    else s.count[i] = 0;
+  }
+  __syncthreads();
+}
+// bins of keys from `hi` down to `lo`
+__device__ __forceinline__ int shift_of(uint32_t lo, uint32_t hi) {
+  const uint32_t span = hi - lo;
+  return span < BINS ? 0 : 32 - __builtin_clz(span) - 11;
+}
 
-// Keys from the largest, `hi`, down to `lo`, until the sum of their amounts reaches a target (at least 1), asked for by the whole: the key that
-// does it, the sum before it, the target. WEIGHTS: amounts are sums of u64, else 0 or 1.
+// Keys from the largest, `hi`, down to `lo`, until the sum of their amounts reaches a target (at least 1), asked for by the whole: the keys [lo,
+// hi], which are one, that do it, the sum before them, the target. WEIGHTS: amounts are sums of u64, else 0 or 1.
 struct Border {
-  uint32_t key;
+  uint32_t lo, hi;
   u64 before, target;
 };
-template <bool WEIGHTS, typename Source, typename F, typename T>
-__device__ __forceinline__ Border border(const Source& from, Shared& s, uint32_t lo, uint32_t hi, F&& amount, T&& target_of) {
-  Border b{0, 0, 0};
+template <bool WEIGHTS, int TY, typename Source, int THREADS, typename F, typename T>
+__device__ __forceinline__ Border border(const Source& from, Shared<THREADS>& s, uint32_t lo, uint32_t hi, F&& amount, T&& target_of) {
+  Border b{0, 0, 0, 0};
   for (bool first = true;; first = false) {
-    const uint32_t span = hi - lo;
-    const int shift = span < BINS ? 0 : 32 - __builtin_clz(span) - 11;
-    __syncthreads();
-    for (int i = threadIdx.x; i < BINS; i += THREADS) {
-      if (WEIGHTS) s.weight[i] = 0;
-      else s.count[i] = 0;
-    }
-    __syncthreads();
+    const int shift = shift_of(lo, hi);
+    clear_bins<WEIGHTS>(s);
     from.each([&](uint32_t k, int32_t v) {
       if (k < lo || k > hi) return;
       const u64 n = amount(k, v);
@@ -361,8 +530,9 @@ __device__ __forceinline__ Border border(const Source& from, Shared& s, uint32_t
     hi -= bin << shift;
     const uint32_t width = (1u << shift) - 1;
     lo = hi - lo > width ? hi - width : lo;
-    if (shift == 0) {
-      b.key = hi;
+    if (shift <= GRAIN<TY>) {
+      b.lo = lo;
+      b.hi = hi;
       return b;
     }
   }
@@ -374,29 +544,42 @@ struct Filters {
   int32_t top_k; // 0: none
   float top_p;
   u64 least;     // min-p, as a weight
-  float uniform;
+  float uniform, min_p;
   Weights weight;
+  // the key below which weights are less than a power of two
+  __device__ __forceinline__ uint32_t key_below(double power) const {
+    const double x = weight.most + power / weight.per_logit;
+    const uint32_t k = x > -(double)FLT_BIG ? key_of((float)x) : 1;
+    return k > 2 ? k - 1 : 1; // (rounded: one further down)
+  }
+  __device__ __forceinline__ double min_power() const { return log2((double)fminf(min_p, 1.0f)) - 0.001; } // (and the roundings on its way)
+  __device__ __forceinline__ u64 share(u64 whole) const { // top-p's
+    const u64 target = (u64)__builtin_ceil((double)top_p * (double)whole);
+    return target > 1 ? target : 1;
+  }
+  __device__ __forceinline__ u64 place(u64 whole) const {
+    const u64 target = uniform > 0.0f ? (u64)((double)(uniform < 1.0f ? uniform : 1.0f) * (double)whole) : (u64)0;
+    return target < whole ? target : whole - 1;
+  }
 };
 
-template <typename Source>
-__device__ __forceinline__ Found draw(const Source& from, Shared& s, const Filters& f, uint32_t lo, Part part) {
+// From whatever holds every token of keys >= lo that may be drawn
+template <int TY, typename Source, int THREADS>
+__device__ __forceinline__ Found draw(const Source& from, Shared<THREADS>& s, const Filters& f, uint32_t lo, Part part) {
   if (f.top_k > 0) {
-    const Border b = border<false>(from, s, lo, f.most, [](uint32_t, int32_t) { return (u64)1; }, [&](u64) { return (u64)f.top_k; });
-    // of that key as many as are missing (where there are fewer than k tokens in all, every one)
-    part.key = b.key;
-    part.last = locate(from, s, [&](uint32_t k, int32_t) { return (u64)(k == b.key); }, [&](u64) { return b.target - b.before - 1; }).token;
+    const Border b = border<false, TY>(from, s, lo, f.most, [](uint32_t, int32_t) { return (u64)1; }, [&](u64) { return (u64)f.top_k; });
+    // of these keys as many as are missing (where there are fewer than k tokens in all, every one)
+    part.lo = b.lo;
+    part.hi = b.hi;
+    part.last = locate(from, s, [&](uint32_t k, int32_t) { return (u64)(k >= b.lo && k <= b.hi); }, [&](u64) { return b.target - b.before - 1; }).token;
   }
   if (f.top_p < 1.0f) {
     const Part within = part;
-    const Border b = border<true>(
-        from, s, lo > within.key ? lo : within.key, f.most, [&](uint32_t k, int32_t v) { return within.has(k, v) ? f.weight(logit_of(k)) : (u64)0; },
-        [&](u64 whole) {
-          const u64 target = (u64)__builtin_ceil((double)f.top_p * (double)whole);
-          return target > 1 ? target : (u64)1;
-        });
-    const u64 each = f.weight(logit_of(b.key)), missing = (b.target - b.before + each - 1) / each;
-    part.key = b.key;
-    part.last = locate(from, s, [&](uint32_t k, int32_t v) { return (u64)(k == b.key && within.has(k, v)); }, [&](u64) { return missing - 1; }).token;
+    const auto weight = [&](uint32_t k, int32_t v) { return within.has(k, v) ? f.weight(logit_of(k)) : (u64)0; };
+    const Border b = border<true, TY>(from, s, lo > within.lo ? lo : within.lo, f.most, weight, [&](u64 whole) { return f.share(whole); });
+    part.lo = b.lo;
+    part.hi = b.hi;
+    part.last = locate(from, s, [&](uint32_t k, int32_t v) { return k >= b.lo && k <= b.hi ? weight(k, v) : (u64)0; }, [&](u64) { return b.target - b.before - 1; }).token;
   }
   return locate(
       from, s,
@@ -405,18 +588,241 @@ __device__ __forceinline__ Found draw(const Source& from, Shared& s, const Filte
         const u64 w = f.weight(logit_of(k));
         return w >= f.least ? w : (u64)0;
       },
-      [&](u64 whole) { return f.uniform > 0.0f ? (u64)((double)(f.uniform < 1.0f ? f.uniform : 1.0f) * (double)whole) : (u64)0; });
+      [&](u64 whole) { return f.place(whole); });
 }
 
-template <int TY>
+// Up to SMALL entries of the list: ranked against each other, then the first wave alone, E entries a lane
+template <int THREADS>
+__device__ __forceinline__ Found draw_small(Shared<THREADS>& s, const Filters& f, int n) {
+  const List<THREADS> list(s);
+  int at = 0;
+  for (int w = 0; w < list.wave; ++w) at += s.listed[w];
+  for (int i = list.lane; i < list.n; i += 64) {
+    s.small_key[at + i] = s.key[list.wave * List<THREADS>::LIST + i];
+    s.small_token[at + i] = s.token[list.wave * List<THREADS>::LIST + i];
+  }
+  constexpr int SMALL = Shared<THREADS>::SMALL, E = SMALL / 64;
+  for (int i = threadIdx.x; i < SMALL; i += THREADS) {
+    if (i >= n) s.small_key[i] = 0; // behind all others
+    s.rank[i] = 0;
+  }
+  __syncthreads();
+  // 64 entries a wave against a part of all
+  const int blocks = (n + 63) / 64, parts = blocks < THREADS / 64 ? THREADS / 64 / blocks : 1, part_of = ((n + 3) / 4 + parts - 1) / parts * 4;
+  for (int b = list.wave; b < blocks * parts; b += THREADS / 64) {
+    const int each = b % blocks * 64 + list.lane, first = b / blocks * part_of, end = first + part_of < n ? first + part_of : n;
+    const uint32_t mine = s.small_key[each];
+    int rank = 0;
+    // entries of the 64 are before or behind one by their places, all others' places are one side's
+    typedef __attribute__((ext_vector_type(4))) uint32_t four;
+    const auto count = [&](int from, int to, auto&& before) {
+      from = from > first ? from : first;
+      to = to < end ? to : end;
+#pragma unroll 4
+      for (int j = from; j < to; j += 4) { // (behind the last entry: keys of 0)
+        const four k = *reinterpret_cast<const four*>(&s.small_key[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rank += before(k[e], j + e);
+      }
+    };
+    const int own = b % blocks * 64;
+    count(0, own, [&](uint32_t k, int) { return k >= mine; });
+    count(own, own + 64, [&](uint32_t k, int j) { return k > mine || (k == mine && j < each); });
+    count(own + 64, SMALL, [&](uint32_t k, int) { return k > mine; });
+    if (rank) atomicAdd(&s.rank[each], rank);
+  }
+  __syncthreads();
+  for (int each = threadIdx.x; each < SMALL; each += THREADS) {
+    const int rank = each < n ? s.rank[each] : each; // (none has a key of 0)
+    const u64 w = each < n && (f.top_k == 0 || rank < f.top_k) ? f.weight(logit_of(s.small_key[each])) : (u64)0;
+    s.rank[each] = rank;
+    s.ranked[rank] = w;
+    s.amount[each] = w;
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    // a lane's running sums, behind those of the lanes before
+    const auto running = [&](const u64 (&w)[E], u64 (&to)[E]) {
+      to[0] = w[0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) to[e] = to[e - 1] + w[e];
+      const u64 before = wave_inclusive(to[E - 1]) - to[E - 1];
+#pragma unroll
+      for (int e = 0; e < E; ++e) to[e] += before;
+      return last_lane(to[E - 1]);
+    };
+    u64 w[E], to[E];
+    int kept = SMALL;
+    if (f.top_p < 1.0f) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) w[e] = s.ranked[E * lane + e];
+      const u64 whole = running(w, to), target = f.share(whole);
+      int mine = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) mine += to[e] - w[e] < target;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) mine += __shfl_xor(mine, d, 64);
+      kept = mine;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const u64 x = s.amount[E * lane + e];
+      w[e] = s.rank[E * lane + e] < kept && x >= f.least ? x : 0;
+    }
+    const u64 whole = running(w, to), target = f.place(whole);
+    const u64 above = __builtin_amdgcn_ballot_w64(target < to[E - 1]);
+    if (lane == __builtin_ctzll(above)) {
+      bool open = true;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (open && target < to[e]) {
+          s.bin = (uint32_t)s.small_token[E * lane + e];
+          s.found = w[e];
+          open = false;
+        }
+      s.wave[0] = whole;
+    }
+  }
+  __syncthreads();
+  return Found{(int32_t)s.bin, 0, s.found, s.wave[0]};
+}
+
+// No top-k, and more tokens than the list takes: the row is weighed by its waves' runs
+template <int TY, int THREADS, typename L>
+__device__ __forceinline__ Found draw_weighed(const Row<TY, THREADS>& row, Shared<THREADS>& s, const Filters& f, uint32_t lo, L&& make_list) {
+  const float most = logit_of(f.most), least = fmaxf(logit_of(lo), -FLT_BIG); // (the lowest keys are no numbers)
+  const auto by_weight = [&]() { // of those that min-p leaves
+    const auto amount = [&](uint32_t k, int32_t) {
+      const u64 w = k ? f.weight(logit_of(k)) : (u64)0;
+      return w >= f.least ? w : (u64)0;
+    };
+    u64 mine = 0;
+    row.each_logit([&](float x, int32_t) {
+      const u64 w = f.weight(x);
+      mine += w >= f.least ? w : 0;
+    });
+    const u64 whole = sum_up(s, mine);
+    return locate_in_run(row, s, amount, whole, f.place(whole));
+  };
+  if (f.top_p >= 1.0f) return by_weight();
+  // bins of logits, evenly from the largest one down to those that weigh nothing
+  const float per_logit = (float)RUN_BINS / fmaxf(most - least, 1e-30f);
+  const auto bin_of = [&](float x) { return (int)fminf(fmaxf((most - x) * per_logit, 0.0f), (float)(RUN_BINS - 1)); };
+  __syncthreads();
+  for (int i = threadIdx.x; i < THREADS / 64 * RUN_BINS; i += THREADS) s.run[0][i] = 0;
+  __syncthreads();
+  row.each_logit([&](float x, int32_t) {
+    const u64 w = f.weight(x);
+    if (w) atomicAdd((unsigned long long*)&s.run[row.wave][bin_of(x)], (unsigned long long)w);
+  });
+  __syncthreads();
+  // the bin that has top-p's border: a thread per bin
+  u64 to = 0;
+  constexpr int EACH = RUN_BINS > THREADS ? RUN_BINS / THREADS : 1;
+  u64 n[EACH] = {}, mine = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+    if ((int)threadIdx.x * EACH + i < RUN_BINS) {
+#pragma unroll 1
+      for (int w = 0; w < THREADS / 64; ++w) n[i] += s.run[w][threadIdx.x * EACH + i];
+      mine += n[i];
+    }
+  const u64 whole = sum_up(s, mine);
+  const u64 target = f.share(whole);
+  to = wave_inclusive(mine) - mine;
+  for (int w = 0; w < row.wave; ++w) to += s.sums[w];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    if (to < target && to + n[i] >= target) {
+      s.bin = threadIdx.x * EACH + i;
+      s.found = to;
+    }
+    to += n[i];
+  }
+  __syncthreads();
+  const int border_bin = (int)s.bin;
+  const u64 before = s.found;
+  // what each run has above that bin
+  u64 above = 0;
+  for (int i = row.lane; i < border_bin; i += 64) above += s.run[row.wave][i];
+  above = wave_sum(above);
+  // its tokens, in a list. (A bin's ends are those of its logits but for roundings, of 2^-22 of the largest number there is.)
+  const float off = 2.4e-7f * (fabsf(most) + fabsf(least)), from = border_bin == RUN_BINS - 1 ? least : most - (border_bin + 1) / per_logit - off,
+              to_most = most - border_bin / per_logit + off;
+  int listed = 0;
+  row.each_piece([&](const auto& p, int32_t v, int32_t) {
+    if (listed <= Shared<THREADS>::LIST) listed = list_pieces<TY>(s, p, v, listed, from, to_most, [&](float x) { return x >= least && bin_of(x) == border_bin; });
+  });
+  if (row.lane == 0) s.listed[row.wave] = listed;
+  const Part all{lo, lo, row.vocab};
+  if (__syncthreads_or(listed > Shared<THREADS>::LIST)) return draw<TY>(row, s, f, lo, all);
+  const List<THREADS> list(s);
+  const auto weight = [&](uint32_t k, int32_t) { return f.weight(logit_of(k)); };
+  const Border b = border<true, TY>(list, s, lo, f.most, weight, [&](u64) { return target - before; });
+  const auto tie = locate(list, s, [&](uint32_t k, int32_t v) { return k >= b.lo && k <= b.hi ? weight(k, v) : (u64)0; }, [&](u64) { return b.target - b.before - 1; });
+  const Part part{b.lo, b.hi, tie.token};
+  const auto amount = [&](uint32_t k, int32_t v) {
+    if (!part.has(k, v)) return (u64)0;
+    const u64 w = f.weight(logit_of(k));
+    return w >= f.least ? w : (u64)0;
+  };
+  if (tie.amount < f.least) { // min-p leaves less than top-p, and equal ones together
+    if (!make_list(f.key_below(f.min_power()))) return by_weight();
+    return locate(List<THREADS>(s), s, amount, [&](u64 sum) { return f.place(sum); });
+  }
+  u64 kept = 0;
+  list.each([&](uint32_t k, int32_t v) { kept += part.has(k, v) ? weight(k, v) : (u64)0; });
+  const u64 left = sum_up(s, row.lane == 0 ? kept + above : kept);
+  return locate_in_run(row, s, amount, left, f.place(left));
+}
+
+template <int TY, int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_tokens_kernel(const SampleArgs a) {
-  __shared__ Shared s;
+  using R = Row<TY, THREADS>;
+  constexpr int N = R::N, LIST = Shared<THREADS>::LIST, WAVES = THREADS / 64;
+  __shared__ Shared<THREADS> s;
   const int64_t at = blockIdx.x;
-  const Row<TY> row(a, at);
-  uint32_t mine = 0; // the thread's largest key
-  row.each([&](uint32_t k, int32_t) { mine = mine > k ? mine : k; });
+  const int32_t pieces = (a.vocab + N - 1) / N;
+  const R row(reinterpret_cast<const char*>(a.logits) + at * a.stride * R::P::BYTES, a.vocab, 0, pieces);
+  const float temperature = a.temperature ? a.temperature[at] : 1.0f, min_p = a.min_p ? a.min_p[at] : 0.0f;
   Filters f;
-  f.most = block_max(s, mine);
+  f.min_p = min_p;
+  f.top_k = a.top_k ? a.top_k[at] : 0;
+  f.top_p = a.top_p ? a.top_p[at] : 1.0f;
+  f.uniform = a.uniform[at];
+  // groups of 1, 2, 4 ... 32 pieces: as many as there is room for
+  int log2_lanes = 0;
+  while (((pieces - 1) >> log2_lanes) >= Shared<THREADS>::MOST_GROUPS) ++log2_lanes;
+  const int lanes = 1 << log2_lanes, groups = ((pieces - 1) >> log2_lanes) + 1;
+  if (threadIdx.x < STEPS) s.roots[threadIdx.x] = ROOTS[threadIdx.x];
+  for (int i = threadIdx.x; i < BINS; i += THREADS) s.count[i] = 0; // for top-k's groups
+  uint32_t high = 0, low = 0; // of the groups' largest: low of the least, as a complement
+  row.template each_piece<FIRST_AHEAD>([&](const auto& p, int32_t, int32_t i) {
+    const uint32_t k = group_lanes_max(largest_of<TY>(p), lanes);
+    high = high > k ? high : k;
+    if (k) low = low > ~k ? low : ~k;
+    if ((row.lane & (lanes - 1)) == 0 && i < pieces) s.group[i >> log2_lanes] = k;
+  });
+  high = wave_max(high), low = wave_max(low);
+  if (row.lane == 0) s.wave32[row.wave] = high, s.low32[row.wave] = low;
+  __syncthreads();
+  f.most = 0;
+  uint32_t least_group = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    f.most = f.most > s.wave32[w] ? f.most : s.wave32[w];
+    least_group = least_group > s.low32[w] ? least_group : s.low32[w];
+  }
+  least_group = ~least_group;
+  __syncthreads(); // (the words are used again)
+  const int group_steps = (groups + THREADS - 1) / THREADS; // of a wave, 64 groups each
+  const auto group_at = [&](int step) { return (row.wave * group_steps + step) * 64 + row.lane; };
+  constexpr int GROUP_STEPS = Shared<THREADS>::MOST_GROUPS / THREADS;
+  uint32_t group[GROUP_STEPS]; // a thread's
+#pragma unroll
+  for (int k = 0; k < GROUP_STEPS; ++k) group[k] = k < group_steps && group_at(k) < groups ? s.group[group_at(k)] : 0;
+  const bool greedy = !(temperature > 0.0f) || f.top_k == 1 || !(f.top_p > 0.0f);
   if (f.most == 0) { // nothing to draw from
     if (threadIdx.x == 0) {
       a.tokens[at] = -1;
@@ -424,51 +830,110 @@ __global__ __launch_bounds__(THREADS) void sample_tokens_kernel(const SampleArgs
     }
     return;
   }
-  const float temperature = a.temperature ? a.temperature[at] : 1.0f, min_p = a.min_p ? a.min_p[at] : 0.0f;
-  f.top_k = a.top_k ? a.top_k[at] : 0;
-  f.top_p = a.top_p ? a.top_p[at] : 1.0f;
-  f.uniform = a.uniform[at];
-  if (!(temperature > 0.0f) || f.top_k == 1 || !(f.top_p > 0.0f)) {
+  const auto write = [&](int32_t token, float log_probability) {
+    a.tokens[at] = token;
+    a.log_probability[at] = log_probability;
+  };
+  // the groups with a key of at least `lo`, in their order; how many
+  const auto choose = [&](uint32_t lo) {
+    u64 in[GROUP_STEPS];
+    int mine = 0; // of the wave
+#pragma unroll
+    for (int k = 0; k < GROUP_STEPS; ++k) {
+      in[k] = __builtin_amdgcn_ballot_w64(group[k] >= lo);
+      mine += __builtin_popcountll(in[k]);
+    }
+    if (row.lane == 0) s.wave32[row.wave] = mine;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < row.wave) before += s.wave32[w];
+      all += s.wave32[w];
+    }
+#pragma unroll
+    for (int k = 0; k < GROUP_STEPS; ++k) {
+      if ((in[k] >> row.lane) & 1) s.chosen[before + __builtin_popcountll(in[k] & ((1ull << row.lane) - 1))] = (uint16_t)group_at(k);
+      before += __builtin_popcountll(in[k]);
+    }
+    __syncthreads();
+    return all;
+  };
+  if (greedy) {
     // the most likely one, the first of equal ones
-    const Found first = locate(row, s, [&](uint32_t k, int32_t) { return (u64)(k == f.most); }, [](u64) { return (u64)0; });
-    if (threadIdx.x == 0) {
-      a.tokens[at] = first.token;
-      a.log_probability[at] = 0.0f;
+    choose(f.most);
+    if (row.wave == 0) {
+      const int32_t i = ((int32_t)s.chosen[0] << log2_lanes) + row.lane;
+      typename R::P p;
+      R::load(p, row.logits, row.lane < lanes && i < pieces ? i * N : a.vocab, a.vocab);
+      int32_t token = -1;
+      R::each_of(p, i * N, [&](float x, int32_t v) {
+        if (token < 0 && key_of(x) == f.most) token = v;
+      });
+      const u64 has = __builtin_amdgcn_ballot_w64(token >= 0);
+      if (row.lane == __builtin_ctzll(has)) write(token, 0.0f);
     }
     return;
   }
   if (f.top_k <= 0 || f.top_k >= a.vocab) f.top_k = 0;
   const int bits = 32 - __builtin_clz(a.vocab);
-  f.weight = Weights{(double)logit_of(f.most), 1.4426950408889634074 / (double)temperature, 62 - bits < 50 ? 62 - bits : 50};
+  f.weight = Weights{(double)logit_of(f.most), 1.4426950408889634074 / (double)temperature, 62 - bits < 50 ? 62 - bits : 50, s.roots};
   f.least = min_p > 0.0f ? (u64)__builtin_ceil(__builtin_ldexp((double)(min_p < 1.0f ? min_p : 1.0f), f.weight.fraction)) : 0;
   // keys below `lo` take no part
   uint32_t lo = 1;
-  if (f.top_k > 0 && f.top_k <= THREADS) { // they are not among the first k: k threads' largest are above them. By bisection
-    uint32_t high = f.most;
-    while (lo < high) {
-      const uint32_t mid = lo + (high - lo + 1) / 2;
-      if (__syncthreads_count(mine >= mid) >= f.top_k) lo = mid;
-      else high = mid - 1;
+  if (f.top_k > 0) { // k groups' largest are above them
+    const uint32_t least = least_group;
+    const int shift = shift_of(least, f.most);
+#pragma unroll
+    for (int k = 0; k < GROUP_STEPS; ++k)
+      if (group[k]) atomicAdd(&s.count[(f.most - group[k]) >> shift], 1u);
+    __syncthreads();
+    bool enough = false;
+    find_bin<false>(s, [&](u64 whole) {
+      enough = whole >= (u64)f.top_k;
+      return (u64)f.top_k;
+    });
+    const uint32_t down = (s.bin << shift) + ((1u << shift) - 1); // (a bin is within the keys' span and less than its double)
+    if (enough) lo = f.most - least > down ? f.most - down : least;
+  } else { // they weigh nothing, or too little for min-p
+    lo = f.key_below(-(f.weight.fraction + 2)); // 2^-2 of a unit
+    if (f.top_p >= 1.0f && f.min_p > 0.0f) lo = max(lo, f.key_below(f.min_power()));
+  }
+  // the tokens of those groups, in the list, a wave's share of the groups 64 pieces at a time; false: it does not hold them
+  const auto make_list = [&](uint32_t from) {
+    const int chosen = choose(from), share = ((chosen << log2_lanes) + THREADS - 1) / THREADS;
+    const float least = fmaxf(logit_of(from), -FLT_BIG); // (the lowest keys are no numbers)
+    int listed = 0;
+    for (int k = 0; k < share && listed <= LIST; ++k) {
+      const int32_t item = (row.wave * share + k) * 64 + row.lane, g = item >> log2_lanes;
+      const int32_t i = g < chosen ? ((int32_t)s.chosen[g] << log2_lanes) + (item & (lanes - 1)) : pieces;
+      typename R::P p;
+      R::load(p, row.logits, i < pieces ? i * N : a.vocab, a.vocab);
+      listed = list_pieces<TY>(s, p, i * N, listed, least, __builtin_inff(), [](float) { return true; });
     }
-  } else if (f.top_k == 0) { // they weigh nothing, or too little for min-p
-    double below = f.weight.fraction + 2;
-    if (min_p > 0.0f && f.top_p >= 1.0f) below = fmin(below, 0.001 - log2((double)fminf(min_p, 1.0f)));
-    const double least = f.weight.most - below / f.weight.per_logit;
-    if (least > -(double)FLT_BIG) lo = key_of((float)least) - 1; // (rounded: one further down)
+    if (row.lane == 0) s.listed[row.wave] = listed;
+    return !__syncthreads_or(listed > LIST);
+  };
+  Found drawn;
+  if (make_list(lo)) {
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) n += s.listed[w];
+    if (n <= Shared<THREADS>::SMALL) drawn = draw_small(s, f, n);
+    else drawn = draw<TY>(List<THREADS>(s), s, f, lo, Part{lo, lo, a.vocab});
+  } else if (f.top_k == 0 && f.weight.most < (double)FLT_BIG) { // (no infinities)
+    drawn = draw_weighed(row, s, f, lo, make_list);
+  } else {
+    drawn = draw<TY>(row, s, f, lo, Part{lo, lo, a.vocab});
   }
-  const Part all{lo, a.vocab};
-  const Found drawn = make_list(row, s, lo) ? draw(List(s), s, f, lo, all) : draw(row, s, f, lo, all);
-  if (threadIdx.x == 0) {
-    a.tokens[at] = drawn.token;
-    a.log_probability[at] = (float)log((double)drawn.amount / (double)drawn.whole);
-  }
+  if (threadIdx.x == 0) write(drawn.token, (float)log((double)drawn.amount / (double)drawn.whole));
 }
 
-template <int TY>
-hipError_t launch(SampleArgs a, hipStream_t stream) {
+template <int TY, int THREADS>
+hipError_t launch_shape(SampleArgs a, hipStream_t stream) {
   constexpr int64_t MOST = 0xffffffffll / THREADS; // rows of a launch: fewer than 2^32 threads
   for (int64_t rows = a.rows; rows > 0; rows -= MOST) {
-    sample_tokens_kernel<TY><<<(unsigned)(rows < MOST ? rows : MOST), THREADS, 0, stream>>>(a);
+    sample_tokens_kernel<TY, THREADS><<<(unsigned)(rows < MOST ? rows : MOST), THREADS, 0, stream>>>(a);
     if (hipError_t e = hipGetLastError()) return e;
     const auto later = [](auto*& p) {
       if (p) p += MOST;
@@ -478,6 +943,13 @@ hipError_t launch(SampleArgs a, hipStream_t stream) {
   }
   return hipSuccess;
 }
+template <int TY>
+hipError_t launch(const SampleArgs& a, hipStream_t stream) {
+  // a small row is no work for 16 waves
+  if (a.vocab <= 4096) return launch_shape<TY, 256>(a, stream);
+  return launch_shape<TY, 1024>(a, stream);
+}
+
 } // namespace
 
 hipError_t launch_sample_tokens(const SampleArgs& a, int32_t ty, hipStream_t stream) {
