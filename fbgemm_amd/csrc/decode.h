@@ -122,8 +122,13 @@ struct AttentionArgs {
   int4* joins;        // [workers]: the last worker of the pair that begins with this one (-1: none goes on), its rows, the first of them
 };
 constexpr int ATTENTION_STEP = 128; // tokens of a unit of work
-// workgroups of the attention kernel that a compute unit holds at once: what its registers leave room for
-constexpr int attention_residents(int dim) { return dim > 128 ? 1 : dim > 64 ? 2 : 3; }
+// Workgroups of the attention kernel that a compute unit holds at once: what its registers leave room for. bits: of an element of the
+// rows; pages: whole tiles of 16 tokens
+constexpr int attention_residents(int dim, int bits, bool pages) {
+  if (dim > 128) return 1;
+  if (bits == 4) return pages ? 3 : 2;
+  return dim > 64 ? 2 : 3;
+}
 constexpr int ATTENTION_ROWS = 16; // queries of a key head that one tile of the matrix cores takes
 hipError_t launch_paged_attention_bf16(const AttentionArgs& a, hipStream_t stream);
 hipError_t launch_paged_attention_fp16(const AttentionArgs& a, hipStream_t stream);

@@ -116,7 +116,7 @@ int compute_units() {
 int attention_workers(const fbgemm_amd_paged_cache& c, int64_t requests, int32_t query_heads, int64_t max_tokens) {
   const int64_t sets = (int64_t)c.heads * ((query_heads / c.heads + ATTENTION_ROWS - 1) / ATTENTION_ROWS);
   const int64_t each = std::max<int64_t>(1, (max_tokens + 15 + ATTENTION_STEP - 1) / ATTENTION_STEP);
-  const int64_t most = (int64_t)compute_units() * attention_residents(c.dim);
+  const int64_t most = (int64_t)compute_units() * attention_residents(c.dim, c.row_ty == ST_CACHE_INT4 ? 4 : c.row_ty == ST_INT8 ? 8 : 16, c.block_size % 16 == 0);
   if (requests * sets >= most || each >= most) return (int)most;
   return (int)std::min(most, requests * sets * each);
 }

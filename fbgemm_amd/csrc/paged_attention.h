@@ -90,12 +90,13 @@ __device__ __forceinline__ float unpack16(uint32_t v, int half) {
   return (float)__builtin_bit_cast(f16x2, v)[half];
 }
 // 8 weights as two operands: rounded, and what the rounding left
-template <bool BF16>
+template <bool BF16, bool ONE_ROUNDING = false>
 __device__ __forceinline__ void split(const float (&p)[8], uint4& hi, uint4& lo) {
   uint32_t h[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     h[i] = pack16<BF16>(p[2 * i], p[2 * i + 1]);
+    if (ONE_ROUNDING) asm("" : "+v"(h[i])); // (else the compiler rounds the first of the two once more for the next line)
     l[i] = pack16<BF16>(p[2 * i] - unpack16<BF16>(h[i], 0), p[2 * i + 1] - unpack16<BF16>(h[i], 1));
   }
   hi = make_uint4(h[0], h[1], h[2], h[3]);
@@ -144,12 +145,14 @@ __device__ __forceinline__ uint4 codes4(uint32_t w) {
 }
 
 __device__ __forceinline__ float half_at(uint32_t pair, int i) { return (float)__builtin_bit_cast(f16x2, pair)[i]; }
+// x * half by one instruction, which converts as it multiplies and adds (for a product alone the compiler takes two)
+__device__ __forceinline__ float times_half(float x, uint32_t pair, int i) { return __builtin_fmaf(x, half_at(pair, i), 0.0f); }
 // what code 128 of an 8-bit row, or 8 of a 4-bit one, stands for, by its scale and bias
 template <int ROWS = 8>
 __device__ __forceinline__ float middle(uint32_t pair) { return __builtin_fmaf(ROWS == 8 ? 128.0f : 8.0f, half_at(pair, 0), half_at(pair, 1)); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // tanh(x) / x = 1 - x^2/3 + 2 x^4/15 - ..., for |x| < TANH_SMALL to 2^-24 (the next term: 0.0036 x^12)
-constexpr float TANH_SMALL = 0.35f;
+constexpr float TANH_SMALL = 0.35f, FLT_MOST = 3.4028234663852886e38f, FLT_LEAST = 1.17549435e-38f;
 __device__ __forceinline__ float tanh_ratio(float x) {
   const float z = x * x;
   float p = -1382.0f / 155925.0f;
@@ -244,7 +247,7 @@ __device__ __forceinline__ uint32_t inclusive_sum(uint32_t v, int lane) {
 // ROWS: bits of an element: 16, or 8 or 4 in rows with a scale and bias. DP: columns the code is laid out for; FULL: dim is DP, else less: lanes that would have the
 // columns behind read the row's first ones in their place, which meet zeros in the queries or make outputs that nobody wants.
 // PAGE16: pages are whole 16-token tiles, whose addresses are then the same for the wave. PACKED (FULL rows of codes, PAGE16): the
-// rows of a page's tokens follow each other without gaps. 16 of them are then read as one run of bytes, every line by one
+// rows of a page's tokens follow each other without gaps, and pages are as far apart for values as for keys. 16 of them are then read as one run of bytes, every line by one
 // load and marked as read once, and go through LDS, where a lane finds its pieces: 262 143 tokens 103 us, 118 with a gap
 // of 4 bytes behind each row (two tiles ahead instead of one: 2 % more); 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, 400 us, 459 with gaps.
 template <bool BF16, int ROWS, int DP, bool FULL, bool PAGE16, bool PACKED>
@@ -263,7 +266,7 @@ struct Attention {
   static constexpr int KREGS = ROWS4 ? (FULL ? (KP < 4 ? KP : 4) : 1) : ROWS8 ? 2 : 4;
   static constexpr int KPIECES = ROWS4 ? KP / KREGS : KP;
   static constexpr int KEY_STEP = ROWS4 ? 4 * KREGS : bytes_of(32); // bytes from a lane's piece to its next one
-  static constexpr int WEIGHT_UP = ROWS4 ? 80 : 0;     // 4-bit rows: weights are 2^80 times larger for the products, whose other operands are subnormal
+  static constexpr int WEIGHT_UP = ROWS4 ? 72 : 0;     // 4-bit rows: weights and their sums are 2^72 times larger, for products whose other operands are subnormal
   static constexpr int DEPTH = 1;                      // tiles loaded ahead
   static constexpr int KEY_AUX = CODES || DP == 64 ? 0 : READ_ONCE, VALUE_AUX = CODES ? 0 : READ_ONCE;
 
@@ -290,6 +293,7 @@ struct Attention {
   // where its pages are: PAGE16 of the two 16-token halves, else of token `lane & 31`
   struct Pages {
     int block[2];
+    int in_block[2]; // PACKED: the half's first token in its page
   };
 
   const AttentionArgs& a;
@@ -324,6 +328,7 @@ struct Attention {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int column = (int)divide((uint32_t)(t0 + 16 * h), a.block);
+        if (PACKED) p.in_block[h] = t0 + 16 * h - column * a.block_size;
         p.block[h] = as_constant<int32_t>(table)[column < last_column ? column : last_column]; // a half behind the end reads rows of the last page
       }
     } else {
@@ -358,16 +363,15 @@ struct Attention {
       const char* run[4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int t = t0 + 16 * h;
-        const int in_block = t - (int)divide((uint32_t)t, a.block) * a.block_size;
         int block = pages.block[h];
         if ((uint32_t)block >= (uint32_t)a.blocks) {
           block = 0;
           tile.partial = true;
           tile.seen &= h ? 0x0f : 0xf0;
         }
-        run[h] = key_base + (block * a.key.block_stride + in_block * a.key.slot_stride);
-        run[2 + h] = value_base + (block * a.value.block_stride + in_block * a.value.slot_stride);
+        const int64_t from = block * a.key.block_stride + pages.in_block[h] * ROW; // of keys and of values
+        run[h] = key_base + from;
+        run[2 + h] = value_base + from;
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -467,8 +471,9 @@ struct Attention {
   float q_sum;
   f32x4 acc[HALVES][VC];
   float m, l, bias;
-  // 4-bit rows: exponent of a sum of codes by queries; and the products of code 8, which is taken off afterwards, at even and at odd columns
-  int q_up;
+  // 4-bit rows: scores (and their maximum) are in units of 1 / unit, so that queries need no factor for each: what a unit is, unless a cap
+  // has made plain scores of them; the factor that does. And the products of code 8, which is taken off afterwards, at even and at odd columns.
+  float unit, to_plain;
   f32x4 eights[2];
 
   __device__ __forceinline__ void begin(int32_t request, int head, int q0, int rows) {
@@ -485,10 +490,12 @@ struct Attention {
         for (int i = 0; i < 4; ++i) q_sum += unpack16<BF16>(w[i], 0) + unpack16<BF16>(w[i], 1);
       }
     }
-    if constexpr (ROWS4) order_queries();
+    int sum_up = 0;
+    if constexpr (ROWS4) sum_up = order_queries();
     if (CODES) {
       q_sum += __shfl_xor(q_sum, 16, 64);
       q_sum += __shfl_xor(q_sum, 32, 64);
+      if (ROWS4) q_sum = __builtin_amdgcn_ldexpf(q_sum, sum_up);
     }
 #pragma unroll
     for (int h = 0; h < HALVES; ++h)
@@ -499,11 +506,12 @@ struct Attention {
     l = bias = 0.0f;
   }
 
-  // 4-bit rows: the queries' elements in the codes' order. bf16: the largest is brought to 2^100, so that products with subnormal
-  // numbers are normal ones (an exact step, but for elements 2^-220 times smaller), and odd elements are 2^-4 of that
-  __device__ __forceinline__ void order_queries() {
-    q_up = 20; // 16 * 2^-24 a step
-    int e = 0;
+  // 4-bit rows: the queries' elements in the codes' order. bf16: the largest is brought to 2^126, so that products with subnormal
+  // numbers are normal ones (an exact step, but for elements 2^-240 times smaller), and odd elements are 2^-4 of that. With a scale
+  // below zero they change their sign, so that the largest score is the largest product. The exponent that brings their sum to
+  // the products' units
+  __device__ __forceinline__ int order_queries() {
+    int e = 0, up = -20; // fp16: codes are 16 * 2^-24
     if constexpr (BF16) {
       float most = 0.0f;
 #pragma unroll
@@ -512,9 +520,16 @@ struct Attention {
 #pragma unroll
         for (int i = 0; i < 4; ++i) most = __builtin_fmaxf(most, __builtin_fmaxf(__builtin_fabsf(unpack16<BF16>(w[i], 0)), __builtin_fabsf(unpack16<BF16>(w[i], 1))));
       }
-      e = 100 - __builtin_amdgcn_frexp_expf(group_max(most)); // (of 0, inf and NaN: 100)
-      q_up = 133 - e;
+      most = group_max(most);
+      // (of zeros, and of what is not finite, as it is)
+      e = most > 0.0f && most <= FLT_MOST ? 126 - __builtin_amdgcn_frexp_expf(most) : 133;
+      up = e - 133;
     }
+    // a number that is not 0, for scores of -inf, nor infinite, for those of 0
+    to_plain = __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(__builtin_fabsf(a.scale), -up), FLT_LEAST, FLT_MOST);
+    unit = a.softcap > 0.0f ? 1.0f : to_plain;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    if (a.scale < 0.0f) q_sum = -q_sum;
 #pragma unroll
     for (int c = 0; c < KP; ++c) {
       const uint4 w = q[c];
@@ -523,12 +538,13 @@ struct Attention {
       if constexpr (BF16) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int up = i & 1 ? e - 4 : e;
-          t[i] = pack_bf16(__builtin_amdgcn_ldexpf(unpack16<BF16>(t[i], 0), up), __builtin_amdgcn_ldexpf(unpack16<BF16>(t[i], 1), up));
+          const int by = i & 1 ? e - 4 : e;
+          t[i] = pack_bf16(__builtin_amdgcn_ldexpf(unpack16<BF16>(t[i], 0), by), __builtin_amdgcn_ldexpf(unpack16<BF16>(t[i], 1), by));
         }
       }
-      q[c] = make_uint4(t[0], t[1], t[2], t[3]);
+      q[c] = make_uint4(t[0] ^ flip, t[1] ^ flip, t[2] ^ flip, t[3] ^ flip);
     }
+    return up;
   }
 
   // PACKED: a lane's part of the runs, through LDS, where no other wave looks. Lanes read what others wrote: that the wave's
@@ -597,7 +613,10 @@ struct Attention {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float y = r[j];
-        if (ROWS4) y = __builtin_fmaf(half_at(tile.k_pair[4 * h + j], 0), __builtin_amdgcn_ldexpf(y, q_up), half_at(tile.k_pair[4 * h + j], 1) * q_sum);
+        if (ROWS4) {
+          s[4 * h + j] = __builtin_fmaf(half_at(tile.k_pair[4 * h + j], 0), y, times_half(q_sum, tile.k_pair[4 * h + j], 1));
+          continue;
+        }
         if (ROWS8) y = __builtin_fmaf(half_at(tile.k_pair[4 * h + j], 0), y, (BF16 ? half_at(tile.k_pair[4 * h + j], 1) : middle(tile.k_pair[4 * h + j])) * q_sum);
         s[4 * h + j] = y * a.scale;
       }
@@ -607,6 +626,7 @@ struct Attention {
     if (a.softcap > 0.0f) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
+        if (ROWS4) s[j] *= to_plain;
         const float x = s[j] * a.cap_inverse;
         s[j] = __builtin_fabsf(x) < TANH_SMALL ? s[j] * tanh_ratio(x) : a.softcap * tanh_fast(x);
       }
@@ -634,7 +654,7 @@ struct Attention {
     most = group_max(most);
     if (__builtin_amdgcn_ballot_w64(most > m)) {
       const float now = __builtin_fmaxf(m, most);
-      const float f = m == now ? 1.0f : exp2_fast(m - now); // m = -inf: 0
+      const float f = m == now ? 1.0f : exp2_fast(ROWS4 ? (m - now) * unit : m - now); // m = -inf: 0
       m = now;
       l *= f;
       bias *= f;
@@ -647,23 +667,24 @@ struct Attention {
         eights[1] *= f;
       }
     }
-    const float ref = m == -__builtin_inff() ? 0.0f : m - SHIFT; // nothing seen yet: all weights 0
+    const float ref = m == -__builtin_inff() ? 0.0f : ROWS4 ? m * unit : m - SHIFT; // nothing seen yet: all weights 0
     float p[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = exp2_fast(s[j] - ref);
+      p[j] = exp2_fast(ROWS4 ? __builtin_fmaf(s[j], unit, -ref) : s[j] - ref);
+      if (ROWS4) p[j] = __builtin_amdgcn_ldexpf(p[j], WEIGHT_UP);
       l += p[j];
     }
     if (CODES) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         bias = __builtin_fmaf(p[j], middle<ROWS>(tile.v_pair[j]), bias);
-        p[j] *= half_at(tile.v_pair[j], 0);
-        if (ROWS4) p[j] = __builtin_amdgcn_ldexpf(p[j], WEIGHT_UP);
+        if (ROWS4) p[j] = times_half(p[j], tile.v_pair[j], 0);
+        else p[j] *= half_at(tile.v_pair[j], 0);
       }
     }
     uint4 hi, lo;
-    split<PBF16>(p, hi, lo);
+    split<PBF16, ROWS4>(p, hi, lo);
     // ---- values ----
     if constexpr (ROWS4) {
       add_codes4(tile, hi, lo);
@@ -790,7 +811,7 @@ __device__ __forceinline__ void write_out(const AttentionArgs& a, int64_t at, in
 }
 
 template <bool BF16, int ROWS, int DP, bool FULL, bool PAGE16, bool PACKED>
-__global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP)) void paged_attention_kernel(const AttentionArgs a) {
+__global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP, ROWS, PAGE16)) void paged_attention_kernel(const AttentionArgs a) {
   using A = Attention<BF16, ROWS, DP, FULL, PAGE16, PACKED>;
   constexpr int THREADS = 64 * ATT_WAVES;
   __shared__ __attribute__((aligned(16))) float s_acc[ATT_WAVES][ATTENTION_ROWS][DP + 4];
@@ -878,6 +899,11 @@ __global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP)) void paged
     if (A::CODES) {
       x.bias += __shfl_xor(x.bias, 16, 64);
       x.bias += __shfl_xor(x.bias, 32, 64);
+    }
+    if (A::ROWS4) { // as they are from here on
+      x.l = __builtin_amdgcn_ldexpf(x.l, -A::WEIGHT_UP);
+      x.bias = __builtin_amdgcn_ldexpf(x.bias, -A::WEIGHT_UP);
+      x.m *= x.unit;
     }
     if (g == 0) {
       s_ml[wave][n][0] = x.m;
@@ -972,7 +998,7 @@ void launch_kernel(const AttentionArgs& a, hipStream_t stream) {
   }
   if constexpr (ROWS < 16 && FULL && !(ROWS == 4 && DP == 64)) {
     constexpr int ROW = DP * ROWS / 8 + 4;
-    if (a.key.slot_stride == ROW && a.value.slot_stride == ROW) {
+    if (a.key.slot_stride == ROW && a.value.slot_stride == ROW && a.key.block_stride == a.value.block_stride) {
       paged_attention_kernel<BF16, ROWS, DP, FULL, true, true><<<grid, block, 0, stream>>>(a);
       return;
     }
