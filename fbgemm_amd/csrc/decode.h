@@ -91,8 +91,7 @@ struct RotateArgs {
   int32_t idx64, interleaved;
   const double* frequencies; // [pairs], radians a position
   float magnitude, sine;     // of cosines and sines: sine is -magnitude where turning back
-  int32_t token_group;       // tokens of a workgroup
-  Divisor units, all_heads;  // units: pieces of work of a head
+  Divisor units;             // pieces of work of a head
 };
 constexpr int ROTATE_MOST_PAIRS = 1024; // their sines are in LDS
 hipError_t launch_rotate_positions(const RotateArgs& a, int32_t ty, bool aligned16, hipStream_t stream);
@@ -123,7 +122,8 @@ struct AttentionArgs {
 };
 constexpr int ATTENTION_STEP = 128; // tokens of a unit of work
 // Workgroups of the attention kernel that a compute unit holds at once: what its registers leave room for. bits: of an element of the
-// rows; pages: whole tiles of 16 tokens
+// rows; pages: whole tiles of 16 tokens. 4-bit rows in such pages, 256 requests of 16 to 8 192 tokens, us: three with one tile on its way 252, two
+// with two tiles 268, with three 279; three with two tiles do not fit the registers, 352.
 constexpr int attention_residents(int dim, int bits, bool pages) {
   if (dim > 128) return 1;
   if (bits == 4) return pages ? 3 : 2;
@@ -160,7 +160,7 @@ hipError_t launch_penalize_logits(const LogitsArgs& a, int32_t ty, bool idx64, h
 struct SampleArgs {
   const void* logits;
   int64_t rows, stride; // stride: elements
-  int32_t vocab;
+  int32_t vocab, compute_units; // the device's
   const float* uniform;
   const float* temperature; // [rows] or null, as the next ones
   const int32_t* top_k;

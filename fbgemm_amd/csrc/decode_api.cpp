@@ -511,11 +511,13 @@ int fbgemm_amd_sample_tokens(
   if (rows == 0) return 0;
   if (!d_logits || !d_uniform || !d_tokens || !d_log_probability) return fail(FBGEMM_AMD_E_ARG, "null data pointer");
   if (logits_stride < 0) return fail(FBGEMM_AMD_E_ARG, "strides must not be negative");
+  if ((uintptr_t)d_logits % storage_bytes(logits_ty)) return fail(FBGEMM_AMD_E_ARG, "rows are not aligned to their elements");
   SampleArgs a;
   a.logits = d_logits;
   a.rows = rows;
   a.stride = rows > 1 ? logits_stride : 0;
   a.vocab = (int32_t)vocab;
+  a.compute_units = compute_units();
   a.uniform = d_uniform;
   a.temperature = d_temperature;
   a.top_k = d_top_k;

@@ -143,7 +143,7 @@ __global__ __launch_bounds__(THREADS) void kv_append_coded_kernel(const AppendAr
 // The common form: rows of whole runs of 8, at most 64 of them, on 16-byte boundaries. The key's and the value's row are
 // loaded together and stay in registers between the search for their extremes and the rounding, lane by lane.
 // 8 191 tokens x 5 heads x 128 bf16 (32 MB read and written, 6 us at a copy's rate) take 31.5 us by the kernel above and 12.1
-// here (13.1 with bytes put together by shifts and extremes exchanged through LDS, 13.3 with two pairs in flight a group).
+// here (13.1 with bytes put together by shifts and extremes exchanged through LDS, 13.3 with two pairs in flight a group). That is 8-bit rows.
 template <int BITS, typename T>
 __global__ __launch_bounds__(THREADS) void kv_append_coded_runs_kernel(const AppendArgs a, const int lanes) {
   typedef piece8 __attribute__((aligned(4))) on4_t; // a row begins on 4 bytes

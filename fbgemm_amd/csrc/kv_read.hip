@@ -191,11 +191,16 @@ unsigned grid_for(int64_t tokens, int run) {
   const int64_t runs = (tokens + run - 1) / run;
   return (unsigned)(runs < (1 << 20) ? runs : 1 << 20);
 }
-// f(tokens of a workgroup, whether results are beyond the caches): enough tokens that a thread has a few, where there are some for all of the device
+// f(tokens of a workgroup, whether results are beyond the caches): enough tokens that a thread has a few, where there are some for all of the device.
+// us with 1, 4 and 16 of them, 4-bit rows of 8 heads of 128 to bf16, then 16-bit rows of 2 heads of 64:
+//    1 024     3.6  3.7  4.7     3.0  2.9  3.1
+//    2 048     5.2  4.4  5.2     4.0  3.1  3.1
+//    8 192    13.5  9.4  8.7     8.7  4.7  3.9
+//   65 536    77.7 43.3 49.0    64.8 23.2 12.8    (the former past the caches; 8-bit rows 80.0 53.0 48.6)
 template <typename F>
 void by_tokens(const ReadArgs& a, int64_t row_bytes, F&& f) {
   if (2 * a.tokens * a.heads * row_bytes >= (128 << 20)) f(std::integral_constant<int, 16>(), std::true_type());
-  else if (a.tokens >= 16384) f(std::integral_constant<int, 16>(), std::false_type());
+  else if (a.tokens >= 8192) f(std::integral_constant<int, 16>(), std::false_type());
   else if (a.tokens >= 2048) f(std::integral_constant<int, 4>(), std::false_type());
   else f(std::integral_constant<int, 1>(), std::false_type());
 }

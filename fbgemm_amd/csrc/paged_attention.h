@@ -31,6 +31,14 @@
 // the scale, not as zeros. Flipping the bytes' top bits costs 0.7 to 2 % (262 143 tokens 101.5 -> 102.2 us). A score's
 // rounding is 2^-24 of that anyway; keys are centred where it is free (fp16).
 //
+// 4-bit rows (fp16 scale a_t and bias b_t in front): the codes are the products' operands as they lie, subnormal numbers of 16 bits (codes4), and
+// no instruction converts them. s_t = a_t (q . k4_t) + b_t sum(q) as above, and values by weights p_t a_t for v4, less 8 times the sum of those
+// weights, beside p_t (b_t + 8 a_t); weights are bf16 pairs 2^72 times larger for both types of queries, so that products with 2^-133 are normal
+// numbers. What bounds them is instructions, not bytes: some 330 vector instructions a wave for 32 tokens of 128 (two thirds of the cycles, with
+// three workgroups a compute unit and what is left their waits). The 256 requests above, 1.15 GB of rows: 252 us, 4.55 TB/s, 2.7 times less than in 16
+// bits; 64 requests of 1 to 4 096: 50 us; one of 500: 10.4 us. (Two tiles at once where 8 queries or fewer share a head, which the other
+// half of the product's columns has room for, take 18 % fewer instructions, but registers and LDS banks run short: 271, 57 and 12.6 us.)
+//
 // Work: steps of 128 tokens of a (request, key head, 16 queries), 32 for each of a worker's (workgroup's) four waves, numbered in
 // that order. Each of W workers takes a W-th of them in a row, whatever requests they are of, so that all end together
 // however long the requests are; a pair of request and head weighs one more than its steps, or a worker that meets

@@ -9,9 +9,9 @@
 // quarters is off by 2^-53 of the angle, in fp32 it would be 2^-24 of it (262 143 radians: 0.02). Sine and
 // cosine of the rest, at most pi/4, are their series.
 //
-// Bound by memory: every element is read once and written once. A workgroup has one or a few tokens: it
-// makes their sines once, in LDS, and turns all heads of queries and keys by them, 16 bytes (two of them,
-// where a pair's elements are apart) a thread at a time.
+// Bound by memory: every element is read once and written once. 16 384 tokens of 40 heads of 128, bf16: 52 us, 6.4 TB/s; 64 of them:
+// 3.0 us. A workgroup has a token: it makes its sines once, in LDS, and turns all heads of queries and keys by them, 16 bytes (two of them,
+// where a pair's elements are apart) a thread at a time. (Four tokens a workgroup, for longer ones: 57.5 us; 8 192 tokens 29.4 instead of 27.2.)
 #include "decode.h"
 
 namespace fbgemm_amd {
@@ -19,7 +19,7 @@ namespace fbgemm_amd {
 namespace {
 
 constexpr int THREADS = 256;
-// Bytes of the results from which on they are marked as not read again soon: 168 MB (16 384 tokens of 40 heads of 128) 65.9 -> 60.5 us,
+// Bytes of the results from which on they are marked as not read again soon: 168 MB (16 384 tokens of 40 heads of 128, four a workgroup) 65.9 -> 60.5 us,
 // 31 MB (4 095 tokens of 24 heads of 80 fp32 numbers), which the last cache holds, 12.4 -> 16.0
 constexpr int64_t STREAM_FROM = 64 << 20;
 typedef __attribute__((ext_vector_type(4))) uint32_t piece16;
@@ -48,13 +48,10 @@ __device__ __forceinline__ Turn turn_of(double position, double frequency, float
   return Turn{(quadrant == 1 || quadrant == 2 ? -cosine : cosine) * magnitude, (quadrant & 2 ? -sine : sine) * sine_magnitude};
 }
 
-// the sines of a workgroup's tokens
-__device__ __forceinline__ void make_turns(const RotateArgs& a, int64_t first, int tokens, Turn* turns) {
-  for (int i = threadIdx.x; i < tokens * a.pairs; i += THREADS) {
-    const int t = i / a.pairs;
-    const int64_t position = a.idx64 ? reinterpret_cast<const int64_t*>(a.positions)[first + t] : reinterpret_cast<const int32_t*>(a.positions)[first + t];
-    turns[i] = turn_of((double)position, a.frequencies[i - t * a.pairs], a.magnitude, a.sine);
-  }
+// the sines of a token
+__device__ __forceinline__ void make_turns(const RotateArgs& a, int64_t token, Turn* turns) {
+  const int64_t position = a.idx64 ? reinterpret_cast<const int64_t*>(a.positions)[token] : reinterpret_cast<const int32_t*>(a.positions)[token];
+  for (int i = threadIdx.x; i < a.pairs; i += THREADS) turns[i] = turn_of((double)position, a.frequencies[i], a.magnitude, a.sine);
   __syncthreads();
 }
 
@@ -107,19 +104,17 @@ __device__ __forceinline__ float second_of(float a, float b, Turn t) { return ro
 struct Place {
   const char* in;
   char* out;
-  int token, unit;
+  int unit;
   bool same; // out is in
 };
-__device__ __forceinline__ Place place_of(const RotateArgs& a, int64_t first, uint32_t item) {
+__device__ __forceinline__ Place place_of(const RotateArgs& a, int64_t token, uint32_t item) {
   Place p;
-  const uint32_t row = divide(item, a.units);
-  p.unit = (int)(item - row * a.units.d);
-  p.token = (int)divide(row, a.all_heads);
-  int head = (int)(row - p.token * a.all_heads.d);
+  int head = (int)divide(item, a.units);
+  p.unit = (int)(item - head * a.units.d);
   const int k = head >= a.heads[0];
   if (k) head -= a.heads[0];
-  p.in = a.in[k] + (first + p.token) * a.in_token[k] + head * a.in_head[k];
-  p.out = a.out[k] + (first + p.token) * a.out_token[k] + head * a.out_head[k];
+  p.in = a.in[k] + token * a.in_token[k] + head * a.in_head[k];
+  p.out = a.out[k] + token * a.out_token[k] + head * a.out_head[k];
   p.same = p.in == p.out;
   return p;
 }
@@ -145,7 +140,7 @@ __device__ __forceinline__ void turn_piece(const RotateArgs& a, const Place& p, 
     const int at = 2 * a.pairs * C::BYTES + (p.unit - turning) * 16;
     store_piece<STREAMED>(p.out + at, load_piece<STREAMED>(p.in + at));
   } else if constexpr (INTERLEAVED) {
-    const Turn* turn = turns + p.token * a.pairs + p.unit * (N / 2);
+    const Turn* turn = turns + p.unit * (N / 2);
     piece16 w = load_piece<STREAMED>(p.in + p.unit * 16);
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
@@ -154,7 +149,7 @@ __device__ __forceinline__ void turn_piece(const RotateArgs& a, const Place& p, 
     }
     store_piece<STREAMED>(p.out + p.unit * 16, w);
   } else {
-    const Turn* turn = turns + p.token * a.pairs + p.unit * N;
+    const Turn* turn = turns + p.unit * N;
     const int other = a.pairs * C::BYTES;
     piece16 v = load_piece<STREAMED>(p.in + p.unit * 16), w = load_piece<STREAMED>(p.in + p.unit * 16 + other);
 #pragma unroll
@@ -175,7 +170,7 @@ __device__ __forceinline__ void turn_element(const RotateArgs& a, const Place& p
   if (p.unit < a.pairs) {
     const int e = (a.interleaved ? 2 * p.unit : p.unit) * C::BYTES, f = e + (a.interleaved ? 1 : a.pairs) * C::BYTES;
     const float x = C::at(p.in + e), y = C::at(p.in + f);
-    const Turn turn = turns[p.token * a.pairs + p.unit];
+    const Turn turn = turns[p.unit];
     C::set(p.out + e, first_of(x, y, turn));
     C::set(p.out + f, second_of(x, y, turn));
   } else if (!p.same) {
@@ -189,13 +184,12 @@ enum { ELEMENTS, HALVES, NEIGHBOURS };
 template <int TY, int FORM, bool STREAMED>
 __global__ __launch_bounds__(THREADS) void rotate_positions_kernel(const RotateArgs a) {
   extern __shared__ Turn s_turns[];
-  for (int64_t first = (int64_t)blockIdx.x * a.token_group; first < a.tokens; first += (int64_t)gridDim.x * a.token_group) {
-    const int tokens = (int)(a.tokens - first < a.token_group ? a.tokens - first : a.token_group);
-    __syncthreads(); // the last group's turns have been read
-    make_turns(a, first, tokens, s_turns);
-    const uint32_t items = (uint32_t)tokens * a.all_heads.d * a.units.d;
+  const uint32_t items = (uint32_t)(a.heads[0] + a.heads[1]) * a.units.d;
+  for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
+    __syncthreads(); // the last token's turns have been read
+    make_turns(a, token, s_turns);
     for (uint32_t i = threadIdx.x; i < items; i += THREADS) {
-      const Place p = place_of(a, first, i);
+      const Place p = place_of(a, token, i);
       if constexpr (FORM == ELEMENTS) turn_element<TY>(a, p, s_turns);
       else turn_piece<TY, FORM == NEIGHBOURS, STREAMED>(a, p, s_turns);
     }
@@ -211,12 +205,8 @@ void launch(RotateArgs a, bool aligned16, hipStream_t stream) {
   const int units = pieces ? (a.interleaved ? 2 * a.pairs / N : a.pairs / N) + rest / N : a.pairs + rest;
   const int heads = a.heads[0] + a.heads[1];
   a.units = make_divisor((uint32_t)units);
-  a.all_heads = make_divisor((uint32_t)heads);
-  // Four tokens a workgroup where the device is full all the same
-  a.token_group = a.tokens >= 8192 ? 4 : 1;
-  const int64_t groups = (a.tokens + a.token_group - 1) / a.token_group;
-  const unsigned grid = (unsigned)(groups < (1 << 22) ? groups : 1 << 22);
-  const size_t lds = (size_t)a.token_group * a.pairs * sizeof(Turn);
+  const unsigned grid = (unsigned)(a.tokens < (1 << 22) ? a.tokens : 1 << 22);
+  const size_t lds = (size_t)a.pairs * sizeof(Turn);
   const bool streamed = a.tokens * heads * a.dim * Chunk<TY>::BYTES >= STREAM_FROM;
   const auto kernel = !pieces ? rotate_positions_kernel<TY, ELEMENTS, false>
       : a.interleaved ? (streamed ? rotate_positions_kernel<TY, NEIGHBOURS, true> : rotate_positions_kernel<TY, NEIGHBOURS, false>)

@@ -22,6 +22,11 @@
 // row is weighed once, a wave a run of its tokens, into bins of logits of its own, which say the bin where top-p's sum is reached
 // and the run where the draw falls; only that bin's tokens and that run are looked at again.
 //
+// Bound by memory only where rows have little to do: 256 rows of 131 071 logits in bf16 (67 MB, 13 us at a copy's rate), us a call:
+// the largest logit 23, the 50 largest 31, 200 and top-p 0.9 of those 36, min-p 0.05 28. A row with all its tokens weighs each of them,
+// some 20 fp64 operations: 60, and with top-p 0.9 of a flat row, an LDS atomic for each beside that, and two more looks at parts of
+// it: 89. Then it is the compute unit's issue and LDS that bound it. One row: 10.5 to 70 us, a chain of dependent steps.
+//
 // Finding where a count or a sum is reached, going down from the largest, by bins: of keys (fp32 bits in ascending order), then of
 // the keys of the bin that has it, until they are one; then the last token of that key that is within.
 #include <type_traits>
@@ -707,7 +712,7 @@ __device__ __forceinline__ Found draw_weighed(const Row<TY, THREADS>& row, Share
   };
   if (f.top_p >= 1.0f) return by_weight();
   // bins of logits, evenly from the largest one down to those that weigh nothing
-  const float per_logit = (float)RUN_BINS / fmaxf(most - least, 1e-30f);
+  const float per_logit = (float)RUN_BINS / fminf(fmaxf(most - least, 1e-30f), FLT_BIG);
   const auto bin_of = [&](float x) { return (int)fminf(fmaxf((most - x) * per_logit, 0.0f), (float)(RUN_BINS - 1)); };
   __syncthreads();
   for (int i = threadIdx.x; i < THREADS / 64 * RUN_BINS; i += THREADS) s.run[0][i] = 0;
@@ -945,8 +950,15 @@ hipError_t launch_shape(SampleArgs a, hipStream_t stream) {
 }
 template <int TY>
 hipError_t launch(const SampleArgs& a, hipStream_t stream) {
-  // a small row is no work for 16 waves
-  if (a.vocab <= 4096) return launch_shape<TY, 256>(a, stream);
+  // A row of 16 waves has a compute unit to itself, of rows of 4 waves three are there at once. Small rows are no work for 16 waves, and
+  // where there are rows to fill the device several times over, more rows at once are better than each of them faster. us with 16 and with 4
+  // waves (bf16; the largest logit, the 50 largest, all, top-p 0.9 of them):
+  //   1 row of 8 192             4.7 10.6 12.5 23.7    3.9  9.1 11.8 21.4
+  //   1 row of 16 384            5.2 11.4 14.8 26.7    4.8  9.2 17.0 30.8
+  //   300 rows of 32 000        11.7 25.9 37.1 65.0    8.9 13.9 39.1 60.8
+  //   1 024 rows of 32 000      26.8 54.4 77.0 132     19.0 27.9 70.3 112
+  //   300 rows of 65 536        14.5 31.8 51.8 88.9   12.4 17.9 67.6 104
+  if (a.vocab <= 8192 || (a.rows > a.compute_units && a.vocab <= 32768)) return launch_shape<TY, 256>(a, stream);
   return launch_shape<TY, 1024>(a, stream);
 }
 

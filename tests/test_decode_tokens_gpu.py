@@ -216,6 +216,26 @@ def test_uniform_numbers_and_temperatures_at_their_ends(decode):
     check_samples(decode, x, u, temperature=[1e-30, 1e-38, 1e-45, 1e30, float("inf"), 1e-3, 100.0, 3e38, 1.0], top_k=[100] * 9, top_p=[0.5] * 9, min_p=[0.9] * 9)
 
 
+def test_samples_of_logits_as_far_apart_as_numbers_are(decode):
+    """Their difference is beyond fp32, and a high temperature lets all of them weigh the same."""
+    for vocab in (6000, 40_000):
+        x = rows_of(8, 6, vocab, torch.float32) * 2e37
+        u = [0.0, 0.2, 0.4, 0.6, 0.8, 0.99]
+        for t in (1e38, 3e38, float("inf")):
+            check_samples(decode, x, u, temperature=[t] * 6, top_p=[0.5, 0.9, 0.1, 0.99, 1.0, 0.3])
+            check_samples(decode, x.bfloat16(), u, temperature=[t] * 6, top_p=[0.5, 0.9, 0.1, 0.99, 1.0, 0.3], min_p=[0.0, 0.3, 0.9, 0.0, 0.5, 0.99])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [8191, 8192, 20_001, 32_768, 32_769])
+def test_samples_of_more_rows_than_the_device_has_compute_units(decode, vocab, dtype):
+    rows = 300
+    rng = np.random.default_rng(vocab)
+    pick = lambda *of: rng.choice(of, rows).tolist()  # noqa: E731
+    check_samples(decode, rows_of(vocab, rows, vocab, dtype), rng.uniform(0, 1, rows).tolist(), temperature=pick(1.0, 0.0, 0.6, 1.4), top_k=pick(0, 0, 0, 50, 3000),
+                  top_p=pick(1.0, 1.0, 0.9, 0.99), min_p=pick(0.0, 0.0, 0.05))
+
+
 def test_samples_of_strided_shared_and_many_rows(decode):
     wide = rows_of(6, 5, 9050, torch.bfloat16)
     u = [0.1, 0.3, 0.5, 0.7, 0.9]
@@ -362,3 +382,23 @@ def test_refusals(decode):
     torch.cuda.synchronize()
     with pytest.raises(NotImplementedError):  # no CPU path
         decode.sample_tokens(s["logits"].cpu(), s["uniform"].cpu())
+
+
+@pytest.mark.parametrize("rows, rotary, temperature", [(16, True, 0.0), (16, True, 0.8), (4, False, 0.0), (4, True, 0.8), (8, True, 1.5)])
+def test_the_example_runs_with_positions_4_bit_rows_and_draws(decode, rows, rotary, temperature):
+    """Logits of the paged path against the dense layer. 16-bit rows: attention's outputs round to bf16 in both, as queries and keys that were turned
+    do. A row of 64 normal numbers has a range of some 5 standard deviations: codes of 8 bits are off by 5 / 255 / sqrt(12) = 0.006 of one, of 4
+    bits by 0.1. A score, of standard deviation 1, and so a weight is off by as much, and an output by both: 0.14 in 4 bits; twice that
+    for the worst of a few requests."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_decode.py")
+    spec = importlib.util.spec_from_file_location("paged_decode", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    said, lengths, logits, d = example.generate(requests=5, steps=20, rows8=rows == 8, rows4=rows == 4, rotary=rotary, temperature=temperature)
+    for r in range(5):
+        n = int(lengths[r])
+        assert (said[r, :n] >= 0).all() and (said[r, n:] == -1).all()
+        want = example.dense_logits(d, said[r, :n - 1]).float()
+        assert float((logits[r].float() - want).norm() / want.norm()) < {16: 0.02, 8: 0.05, 4: 0.28}[rows]
