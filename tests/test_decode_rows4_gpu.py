@@ -142,6 +142,25 @@ def test_read_of_many_tokens(decode, tokens, store):
     check_read(decode, read_case(decode, 1, lengths, None, 2, 16, 16, store, "hnd"), store, None, np.int32, tokens, 16)
 
 
+@pytest.mark.parametrize("store,dtype,tokens", [(4, torch.float32, 16_500), (4, torch.bfloat16, 33_001), (8, torch.float16, 33_001), (torch.bfloat16, None, 33_001)])
+def test_read_past_the_caches_gives_the_same_bits(decode, store, dtype, tokens):
+    """Results of more than 128 MB, and the same tokens in parts."""
+    blocks = -(-tokens // 16)
+    caches = [torch.randn((blocks, 8, 16, 128), device="cuda").bfloat16() for _ in "kv"]
+    bits = store if store in (4, 8) else 8
+    if store in (4, 8):
+        for i, c in enumerate(caches):
+            caches[i] = torch.randint(0, 256, (*c.shape[:3], decode.kv_row_bytes(128, store)), dtype=torch.uint8, device="cuda")
+            caches[i][..., :4] = torch.randn((*c.shape[:3], 2), device="cuda").half().view(torch.uint8)
+    tables = torch.randperm(blocks, device="cuda").int()[None]
+    at = lambda *v: torch.tensor(v, device="cuda")  # noqa: E731
+    got = decode.kv_cache_read(*caches, tables, at(0, tokens), tokens, 128, dtype, row_bits=bits)
+    for first in range(0, tokens, 1999):
+        n = min(1999, tokens - first)
+        want = decode.kv_cache_read(*caches, tables, at(0, n), n, 128, dtype, at(first), row_bits=bits)
+        assert all(torch.equal(x[first:first + n], y) for x, y in zip(got, want))
+
+
 @pytest.mark.parametrize("store", [4, 8, torch.float16])
 def test_read_of_tokens_without_a_page(decode, store):
     lengths, starts = [20, 40, 5], [0, 8, 0]

@@ -88,6 +88,22 @@ def test_rotation_of_far_positions(decode):
     assert torch.equal(got[0], x[0])
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype,tokens", [(torch.bfloat16, 4300), (torch.float16, 4300), (torch.float32, 2150)])
+def test_rotation_past_the_caches_gives_the_same_bits(decode, dtype, tokens, interleaved):
+    """Results of more than 64 MB, and the same tokens in parts."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(tokens)
+    q, k = (torch.randn((tokens, n, 128), device="cuda", generator=g).to(dtype) for n in (48, 16))
+    positions, f = torch.arange(tokens, device="cuda") * 3, decode.rotary_frequencies(96)
+    got = decode.rotate_positions(q, k, positions, f, interleaved=interleaved)
+    for part in torch.arange(tokens, device="cuda").split(1000):
+        want = decode.rotate_positions(q[part], k[part], positions[part], f, interleaved=interleaved)
+        assert all(torch.equal(x[part], y) for x, y in zip(got, want))
+    decode.rotate_positions(q, k, positions, f, interleaved=interleaved, out=(q, k))
+    assert torch.equal(q, got[0]) and torch.equal(k, got[1])
+
+
 def test_a_rotations_gradient_is_the_inverse(decode):
     """<R x, y> = <x, R' y> of the linear map, and turning back and forth: a rounding of each of the two turns."""
     g = torch.Generator(device="cuda")
