@@ -62,32 +62,59 @@ bool rows_apart(const fbgemm_amd_paged_cache& c, const int64_t (&strides)[3]) {
   return true;
 }
 
-// Two arrays of rows of `width_a` and `width_b` bytes, `stride_a` and `stride_b` apart, that share a byte (or may, where neither stride divides the other)
-bool rows_meet(const void* a, int64_t stride_a, int64_t width_a, const void* b, int64_t stride_b, int64_t width_b, int64_t rows) {
-  typedef __int128 wide; // strides are the caller's
-  const wide d = (wide)(uintptr_t)b - (wide)(uintptr_t)a, last_a = (wide)(rows - 1) * stride_a + width_a, last_b = (wide)(rows - 1) * stride_b + width_b;
-  if (d >= last_a || -d >= last_b) return false;
-  const int64_t every = std::gcd(stride_a, stride_b);
-  if (rows == 1 || every == 0) return true;
-  const wide r = (d % every + every) % every; // of b's rows behind a's, whole steps left out
-  return r < width_a || every - r < width_b;
-}
+typedef __int128 wide; // strides are the caller's
 
-// [tokens][heads][dim] as rows of `width` bytes, `stride` apart: a token's heads, or a head's tokens. apart: no two elements are one.
-struct Span {
-  int64_t rows, stride, width;
-  bool apart;
+// Rows of `row` bytes, `step` apart
+struct Line {
+  int64_t count, step;
+  wide row;
+  wide extent() const { return (wide)(count - 1) * step + row; }
+  int64_t moves() const { return count > 1 ? step : 0; }
 };
-Span span_of(const fbgemm_amd_head_rows& r, const int64_t (&strides)[2], int64_t tokens, int64_t dim, int64_t element) {
+// whether rows of `a` and `b`, where every row begins at a multiple of `every` behind the first one of its kind, can share a byte; b's first is d behind a's
+bool rows_within(wide a, wide b, wide d, int64_t every) {
+  const wide r = (d % every + every) % every; // of b's rows behind a's, whole steps left out
+  return r < a || every - r < b;
+}
+// Two lines, the second d bytes behind the first, that share a byte (or may, where neither step divides the other)
+bool lines_meet(const Line& a, const Line& b, wide d) {
+  if (d >= a.extent() || -d >= b.extent()) return false;
+  const int64_t every = std::gcd(a.moves(), b.moves());
+  return every == 0 || rows_within(a.row, b.row, d, every);
+}
+wide between(const void* a, const void* b) { return (wide)(uintptr_t)b - (wide)(uintptr_t)a; }
+
+// [tokens][heads][dim] as lines of rows: a token's heads, or a head's tokens, whichever are closer together. outer: these lines as solid rows
+struct Grid {
+  Line outer, inner;
+  // no two elements are one
+  bool apart() const { return (inner.count <= 1 || inner.step >= inner.row) && (outer.count <= 1 || outer.step >= outer.row); }
+};
+Grid grid_of(const fbgemm_amd_head_rows& r, const int64_t (&strides)[2], int64_t tokens, int64_t dim, int64_t element) {
   const int64_t size[2] = {tokens, r.heads};
   const int outer = r.heads == 1 || (tokens > 1 && strides[0] >= strides[1]) ? 0 : 1, inner = 1 - outer;
-  Span s{size[outer], size[outer] > 1 ? strides[outer] * element : 0, ((size[inner] > 1 ? (size[inner] - 1) * strides[inner] : 0) + dim) * element, true};
-  s.apart = (size[inner] <= 1 || strides[inner] >= dim) && (s.rows <= 1 || s.stride >= s.width);
-  return s;
+  Grid g;
+  g.inner = Line{size[inner], strides[inner] * element, dim * element};
+  g.outer = Line{size[outer], strides[outer] * element, g.inner.extent()};
+  return g;
 }
-bool spans_meet(const void* a, const Span& x, const void* b, const Span& y) {
-  if (x.rows == y.rows) return rows_meet(a, x.stride, x.width, b, y.stride, y.width, x.rows);
-  return rows_meet(a, 0, (x.rows - 1) * x.stride + x.width, b, 0, (y.rows - 1) * y.stride + y.width, 1);
+// Two grids that share a byte (or may, where they are laid out differently). What one has between its rows may be the other's: queries and
+// keys of a projection [tokens][heads][3][dim] do not meet.
+bool grids_meet(const void* a, const Grid& x, const void* b, const Grid& y) {
+  const wide d = between(a, b);
+  if (!lines_meet(x.outer, y.outer, d)) return false;
+  const int64_t every = std::gcd(std::gcd(x.outer.moves(), x.inner.moves()), std::gcd(y.outer.moves(), y.inner.moves()));
+  if (every != 0 && !rows_within(x.inner.row, y.inner.row, d, every)) return false;
+  if (x.outer.moves() && y.outer.moves() && x.outer.step != y.outer.step) return true;
+  const int64_t step = std::max(x.outer.moves(), y.outer.moves());
+  if (step == 0) return lines_meet(x.inner, y.inner, d);
+  // line j of y begins d + (j - i) * step behind line i of x: those that are near enough, of lines inside one step no more than two
+  wide k = std::max<wide>(-(wide)(x.outer.count - 1), (-y.outer.row - d) / step - 1);
+  const wide last = std::min<wide>(y.outer.count - 1, (x.outer.row - d) / step + 1);
+  if (last - k > 8) return true;
+  for (; k <= last; ++k)
+    if (lines_meet(x.inner, y.inner, d + k * step)) return true;
+  return false;
 }
 
 // a status block holds a 64-bit number that kernels update atomically
@@ -352,7 +379,7 @@ int fbgemm_amd_rotate_positions(
     if (!r || r->heads == 0) continue;
     if (!r->in || !r->out) return fail(FBGEMM_AMD_E_ARG, "null data pointer");
     if ((uintptr_t)r->in % e || (uintptr_t)r->out % e) return fail(FBGEMM_AMD_E_ARG, "rows are not aligned to their elements");
-    if (!span_of(*r, r->out_strides, tokens, dim, e).apart) return fail(FBGEMM_AMD_E_ARG, "rows of a result must not overlap");
+    if (!grid_of(*r, r->out_strides, tokens, dim, e).apart()) return fail(FBGEMM_AMD_E_ARG, "rows of a result must not overlap");
     a.in[k] = (const char*)r->in;
     a.out[k] = (char*)r->out;
     a.in_token[k] = r->in_strides[0] * e;
@@ -366,10 +393,10 @@ int fbgemm_amd_rotate_positions(
     for (int i = 0; i < 2; ++i) {
       if (!a.heads[k] || !a.heads[i]) continue;
       const bool in_place = i == k && a.in[k] == a.out[k] && (tokens == 1 || a.in_token[k] == a.out_token[k]) && (a.heads[k] == 1 || a.in_head[k] == a.out_head[k]);
-      const Span out = span_of(*of[k], of[k]->out_strides, tokens, dim, e);
-      if (!in_place && spans_meet(a.in[i], span_of(*of[i], of[i]->in_strides, tokens, dim, e), a.out[k], out))
+      const Grid out = grid_of(*of[k], of[k]->out_strides, tokens, dim, e);
+      if (!in_place && grids_meet(a.in[i], grid_of(*of[i], of[i]->in_strides, tokens, dim, e), a.out[k], out))
         return fail(FBGEMM_AMD_E_ARG, "a result may be its own input, but must not overlap inputs otherwise");
-      if (i < k && spans_meet(a.out[i], span_of(*of[i], of[i]->out_strides, tokens, dim, e), a.out[k], out))
+      if (i < k && grids_meet(a.out[i], grid_of(*of[i], of[i]->out_strides, tokens, dim, e), a.out[k], out))
         return fail(FBGEMM_AMD_E_ARG, "the results must not overlap each other");
     }
   a.dim = dim;
@@ -475,7 +502,7 @@ int fbgemm_amd_penalize_logits(
   if (d_mask && rows > 1 && mask_stride != 0 && mask_stride < (vocab + 31) / 32) return fail(FBGEMM_AMD_E_ARG, "a row of the mask has one bit per token of the vocabulary");
   const int64_t e = storage_bytes(logits_ty);
   const bool in_place = d_output == d_logits && (rows == 1 || output_stride == logits_stride);
-  if (!in_place && rows_meet(d_logits, rows > 1 ? logits_stride * e : 0, vocab * e, d_output, rows > 1 ? output_stride * e : 0, vocab * e, rows))
+  if (!in_place && lines_meet(Line{rows, logits_stride * e, vocab * e}, Line{rows, output_stride * e, vocab * e}, between(d_logits, d_output)))
     return fail(FBGEMM_AMD_E_ARG, "the result may be the logits themselves, but must not overlap them otherwise");
   LogitsArgs a;
   a.logits = d_logits;
