@@ -1,5 +1,8 @@
 // torch operators of a decoding step, continued (torch_op_decode.cpp): rotary positions, cache rows read back,
 // sampling. The same manner: namespace fbgemm_amd, all work through the C ABI, results from torch's allocator.
+// The rotation has a gradient; where it writes into given tensors it refuses to be recorded.
+#include <torch/csrc/autograd/custom_function.h>
+
 #include <tuple>
 
 #include "torch_op_decode.h"
@@ -77,6 +80,78 @@ std::tuple<Tensor, Tensor> rotate_new(
   return rotate(query, key, positions, frequencies, interleaved, magnitude, inverse, at::empty(query.sizes(), query.options()), at::empty(key.sizes(), key.options()));
 }
 
+// ---- the rotation's gradient ----
+
+// the operators as the dispatcher has them
+const auto& dispatched() {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fbgemm_amd::rotate_positions", "").typed<decltype(rotate_new)>();
+  return op;
+}
+const auto& dispatched_out() {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fbgemm_amd::rotate_positions", "out").typed<decltype(rotate)>();
+  return op;
+}
+
+// Linear in queries and keys: a gradient goes the other way round, with the same magnitude, by the operator itself (so that it has a gradient too)
+struct Rotation : torch::autograd::Function<Rotation> {
+  static torch::autograd::variable_list forward(
+      torch::autograd::AutogradContext* ctx, const Tensor& query, const Tensor& key, const Tensor& positions, const Tensor& frequencies, bool interleaved,
+      double magnitude, bool inverse) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({positions, frequencies});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["magnitude"] = magnitude;
+    ctx->saved_data["inverse"] = inverse;
+    const auto turned = dispatched().call(query, key, positions, frequencies, interleaved, magnitude, inverse);
+    return {std::get<0>(turned), std::get<1>(turned)};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list result(7);
+    const bool of[2] = {grads[0].defined() && ctx->needs_input_grad(0), grads[1].defined() && ctx->needs_input_grad(1)};
+    if (!of[0] && !of[1]) return result;
+    Tensor in[2];
+    for (int k = 0; k < 2; ++k) {
+      if (of[k]) in[k] = grads[k].size(2) > 1 && grads[k].stride(2) != 1 ? grads[k].contiguous() : grads[k]; // (that of a sum is one number for all)
+      else in[k] = grads[1 - k].new_empty({grads[1 - k].size(0), 0, grads[1 - k].size(2)}); // no heads
+    }
+    const auto saved = ctx->get_saved_variables();
+    const auto back = dispatched().call(in[0], in[1], saved[0], saved[1], ctx->saved_data["interleaved"].toBool(), ctx->saved_data["magnitude"].toDouble(),
+                                 !ctx->saved_data["inverse"].toBool());
+    if (of[0]) result[0] = std::get<0>(back);
+    if (of[1]) result[1] = std::get<1>(back);
+    return result;
+  }
+};
+// whether what is made of a tensor would be followed
+bool followed(const Tensor& t) { return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined(); }
+
+std::tuple<Tensor, Tensor> rotate_new_autograd(
+    c10::DispatchKeySet keys, const Tensor& query, const Tensor& key, const Tensor& positions, const Tensor& frequencies, bool interleaved, double magnitude, bool inverse) {
+  TORCH_CHECK(!followed(frequencies), "fbgemm_amd: rotate_positions has no gradient for its frequencies");
+  if (!followed(query) && !followed(key))
+    return dispatched().redispatch(keys & c10::after_ADInplaceOrView_keyset, query, key, positions, frequencies, interleaved, magnitude, inverse);
+  const auto turned = Rotation::apply(query, key, positions, frequencies, interleaved, magnitude, inverse);
+  return {turned[0], turned[1]};
+}
+std::tuple<Tensor, Tensor> rotate_autograd(
+    c10::DispatchKeySet keys, const Tensor& query, const Tensor& key, const Tensor& positions, const Tensor& frequencies, bool interleaved, double magnitude, bool inverse,
+    Tensor query_out, Tensor key_out) {
+  for (const Tensor* t : {&query, &key, &frequencies, (const Tensor*)&query_out, (const Tensor*)&key_out})
+    TORCH_CHECK(!followed(*t), "fbgemm_amd: rotate_positions into given tensors has no gradient, and one of its tensors requires it: "
+                               "take new results, or call it under torch.no_grad()");
+  return dispatched_out().redispatch(keys & c10::after_autograd_keyset, query, key, positions, frequencies, interleaved, magnitude, inverse, query_out, key_out);
+}
+// given tensors have other contents now: a graph that holds the former ones has to know
+std::tuple<Tensor, Tensor> rotate_written(
+    c10::DispatchKeySet keys, const Tensor& query, const Tensor& key, const Tensor& positions, const Tensor& frequencies, bool interleaved, double magnitude, bool inverse,
+    Tensor query_out, Tensor key_out) {
+  dispatched_out().redispatch(keys & c10::after_ADInplaceOrView_keyset, query, key, positions, frequencies, interleaved, magnitude, inverse, query_out, key_out);
+  for (const Tensor* t : {(const Tensor*)&query_out, (const Tensor*)&key_out})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  return {query_out, key_out};
+}
+
 std::tuple<Tensor, Tensor> sample_tokens(
     const Tensor& logits, const Tensor& uniform, const OptTensor& temperature, const OptTensor& top_k, const OptTensor& top_p, const OptTensor& min_p) {
   TORCH_CHECK(logits.dim() == 2, "fbgemm_amd: logits must be [rows, vocab], got ", logits.sizes());
@@ -143,3 +218,8 @@ TORCH_LIBRARY_IMPL(fbgemm_amd, Meta, m) {
   m.impl("rotate_positions.out", TORCH_FN(rotate_out_meta));
   m.impl("sample_tokens", TORCH_FN(sample_tokens_meta));
 }
+TORCH_LIBRARY_IMPL(fbgemm_amd, Autograd, m) {
+  m.impl("rotate_positions", TORCH_FN(rotate_new_autograd));
+  m.impl("rotate_positions.out", TORCH_FN(rotate_autograd));
+}
+TORCH_LIBRARY_IMPL(fbgemm_amd, ADInplaceOrView, m) { m.impl("rotate_positions.out", TORCH_FN(rotate_written)); }

@@ -112,7 +112,8 @@ def rotate_positions(query, key, positions, frequencies, interleaved=False, magn
     ``rotary_frequencies``); the elements behind them stay as they are. Angles are taken in fp64, products in fp32, rounded once.
     With ``inverse`` the other way round, with the same magnitude: what a gradient goes through, or a key that gives up its position.
 
-    Returns new tensors, or ``out``, a pair, which may be ``(query, key)``; nothing else that is read may overlap it."""
+    Returns new tensors, through which gradients go to ``query`` and ``key``, or ``out``, a pair, which may be ``(query, key)``; nothing
+    else that is read may overlap it. Into ``out`` there is no gradient: a call that would need one is refused (``torch.no_grad()``)."""
     if out is None:
         return _rotate(query, key, positions, frequencies, interleaved, magnitude, inverse)
     return _rotate_out(query, key, positions, frequencies, interleaved, magnitude, inverse, query_out=out[0], key_out=out[1])

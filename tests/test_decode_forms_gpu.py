@@ -1,6 +1,9 @@
 """Forms of the decoding step's operators that a program may use and that no other file here runs: layouts, gradients, extremes."""
 import pytest
 
+import decode_tokens_reference as R
+from test_decode_finite_gpu import close_and_finite as close
+from test_decode_gpu import np64
 from test_decode_tokens_gpu import TYPES, check_rotation
 
 torch = pytest.importorskip("torch")
@@ -30,3 +33,63 @@ def test_rotation_of_heads_whose_parts_are_side_by_side(decode, tokens, dtype, i
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and (places[:, :, 1] == 0).all()
     decode.rotate_positions(query, key, positions, f, interleaved=interleaved, out=(query, key))
     assert torch.equal(query, want[0]) and torch.equal(key, want[1]) and torch.equal(value, held)
+
+
+@pytest.mark.parametrize("inverse", [False, True])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_of_a_rotation(decode, dtype, interleaved, inverse):
+    """Of a fused projection's parts, through autograd: the formula's in 64 bits, and differences of single elements."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(7)
+    normal = lambda *shape: torch.randn(shape, device="cuda", generator=g)  # noqa: E731
+    fused = normal(40, 12, 64).to(dtype).requires_grad_()
+    positions, f = torch.randint(0, 5000, (40,), device="cuda", generator=g), decode.rotary_frequencies(48)
+    kw = dict(interleaved=interleaved, magnitude=1.25, inverse=inverse)
+    query, key = decode.rotate_positions(fused[:, :8], fused[:, 8:10], positions, f, **kw)
+    back = [normal(40, 8, 64).to(dtype), normal(40, 2, 64).to(dtype)]
+    got, = torch.autograd.grad((query, key), fused, back)
+    for k, part in enumerate((slice(0, 8), slice(8, 10))):
+        want, off = R.rotate(np64(back[k]), positions.cpu().numpy(), f.cpu().numpy(), interleaved, 1.25, inverse=not inverse)
+        close(got[:, part], want, off, dtype)
+    assert (got[:, 10:] == 0).all()
+    # against differences: the map is linear, so a step of one will do; fp32 numbers, some 64 products of 2^-21
+    if dtype == torch.float32:
+        with torch.no_grad():
+            for t, h, d in ((3, 1, 5), (39, 9, 40), (0, 8, 63)):
+                there = fused.detach().clone()
+                there[t, h, d] += 1.0
+                a, b = decode.rotate_positions(there[:, :8], there[:, 8:10], positions, f, **kw)
+                change = ((a.double() - query.double()) * back[0]).sum() + ((b.double() - key.double()) * back[1]).sum()
+                assert abs(float(change) - float(got[t, h, d])) < 64 * 2.0 ** -21 * 16
+    # only one of the two, gradients that are one number for all, and a gradient's gradient
+    q = normal(40, 8, 64).to(dtype).requires_grad_()
+    decode.rotate_positions(q, fused[:, 8:10].detach(), positions, f, **kw)[0].sum().backward()
+    want, off = R.rotate(np64(torch.ones_like(q)), positions.cpu().numpy(), f.cpu().numpy(), interleaved, 1.25, inverse=not inverse)
+    close(q.grad, want, off, dtype)
+    v = back[0].clone().requires_grad_()
+    first, = torch.autograd.grad(decode.rotate_positions(q, q, positions, f, **kw)[0], q, v, create_graph=True)
+    w = normal(40, 8, 64).to(dtype)
+    second, = torch.autograd.grad(first, v, w)
+    want, off = R.rotate(np64(w), positions.cpu().numpy(), f.cpu().numpy(), interleaved, 1.25, inverse=inverse)
+    close(second, want, off, dtype)
+    # on another stream, whose backward runs there too
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again, = torch.autograd.grad(decode.rotate_positions(fused[:, :8], fused[:, 8:10], positions, f, **kw), fused, back)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(again, got)
+
+
+def test_given_tensors_that_a_graph_follows_are_refused(decode):
+    x = torch.randn((5, 12, 64), device="cuda", requires_grad=True) * 1
+    q, k, p, f = x[:, :8], x[:, 8:10], torch.arange(5, device="cuda"), decode.rotary_frequencies(64)
+    held = x.detach().clone()
+    for call in (lambda: decode.rotate_positions(q, k, p, f, out=(q, k)), lambda: decode.rotate_positions(q.detach(), k.detach(), p, f, out=(q, k))):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+    assert torch.equal(x, held)
+    with torch.no_grad():
+        decode.rotate_positions(q, k, p, f, out=(q, k))
+    assert not torch.equal(x, held)
