@@ -160,7 +160,7 @@ template <int ROWS = 8>
 __device__ __forceinline__ float middle(uint32_t pair) { return __builtin_fmaf(ROWS == 8 ? 128.0f : 8.0f, half_at(pair, 0), half_at(pair, 1)); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // tanh(x) / x = 1 - x^2/3 + 2 x^4/15 - ..., for |x| < TANH_SMALL to 2^-24 (the next term: 0.0036 x^12)
-constexpr float TANH_SMALL = 0.35f, FLT_MOST = 3.4028234663852886e38f, FLT_LEAST = 1.17549435e-38f;
+constexpr float TANH_SMALL = 0.35f, FLT_MOST = 3.4028234663852886e38f, FLT_LEAST = 1.17549435e-38f, FAR = 1.6777216e7f; // the last: 2^24
 __device__ __forceinline__ float tanh_ratio(float x) {
   const float z = x * x;
   float p = -1382.0f / 155925.0f;
@@ -482,6 +482,7 @@ struct Attention {
   // 4-bit rows: scores (and their maximum) are in units of 1 / unit, so that queries need no factor for each: what a unit is, unless a cap
   // has made plain scores of them; the factor that does. And the products of code 8, which is taken off afterwards, at even and at odd columns.
   float unit, to_plain;
+  bool far; // some maximum is so many times 1 / unit that rounding their product would change weights, and soon make them infinite
   f32x4 eights[2];
 
   __device__ __forceinline__ void begin(int32_t request, int head, int q0, int rows) {
@@ -512,6 +513,7 @@ struct Attention {
     eights[0] = eights[1] = f32x4{0, 0, 0, 0};
     m = -__builtin_inff();
     l = bias = 0.0f;
+    far = false;
   }
 
   // 4-bit rows: the queries' elements in the codes' order. bf16: the largest is brought to 2^126, so that products with subnormal
@@ -673,13 +675,22 @@ struct Attention {
       if (ROWS4) {
         eights[0] *= f;
         eights[1] *= f;
+        far = __builtin_amdgcn_ballot_w64(__builtin_fabsf(m * unit) > FAR && m != -__builtin_inff()) != 0;
       }
     }
     const float ref = m == -__builtin_inff() ? 0.0f : ROWS4 ? m * unit : m - SHIFT; // nothing seen yet: all weights 0
     float p[8];
+    if (ROWS4 && far) { // differences first: exact, where they matter
+      const float least = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = (s[j] - least) * unit;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = ROWS4 ? __builtin_fmaf(s[j], unit, -ref) : s[j] - ref;
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = exp2_fast(ROWS4 ? __builtin_fmaf(s[j], unit, -ref) : s[j] - ref);
+      p[j] = exp2_fast(p[j]);
       if (ROWS4) p[j] = __builtin_amdgcn_ldexpf(p[j], WEIGHT_UP);
       l += p[j];
     }

@@ -1,7 +1,9 @@
 """Forms of the decoding step's operators that a program may use and that no other file here runs: layouts, gradients, extremes."""
+import numpy as np
 import pytest
 
 import decode_tokens_reference as R
+import test_decode_rows4_gpu as A
 from test_decode_finite_gpu import close_and_finite as close
 from test_decode_gpu import np64
 from test_decode_tokens_gpu import TYPES, check_rotation
@@ -93,3 +95,48 @@ def test_given_tensors_that_a_graph_follows_are_refused(decode):
     with torch.no_grad():
         decode.rotate_positions(q, k, p, f, out=(q, k))
     assert not torch.equal(x, held)
+
+
+def large_case(decode, dim, power, dtype, down, block=16):
+    """Queries of up to 2^power, and keys that are 2^-down of attention_case's."""
+    query, caches, tables, lengths = A.attention_case(decode, dim, dim, 4, 2, block, [1, 33, 200], dtype)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(power)
+    query = ((2 * torch.rand(query.shape, device="cuda", generator=g, dtype=torch.float64) - 1) * 2.0 ** power).clamp(-float(torch.finfo(dtype).max), float(torch.finfo(dtype).max)).to(dtype)
+    pair = caches[0][..., :4].clone().view(torch.float16)
+    caches[0][..., :4] = (pair.float() * 2.0 ** -down).half().view(torch.uint8)
+    return query, caches, tables, lengths
+
+
+def one_token_each(case, scale):
+    """Where the largest score is so far above the next one, rounded however, that its token's value is the output: which, and that value."""
+    query, caches, tables, lengths = case
+    B, Hq, D = query.shape
+    H, S = caches[0].shape[1:3]
+    hosts, q = [c.cpu().numpy() for c in caches], np64(query)
+    sure, value = np.zeros((B, Hq), bool), np.zeros((B, Hq, D))
+    for r, n in enumerate(lengths.tolist()):
+        at = lambda c, h: c[tables[r].cpu().numpy()[np.arange(n) // S], h, np.arange(n) % S]  # noqa: E731
+        for h in range(Hq):
+            k, v = (R.rows4_values(at(c, h // (Hq // H)), D) for c in hosts)
+            s, wrong = scale * (k @ q[r, h]), (D + 8) * 2.0 ** -22 * abs(scale) * 15 * (np.abs(k).max(0) @ np.abs(q[r, h]))
+            order = np.argsort(s)
+            sure[r, h] = n == 1 or s[order[-1]] - s[order[-2]] > 2 * wrong + 100
+            value[r, h] = v[order[-1]]
+    return sure, value
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("block", [16, 10])
+@pytest.mark.parametrize("power", [10, 20, 26, 30, 40, 60])
+def test_attention_over_4_bit_rows_of_large_scores(decode, power, block, dtype):
+    """Scores of 2^power and beyond: their differences are what weights are made of, however large they are themselves."""
+    case = large_case(decode, 128, 0, dtype, 0, block)
+    A.check(decode, case, dtype, scale=2.0 ** power)
+    A.check(decode, case, dtype, scale=-2.0 ** power, window=40)
+    if power >= 20:
+        out, lse = decode.paged_attention(case[0], *case[1], *case[2:], scale=2.0 ** power, row_bits=4)
+        sure, value = one_token_each(case, 2.0 ** power)
+        assert sure.mean() > 0.8
+        near = 2.0 ** -15 * 30 * np.abs(value).max() + torch.finfo(dtype).eps * np.abs(value)
+        assert (np.abs(np64(out) - value) <= near)[sure].all()
