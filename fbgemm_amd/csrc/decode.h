@@ -109,6 +109,8 @@ struct AttentionArgs {
   int64_t max_tokens; // table width * block size
   Divisor block;
   float scale;       // of the scores, times log2(e)
+  float scale_part;  // |scale| (but at least the smallest normal number) is scale_part * 2^scale_up, scale_part in [1/2, 1]
+  int32_t scale_up;
   float softcap;     // times log2(e); 0: none
   float cap_inverse; // 1 / softcap
   int64_t window; // 0: none

@@ -463,6 +463,9 @@ int fbgemm_amd_paged_attention(
   a.block = make_divisor((uint32_t)cache->block_size);
   constexpr double LOG2E = 1.4426950408889634;
   a.scale = (float)(scale * LOG2E);
+  int up = 0;
+  a.scale_part = (float)std::frexp(std::max(std::fabs(scale * LOG2E), (double)std::numeric_limits<float>::min()), &up);
+  a.scale_up = up;
   // normal and of a finite inverse for the smallest cap too: a score of zero times infinity would be none
   const double cap = softcap > 0.0f ? std::max(softcap * LOG2E, (double)std::numeric_limits<float>::min()) : 0.0;
   a.softcap = (float)cap;

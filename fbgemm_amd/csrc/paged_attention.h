@@ -160,7 +160,7 @@ template <int ROWS = 8>
 __device__ __forceinline__ float middle(uint32_t pair) { return __builtin_fmaf(ROWS == 8 ? 128.0f : 8.0f, half_at(pair, 0), half_at(pair, 1)); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // tanh(x) / x = 1 - x^2/3 + 2 x^4/15 - ..., for |x| < TANH_SMALL to 2^-24 (the next term: 0.0036 x^12)
-constexpr float TANH_SMALL = 0.35f, FLT_MOST = 3.4028234663852886e38f, FLT_LEAST = 1.17549435e-38f, FAR = 1.6777216e7f; // the last: 2^24
+constexpr float TANH_SMALL = 0.35f, FLT_MOST = 3.4028234663852886e38f, FLT_LEAST = 1.17549435e-38f, UNIT_MOST = 1.2676506e30f, FAR = 1.6777216e7f; // the last: 2^100 and 2^24
 __device__ __forceinline__ float tanh_ratio(float x) {
   const float z = x * x;
   float p = -1382.0f / 155925.0f;
@@ -480,8 +480,10 @@ struct Attention {
   f32x4 acc[HALVES][VC];
   float m, l, bias;
   // 4-bit rows: scores (and their maximum) are in units of 1 / unit, so that queries need no factor for each: what a unit is, unless a cap
-  // has made plain scores of them; the factor that does. And the products of code 8, which is taken off afterwards, at even and at odd columns.
-  float unit, to_plain;
+  // has made plain scores of them, by |scale| and this exponent. And the products of code 8, which is taken off afterwards, at even and at
+  // odd columns.
+  float unit;
+  int plain_up;
   bool far; // some maximum is so many times 1 / unit that rounding their product would change weights, and soon make them infinite
   f32x4 eights[2];
 
@@ -519,7 +521,7 @@ struct Attention {
   // 4-bit rows: the queries' elements in the codes' order. bf16: the largest is brought to 2^126, so that products with subnormal
   // numbers are normal ones (an exact step, but for elements 2^-240 times smaller), and odd elements are 2^-4 of that. With a scale
   // below zero they change their sign, so that the largest score is the largest product. The exponent that brings their sum to
-  // the products' units
+  // the products' units (0: it has been)
   __device__ __forceinline__ int order_queries() {
     int e = 0, up = -20; // fp16: codes are 16 * 2^-24
     if constexpr (BF16) {
@@ -535,9 +537,20 @@ struct Attention {
       e = most > 0.0f && most <= FLT_MOST ? 126 - __builtin_amdgcn_frexp_expf(most) : 133;
       up = e - 133;
     }
-    // a number that is not 0, for scores of -inf, nor infinite, for those of 0
-    to_plain = __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(__builtin_fabsf(a.scale), -up), FLT_LEAST, FLT_MOST);
-    unit = a.softcap > 0.0f ? 1.0f : to_plain;
+    // Scores are below 2^24 units (of bf16 queries 2^21). A unit is not 0, for scores of -inf, and no more than 2^100, so that none becomes
+    // infinite; with more of it weights would tell scores apart that differ by less than 2^-93 of the largest element's share of one.
+    plain_up = a.scale_up - up;
+    unit = a.softcap > 0.0f ? 1.0f : __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(a.scale_part, plain_up), FLT_LEAST, UNIT_MOST);
+    const bool large = BF16 && __builtin_amdgcn_ballot_w64(e < 8) != 0; // a sum of numbers near the type's largest would be infinite
+    if (large) {
+      q_sum = 0.0f;
+#pragma unroll
+      for (int c = 0; c < KP; ++c) {
+        const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q_sum += __builtin_amdgcn_ldexpf(unpack16<BF16>(w[i], 0), up) + __builtin_amdgcn_ldexpf(unpack16<BF16>(w[i], 1), up);
+      }
+    }
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
     if (a.scale < 0.0f) q_sum = -q_sum;
 #pragma unroll
@@ -554,8 +567,9 @@ struct Attention {
       }
       q[c] = make_uint4(t[0] ^ flip, t[1] ^ flip, t[2] ^ flip, t[3] ^ flip);
     }
-    return up;
+    return large ? 0 : up;
   }
+  __device__ __forceinline__ float plain_score(float s) const { return __builtin_amdgcn_ldexpf(s * a.scale_part, plain_up); }
 
   // PACKED: a lane's part of the runs, through LDS, where no other wave looks. Lanes read what others wrote: that the wave's
   // writes and reads keep their order is said to the compiler, for which the addresses of one lane have nothing to do with each other
@@ -636,7 +650,7 @@ struct Attention {
     if (a.softcap > 0.0f) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (ROWS4) s[j] *= to_plain;
+        if (ROWS4) s[j] = plain_score(s[j]);
         const float x = s[j] * a.cap_inverse;
         s[j] = __builtin_fabsf(x) < TANH_SMALL ? s[j] * tanh_ratio(x) : a.softcap * tanh_fast(x);
       }
@@ -922,7 +936,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES, attention_residents(DP, ROWS, PAGE1
     if (A::ROWS4) { // as they are from here on
       x.l = __builtin_amdgcn_ldexpf(x.l, -A::WEIGHT_UP);
       x.bias = __builtin_amdgcn_ldexpf(x.bias, -A::WEIGHT_UP);
-      x.m *= x.unit;
+      if (!(a.softcap > 0.0f)) x.m = x.plain_score(x.m);
     }
     if (g == 0) {
       s_ml[wave][n][0] = x.m;

@@ -140,3 +140,28 @@ def test_attention_over_4_bit_rows_of_large_scores(decode, power, block, dtype):
         assert sure.mean() > 0.8
         near = 2.0 ** -15 * 30 * np.abs(value).max() + torch.finfo(dtype).eps * np.abs(value)
         assert (np.abs(np64(out) - value) <= near)[sure].all()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("power", [90, 100, 117, 119, 122, 125, 127])
+def test_attention_over_4_bit_rows_of_queries_near_the_types_largest(decode, power, dim):
+    """The logarithm of the sum is the largest score there, up to 2^112, and one token's value the output."""
+    case = large_case(decode, dim, power, torch.bfloat16, 18)
+    A.check(decode, case, torch.bfloat16)
+    out, lse = decode.paged_attention(case[0], *case[1], *case[2:], row_bits=4)
+    assert lse.abs().max() > 2.0 ** (power - 24)
+    sure, value = one_token_each(case, dim ** -0.5)
+    assert sure.mean() > 0.8
+    # weights of 16 bits, a rounding to bf16, and codes up to 15 in sums of fp32
+    near = 2.0 ** -15 * 30 * np.abs(value).max() + torch.finfo(torch.bfloat16).eps * np.abs(value)
+    assert (np.abs(np64(out) - value) <= near)[sure].all()
+    A.check(decode, case, torch.bfloat16, softcap=2.0 ** (power - 20))  # caps that leave most scores a slope
+    A.check(decode, case, torch.bfloat16, scale=-dim ** -0.5, window=17)
+
+
+@pytest.mark.parametrize("power", [80, 100, 110])
+def test_attention_over_4_bit_rows_with_large_scales(decode, power):
+    for dtype in (torch.float16, torch.bfloat16):
+        case = large_case(decode, 128, 0, dtype, 4)
+        A.check(decode, case, dtype, scale=2.0 ** power)
+        A.check(decode, case, dtype, scale=-2.0 ** power, softcap=2.0 ** (power - 3))
