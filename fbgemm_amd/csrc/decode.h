@@ -131,6 +131,16 @@ constexpr int attention_residents(int dim, int bits, bool pages) {
   if (bits == 4) return pages ? 3 : 2;
   return dim > 64 ? 2 : 3;
 }
+// How the attention kernel finds rows of `bits` bits: lane by lane; in pages of whole tiles of 16 tokens, whose addresses are the wave's; or there as
+// runs of bytes, where a page's rows follow each other without gaps and 16 of them are what its loads are laid out for (however far apart
+// pages are, of keys or of values).
+enum AttentionForm : int { ATTENTION_LANES, ATTENTION_PAGES, ATTENTION_RUNS };
+constexpr bool attention_has_runs(int dim, int bits) { return bits == 8 ? dim == 64 || dim == 128 || dim == 256 : bits == 4 && (dim == 128 || dim == 256); }
+inline AttentionForm attention_form(int dim, int bits, int block_size, int64_t key_slot_stride, int64_t value_slot_stride) {
+  if (block_size % 16) return ATTENTION_LANES;
+  const int64_t row = dim * bits / 8 + 4;
+  return attention_has_runs(dim, bits) && key_slot_stride == row && value_slot_stride == row ? ATTENTION_RUNS : ATTENTION_PAGES;
+}
 constexpr int ATTENTION_ROWS = 16; // queries of a key head that one tile of the matrix cores takes
 hipError_t launch_paged_attention_bf16(const AttentionArgs& a, hipStream_t stream);
 hipError_t launch_paged_attention_fp16(const AttentionArgs& a, hipStream_t stream);

@@ -8,6 +8,7 @@
 #include <numeric>
 
 #include "../../include/fbgemm_amd.h"
+#include "../../include/fbgemm_amd_bench.h"
 #include "api_error.h"
 #include "decode.h"
 
@@ -416,6 +417,12 @@ int64_t fbgemm_amd_paged_attention_workspace(const fbgemm_amd_paged_cache* cache
   if (int rc = check_attention(cache, requests, query_heads, table_width)) return rc;
   if (requests == 0) return 0;
   return attention_space(attention_workers(*cache, requests, query_heads, attention_max_tokens(*cache, table_width)), cache->dim).total;
+}
+
+int fbgemm_amd_paged_attention_form(const fbgemm_amd_paged_cache* cache) {
+  if (int rc = check_attention(cache, 1, cache ? cache->heads : 1, 1)) return rc;
+  const int64_t e = storage_bytes(cache->row_ty);
+  return attention_form(cache->dim, cache->row_ty == ST_CACHE_INT4 ? 4 : cache->row_ty == ST_INT8 ? 8 : 16, cache->block_size, cache->key_strides[2] * e, cache->value_strides[2] * e);
 }
 
 int fbgemm_amd_paged_attention(

@@ -255,7 +255,7 @@ __device__ __forceinline__ uint32_t inclusive_sum(uint32_t v, int lane) {
 // ROWS: bits of an element: 16, or 8 or 4 in rows with a scale and bias. DP: columns the code is laid out for; FULL: dim is DP, else less: lanes that would have the
 // columns behind read the row's first ones in their place, which meet zeros in the queries or make outputs that nobody wants.
 // PAGE16: pages are whole 16-token tiles, whose addresses are then the same for the wave. PACKED (FULL rows of codes, PAGE16): the
-// rows of a page's tokens follow each other without gaps, and pages are as far apart for values as for keys. 16 of them are then read as one run of bytes, every line by one
+// rows of a page's tokens follow each other without gaps. 16 of them are then read as one run of bytes, every line by one
 // load and marked as read once, and go through LDS, where a lane finds its pieces: 262 143 tokens 103 us, 118 with a gap
 // of 4 bytes behind each row (two tiles ahead instead of one: 2 % more); 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, 400 us, 459 with gaps.
 template <bool BF16, int ROWS, int DP, bool FULL, bool PAGE16, bool PACKED>
@@ -377,9 +377,9 @@ struct Attention {
           tile.partial = true;
           tile.seen &= h ? 0x0f : 0xf0;
         }
-        const int64_t from = block * a.key.block_stride + pages.in_block[h] * ROW; // of keys and of values
-        run[h] = key_base + from;
-        run[2 + h] = value_base + from;
+        const int in_page = pages.in_block[h] * ROW; // of keys and of values
+        run[h] = key_base + (block * a.key.block_stride + in_page);
+        run[2 + h] = value_base + (block * a.value.block_stride + in_page);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -1025,18 +1025,15 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const Attenti
 template <bool BF16, int ROWS, int DP, bool FULL>
 void launch_kernel(const AttentionArgs& a, hipStream_t stream) {
   const dim3 grid(a.workers), block(64 * ATT_WAVES);
-  if (a.block_size % 16) {
-    paged_attention_kernel<BF16, ROWS, DP, FULL, false, false><<<grid, block, 0, stream>>>(a);
-    return;
-  }
-  if constexpr (ROWS < 16 && FULL && !(ROWS == 4 && DP == 64)) {
-    constexpr int ROW = DP * ROWS / 8 + 4;
-    if (a.key.slot_stride == ROW && a.value.slot_stride == ROW && a.key.block_stride == a.value.block_stride) {
+  const AttentionForm form = attention_form(a.dim, ROWS, a.block_size, a.key.slot_stride, a.value.slot_stride);
+  if constexpr (FULL && attention_has_runs(DP, ROWS)) {
+    if (form == ATTENTION_RUNS) {
       paged_attention_kernel<BF16, ROWS, DP, FULL, true, true><<<grid, block, 0, stream>>>(a);
       return;
     }
   }
-  paged_attention_kernel<BF16, ROWS, DP, FULL, true, false><<<grid, block, 0, stream>>>(a);
+  if (form == ATTENTION_LANES) paged_attention_kernel<BF16, ROWS, DP, FULL, false, false><<<grid, block, 0, stream>>>(a);
+  else paged_attention_kernel<BF16, ROWS, DP, FULL, true, false><<<grid, block, 0, stream>>>(a);
 }
 
 template <bool BF16, int ROWS, int DP>

@@ -81,6 +81,11 @@ int fbgemm_amd_tbe_plan_reuse_order(struct fbgemm_amd_tbe_plan* plan, int32_t on
  * among them: what a test of that kernel asks before it believes its result. */
 int64_t fbgemm_amd_tbe_plan_matrix_forwards(struct fbgemm_amd_tbe_plan* plan);
 
+/* How paged attention finds a cache's rows: 0 lane by lane, 1 in pages of whole
+ * tiles of 16 tokens, 2 there as runs of bytes without gaps; negative where it
+ * does not take the cache. */
+int fbgemm_amd_paged_attention_form(const struct fbgemm_amd_paged_cache* cache);
+
 #ifdef __cplusplus
 }
 #endif

@@ -165,3 +165,27 @@ def test_attention_over_4_bit_rows_with_large_scales(decode, power):
         case = large_case(decode, 128, 0, dtype, 4)
         A.check(decode, case, dtype, scale=2.0 ** power)
         A.check(decode, case, dtype, scale=-2.0 ** power, softcap=2.0 ** (power - 3))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_over_caches_whose_pages_are_differently_far_apart(decode, dim, bits, dtype):
+    """Value pages beside something else, key pages behind each other, and the other way round: the same bits as of caches alike."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(dim)
+    row = decode.kv_row_bytes(dim, bits)
+    caches = [torch.randint(0, 256, (60, 2, 32, row), device="cuda", generator=g, dtype=torch.uint8) for _ in "kv"]
+    for c in caches:
+        c[..., :4] = torch.randn((60, 2, 32, 2), device="cuda", generator=g).half().view(torch.uint8)
+    tables = torch.randperm(60, device="cuda", generator=g).to(torch.int32).view(3, 20)
+    lengths = torch.tensor([1, 333, 640], device="cuda")
+    query = torch.randn((3, 8, dim), device="cuda", generator=g).to(dtype)
+    want = decode.paged_attention(query, *caches, tables, lengths, row_bits=bits)
+    for k in range(2):
+        apart = list(caches)
+        apart[k] = torch.full((60, 3, 32, row), 255, device="cuda", dtype=torch.uint8)[:, 1:]  # beside rows of NaN
+        apart[k].copy_(caches[k])
+        got = decode.paged_attention(query, *apart, tables, lengths, row_bits=bits)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.isfinite(want[0]).all()

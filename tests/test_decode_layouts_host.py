@@ -1,11 +1,12 @@
-"""Which layouts of queries, keys and their results ``rotate_positions`` takes: what shares a byte is refused, what does not is not."""
+"""Which layouts of queries, keys and their results ``rotate_positions`` takes: what shares a byte is refused, what does not is not. And which
+caches ``paged_attention`` reads as runs of bytes."""
 import ctypes as C
 import itertools
 import random
 
 import pytest
 
-from test_decode_host import P, decode, lib, refused  # noqa: F401  (decode, lib: fixtures)
+from test_decode_host import P, cache, decode, lib, refused  # noqa: F401  (decode, lib: fixtures)
 
 torch = pytest.importorskip("torch")
 BASE, ELEMENT = 1 << 24, 2
@@ -111,3 +112,21 @@ def test_layouts_of_equal_steps_are_decided_exactly(lib):  # noqa: F811
                 refused(lib, call(lib, tokens, D, rows(0, (token, head), heads), key), "overlap")
             else:
                 taken(lib, tokens, D, rows(0, (token, head), heads), key)
+
+
+@pytest.mark.parametrize("row_ty,row", [(2, lambda d: d + 4), (16, lambda d: d // 2 + 4)])
+def test_rows_without_gaps_are_read_as_runs_however_far_apart_pages_are(lib, row_ty, row):  # noqa: F811
+    """The faster form (a tenth of a call over long contexts) asks for nothing but a page's rows behind each other, 16 of them or a multiple."""
+    form = lambda **c: lib.fbgemm_amd_paged_attention_form(C.byref(cache(row_ty=row_ty, **c)))  # noqa: E731
+    for dim in (64, 128, 256):
+        n, runs = row(dim), 1 if (row_ty, dim) == (16, 64) else 2
+        page = 2 * 16 * n
+        for keys, values in (((page, 16 * n, n),) * 2, ((page, 16 * n, n), (2 * page, 16 * n, n)), ((3 * page, 48 * n, n), (2 * page, 32 * n, n)),
+                             ((page + 4, 16 * n, n), (page, 16 * n, n))):
+            assert form(dim=dim, key_strides=keys, value_strides=values) == runs
+        for keys, values in (((2 * page, 16 * n, n + 4), (page, 16 * n, n)), ((page, 16 * n, n), (2 * page, 16 * n, n + 4)), ((page, n, 2 * n),) * 2):
+            assert form(dim=dim, key_strides=keys, value_strides=values) == 1
+        assert form(dim=dim, block_size=24, key_strides=(48 * n, 24 * n, n), value_strides=(48 * n, 24 * n, n)) == 0
+    n = row(96)
+    assert form(dim=96, key_strides=(32 * n, 16 * n, n), value_strides=(32 * n, 16 * n, n)) == 1
+    assert lib.fbgemm_amd_paged_attention_form(C.byref(cache())) == 1 and lib.fbgemm_amd_paged_attention_form(C.byref(cache(dim=60))) < 0
