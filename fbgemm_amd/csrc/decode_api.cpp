@@ -84,6 +84,12 @@ bool lines_meet(const Line& a, const Line& b, wide d) {
   return every == 0 || rows_within(a.row, b.row, d, every);
 }
 wide between(const void* a, const void* b) { return (wide)(uintptr_t)b - (wide)(uintptr_t)a; }
+bool bytes_meet(const void* a, wide bytes_a, const void* b, wide bytes_b) { return between(a, b) < bytes_a && between(b, a) < bytes_b; }
+// from a cache's first row to its last
+wide cache_extent(const fbgemm_amd_paged_cache& c, const int64_t (&strides)[3]) {
+  if (c.blocks == 0) return 0;
+  return ((wide)(c.blocks - 1) * strides[0] + (wide)(c.heads - 1) * strides[1] + (wide)(c.block_size - 1) * strides[2]) * storage_bytes(c.row_ty) + cache_row_bytes(c);
+}
 
 // [tokens][heads][dim] as lines of rows: a token's heads, or a head's tokens, whichever are closer together. outer: these lines as solid rows
 struct Grid {
@@ -332,8 +338,17 @@ int fbgemm_amd_kv_cache_read(
     for (const CacheRows& c : a.cache) ok = ok && divides(p, {c.block_stride, c.head_stride, c.slot_stride}) && (uintptr_t)c.base % p == 0;
     return ok;
   };
+  const auto check_apart = [&]() { // a row may be read after another one's thread has written
+    const wide bytes = (wide)tokens * cache->heads * cache->dim * storage_bytes(output_ty);
+    if (bytes_meet(d_key, bytes, d_value, bytes)) return fail(FBGEMM_AMD_E_ARG, "keys and values must not overlap");
+    for (const char* out : a.out)
+      if (bytes_meet(out, bytes, d_key_cache, cache_extent(*cache, cache->key_strides)) || bytes_meet(out, bytes, d_value_cache, cache_extent(*cache, cache->value_strides)))
+        return fail(FBGEMM_AMD_E_ARG, "keys and values must not overlap the cache");
+    return 0;
+  };
   if (codes) {
     if (!on(4)) return fail(FBGEMM_AMD_E_ARG, "8-bit and 4-bit rows begin on 4-byte boundaries");
+    if (int rc = check_apart()) return rc;
     const bool whole = cache->dim % READ_RUN == 0;
     pieces(whole ? cache->dim / READ_RUN : cache->dim);
     HIP_TRY(launch_kv_read_coded(a, cache->row_ty == ST_INT8 ? 8 : 4, output_ty, whole, (hipStream_t)stream));
@@ -344,6 +359,7 @@ int fbgemm_amd_kv_cache_read(
   const auto fits = [&](int p) { return row_bytes % p == 0 && on(p); };
   while (piece > 2 && !fits(piece)) piece >>= 1;
   if (!fits(piece)) return fail(FBGEMM_AMD_E_ARG, "rows are not aligned to their elements");
+  if (int rc = check_apart()) return rc;
   pieces(row_bytes / piece);
   HIP_TRY(launch_kv_read(a, piece, (hipStream_t)stream));
   return 0;

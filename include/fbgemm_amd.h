@@ -634,7 +634,8 @@ int fbgemm_amd_kv_cache_append(
     void* d_status, void* stream);
 
 /* Rows of requests' tokens, out of their pages into dense arrays d_key and d_value
- * [tokens][heads][dim] on 16-byte boundaries: what attention of a prompt's later part
+ * [tokens][heads][dim] on 16-byte boundaries, which overlap neither each other nor what lies
+ * between a cache's first row and its last: what attention of a prompt's later part
  * reads of its earlier one. Token i belongs to the request r with d_offsets[r] <= i <
  * d_offsets[r + 1] (requests + 1 entries, ascending, int32 or int64 by index_bits) and is at position
  * d_starts[r] + i - d_offsets[r] of it (d_starts NULL: 0). Rows come as they are, in the cache's type;

@@ -1,4 +1,4 @@
-"""Which layouts of queries, keys and their results ``rotate_positions`` takes: what shares a byte is refused, what does not is not. And which
+"""Which layouts of queries, keys and their results ``rotate_positions`` takes: what shares a byte is refused, what does not is not. The same of ``kv_cache_read``. And which
 caches ``paged_attention`` reads as runs of bytes."""
 import ctypes as C
 import itertools
@@ -130,3 +130,39 @@ def test_rows_without_gaps_are_read_as_runs_however_far_apart_pages_are(lib, row
     n = row(96)
     assert form(dim=96, key_strides=(32 * n, 16 * n, n), value_strides=(32 * n, 16 * n, n)) == 1
     assert lib.fbgemm_amd_paged_attention_form(C.byref(cache())) == 1 and lib.fbgemm_amd_paged_attention_form(C.byref(cache(dim=60))) < 0
+
+
+def read_call(lib, key, value, key_cache, value_cache, tokens=5, **change):  # noqa: F811
+    at = lambda n: C.c_void_p(BASE + n)  # noqa: E731
+    return lib.fbgemm_amd_kv_cache_read(C.byref(cache(**change)), at(key_cache), at(value_cache), P, 4, 4, P, None, 32, 2, tokens, 5, at(key), at(value), None, None)
+
+
+READ = 5 * 2 * 64 * 2  # bytes of a result
+HELD = 4 * 2048 * 2    # of a cache
+CACHES4 = dict(row_ty=16, key_strides=(1152, 576, 36), value_strides=(2304, 576, 36))
+HELD4 = 4 * 1152, 3 * 2304 + 1152
+
+
+def test_results_of_reading_that_overlap_are_refused(lib):  # noqa: F811
+    far = 1 << 20
+    for key, value in ((0, 0), (0, 16), (0, READ - 16), (READ - 16, 0)):
+        refused(lib, read_call(lib, key, value, far, 2 * far), "overlap")
+    for k in (0, 1):
+        for at in (0, 16, READ - 16, 16 - HELD):
+            caches = [2 * far, 3 * far]
+            caches[k] = far + at  # with the values' result at `far`
+            refused(lib, read_call(lib, 0, far, *caches), "overlap the cache")
+            refused(lib, read_call(lib, far, 0, *caches), "overlap the cache")
+        caches = [2 * far, 3 * far]
+        caches[k] = far + 16 - HELD4[k]
+        refused(lib, read_call(lib, 0, far, *caches, **CACHES4), "overlap the cache")
+
+
+@without_gpu
+def test_results_of_reading_beside_each_other_are_taken(lib):  # noqa: F811
+    far = 1 << 20
+    for args in ((0, READ, far, 2 * far), (READ, 0, far, far), (0, READ, 2 * READ, 2 * READ + HELD), (HELD, HELD + READ, 0, 0)):
+        assert read_call(lib, *args) == -2, lib.fbgemm_amd_last_error()
+    assert read_call(lib, HELD4[0], HELD4[0] + READ, 0, HELD4[0] + 2 * READ, **CACHES4) == -2, lib.fbgemm_amd_last_error()
+    assert read_call(lib, 0, READ, 0, 0, blocks=0) == -2, lib.fbgemm_amd_last_error()
+    assert read_call(lib, 0, 0, 0, 0, tokens=0) == 0
