@@ -37,11 +37,11 @@ __device__ __forceinline__ Rows rows_of(const ReadArgs& a, int64_t token) {
     if ((int64_t)offsets[mid] <= token) lo = mid;
     else hi = mid;
   }
-  const int64_t in_request = token - (int64_t)offsets[lo];
+  const int64_t in_request = (int64_t)((uint64_t)token - (uint64_t)(int64_t)offsets[lo]); // (offsets may be anything; beyond 2^63 it is below 0)
   const int64_t start = a.starts ? (int64_t)reinterpret_cast<const index_t*>(a.starts)[lo] : 0;
   const int64_t room = a.table_width * a.block.d; // below 2^31, as the number of tokens
-  // (sums of 64-bit numbers far from 32-bit ones are no positions)
-  if (in_request >= 0 && start > -(1ll << 32) && start < room && start + in_request >= 0 && start + in_request < room) {
+  // 0 <= start + in_request < room, by differences of numbers that are small: the sum itself could be beyond 2^63, and mean anything to the compiler
+  if (in_request >= 0 && start > -(1ll << 32) && start < room && in_request >= -start && in_request < room - start) {
     const uint32_t position = (uint32_t)(start + in_request), column = divide(position, a.block);
     const int32_t block = a.tables[lo * a.table_stride + column];
     if (block >= 0 && block < a.blocks) {

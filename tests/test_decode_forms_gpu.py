@@ -189,3 +189,20 @@ def test_attention_over_caches_whose_pages_are_differently_far_apart(decode, dim
         got = decode.paged_attention(query, *apart, tables, lengths, row_bits=bits)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert torch.isfinite(want[0]).all()
+
+
+def test_reading_back_by_offsets_and_starts_at_the_ends_of_64_bits(decode):
+    """Tokens of such requests have no page: zeros, and the first one's number in the status block."""
+    from fbgemm_amd import ops
+    c = torch.randint(1, 100, (6, 2, 16, 36), device="cuda", dtype=torch.uint8)
+    tables = torch.arange(6, device="cuda", dtype=torch.int32).view(2, 3)
+    least, most = -2 ** 63, 2 ** 63 - 1
+    st = ops.Status()
+    for offsets, starts in (((least, 3, 9), (0, 0)), ((least, 3, 9), (5, 0)), ((least + 1, 3, 9), (47, 0)), ((-2 ** 62, 3, 9), (47, 0)), ((0, 3, 9), (most, 0)),
+                            ((0, 3, 9), (least, 0)), ((-most, 3, 9), (most, 0)), ((-2 ** 32 + 3, 3, 9), (-2 ** 32, 0))):
+        st.clear()
+        at = lambda v: torch.tensor(v, device="cuda")  # noqa: E731
+        key, value = decode.kv_cache_read(c, c, tables, at(offsets), 9, 64, starts=at(starts), status=st, row_bits=4)
+        want = torch.from_numpy(R.rows4_values(c[3].cpu().numpy(), 64)).float().cuda().transpose(0, 1)
+        assert (key[:3] == 0).all() and torch.equal(key[3:], want[:6]) and torch.equal(value, key)
+        assert st.read() == (1, 0)
