@@ -206,3 +206,66 @@ def test_reading_back_by_offsets_and_starts_at_the_ends_of_64_bits(decode):
         want = torch.from_numpy(R.rows4_values(c[3].cpu().numpy(), 64)).float().cuda().transpose(0, 1)
         assert (key[:3] == 0).all() and torch.equal(key[3:], want[:6]) and torch.equal(value, key)
         assert st.read() == (1, 0)
+
+
+# ---- more work than one launch has workgroups for ----------------------------------------------------
+
+
+def test_rotation_of_more_tokens_than_workgroups(decode):
+    tokens = (1 << 22) + 5
+    x = torch.randn((tokens, 2, 8), device="cuda").bfloat16()
+    positions, f = torch.arange(tokens, device="cuda"), decode.rotary_frequencies(8)
+    got = decode.rotate_positions(x[:, :1], x[:, 1:], positions, f)
+    for part in (slice(0, 9), slice((1 << 22) - 4, None)):
+        want = check_rotation(decode, x[part, :1], x[part, 1:], positions[part], f)
+        assert torch.equal(got[0][part], want[0]) and torch.equal(got[1][part], want[1])
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_reading_back_of_more_tokens_than_workgroups(decode, bits):
+    tokens = (1 << 24) + 77
+    blocks = -(-tokens // 16)
+    if bits == 16:
+        c = torch.randn((blocks, 1, 16, 8), device="cuda").bfloat16()
+    else:
+        c = torch.randint(0, 256, (blocks, 1, 16, decode.kv_row_bytes(8, 4)), device="cuda", dtype=torch.uint8)
+        c[..., :4] = torch.randn((blocks, 1, 16, 2), device="cuda").half().view(torch.uint8)
+    tables = torch.randperm(blocks, device="cuda").int()[None]
+    at = lambda *v: torch.tensor(v, device="cuda")  # noqa: E731
+    kw = dict(dtype=torch.bfloat16, row_bits=8 if bits == 16 else 4)
+    key, value = decode.kv_cache_read(c, c, tables, at(0, tokens), tokens, 8, **kw)
+    assert torch.equal(key, value)
+    if bits == 16:
+        assert torch.equal(key, c[tables[0].long(), 0].view(-1, 1, 8)[:tokens])
+    for first, n in ((0, 50), ((1 << 24) - 40, 117)):
+        want = decode.kv_cache_read(c, c, tables, at(0, n), n, 8, starts=at(first), **kw)
+        assert torch.equal(key[first:first + n], want[0])
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+def test_append_of_more_rows_than_workgroups(decode, shift):
+    """4-bit rows of 8: a lane a row, 256 rows a workgroup and 8 192 of those."""
+    from fbgemm_amd import ops
+    tokens = 8192 * 256 + 300
+    new = torch.randn((tokens, 1, 16), device="cuda").bfloat16()[..., shift:shift + 8]
+    kc, vc = (torch.zeros((tokens // 4, 1, 4, 8), device="cuda", dtype=torch.uint8) for _ in "kv")
+    slots = torch.randperm(tokens, device="cuda")
+    decode.kv_cache_append(new, -new, kc, vc, slots, row_bits=4)
+    for c, x in ((kc, new), (vc, -new)):
+        want = ops.quantize_rowwise(x.float().reshape(-1, 8), 4, layout=ops.QLAYOUT_TBE)
+        assert torch.equal(c.view(tokens, 8)[slots], want)
+
+
+def test_samples_of_more_rows_than_a_launch_takes(decode):
+    """Rows of one launch have fewer than 2^32 threads, 1 024 of them a row; all rows have the same logits."""
+    rows = (1 << 22) + 9
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    x = (3 * torch.randn((1, 33_000), device="cuda", generator=g)).bfloat16()
+    uniform = torch.rand(rows, device="cuda", generator=g)
+    top_k = torch.randint(1, 40, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    got = decode.sample_tokens(x.expand(rows, -1), uniform, top_k=top_k)
+    for part in (slice(0, 99), slice((1 << 22) - 50, None)):
+        want = decode.sample_tokens(x.expand(len(uniform[part]), -1), uniform[part], top_k=top_k[part])
+        assert torch.equal(got.tokens[part], want.tokens) and torch.equal(got.log_probabilities[part], want.log_probabilities)
+    assert (got.tokens >= 0).all()
