@@ -269,3 +269,46 @@ def test_samples_of_more_rows_than_a_launch_takes(decode):
         want = decode.sample_tokens(x.expand(len(uniform[part]), -1), uniform[part], top_k=top_k[part])
         assert torch.equal(got.tokens[part], want.tokens) and torch.equal(got.log_probabilities[part], want.log_probabilities)
     assert (got.tokens >= 0).all()
+
+
+# ---- what refusals say --------------------------------------------------------------------------------
+
+
+def test_refusals_name_what_they_refuse(decode):
+    z = lambda *shape, t=torch.bfloat16: torch.zeros(shape, device="cuda", dtype=t)  # noqa: E731
+    q, k, p, f = z(5, 8, 64), z(5, 2, 64), torch.arange(5, device="cuda"), decode.rotary_frequencies(64)
+    rotate = lambda query=q, key=k, positions=p, frequencies=f, **kw: decode.rotate_positions(query, key, positions, frequencies, **kw)  # noqa: E731
+    logits, uniform = z(5, 100), z(5, t=torch.float32)
+    sample = lambda x=logits, u=uniform, **kw: decode.sample_tokens(x, u, **kw)  # noqa: E731
+    u8 = lambda *shape: z(*shape, t=torch.uint8)  # noqa: E731
+    c4, c16, tables, offsets = u8(4, 2, 16, 36), z(4, 2, 16, 64), z(3, 2, t=torch.int32), torch.arange(4, device="cuda")
+    read = lambda kc=c4, vc=c4, t=tables, o=offsets, n=3, dim=64, dtype=None, bits=4, **kw: decode.kv_cache_read(kc, vc, t, o, n, dim, dtype, row_bits=bits, **kw)  # noqa: E731
+    append = lambda key=z(3, 2, 64), kc=c4, vc=u8(4, 2, 16, 36), bits=4: decode.kv_cache_append(key, key, kc, vc, torch.arange(3, device="cuda"), row_bits=bits)  # noqa: E731
+    attend = lambda query=z(3, 4, 64), kc=c4, vc=c4, bits=4: decode.paged_attention(query, kc, vc, tables, offsets[1:], row_bits=bits)  # noqa: E731
+    refused = [
+        (lambda: rotate(query=q.float()), "of one type"), (lambda: rotate(query=q.double(), key=k.double()), "float32, float16 or bfloat16"), (lambda: rotate(query=q[:4]), "of one type"),
+        (lambda: rotate(positions=p.float()), "positions must be int32 or int64"), (lambda: rotate(positions=p[:4]), "positions must hold 5"), (lambda: rotate(positions=p.cpu()), "positions must be on"),
+        (lambda: rotate(frequencies=f.float()), "frequencies must be Double"), (lambda: rotate(frequencies=torch.ones(33, device="cuda", dtype=torch.float64)), "33 frequencies"),
+        (lambda: rotate(magnitude=float("inf")), "magnitude must be finite"), (lambda: rotate(query=z(5, 64, 8).transpose(1, 2), key=z(5, 64, 2).transpose(1, 2)), "next to each other"),
+        (lambda: rotate(out=(q, q[:, :2])), "must not overlap"), (lambda: rotate(out=(q, k[:, :1].expand(-1, 2, -1))), "rows of a result must not overlap"),
+        (lambda: rotate(out=(q.float(), k)), "shapes and type of query and key"), (lambda: rotate(out=(q[:, :, :63], k)), "shapes and type of query and key"),
+        (lambda: sample(x=logits.double()), "float32, float16 or bfloat16"), (lambda: sample(x=logits[0]), r"logits must be \[rows, vocab\]"), (lambda: sample(x=z(100, 5).t()), "next to each other"),
+        (lambda: sample(x=logits[:, :0]), "vocab must be in 1"), (lambda: sample(u=uniform[:4]), "uniform must hold 5"), (lambda: sample(u=uniform.double()), "uniform must be Float"),
+        (lambda: sample(temperature=uniform[:3]), "temperature must hold 5"), (lambda: sample(top_k=p), "top_k must be Int"), (lambda: sample(top_p=uniform.half()), "top_p must be Float"),
+        (lambda: sample(min_p=uniform.cpu()), "min_p must be on"), (lambda: sample(u=uniform[:1].expand(5)), "uniform must be contiguous"),
+        (lambda: read(bits=8), "rows of 36 do not hold 64"), (lambda: read(bits=2), "row_bits must be 8 or 4"), (lambda: read(dim=63), "even number"), (lambda: read(dim=0), "dim must be in 1"),
+        (lambda: read(dtype=torch.float64), "float32, float16 or bfloat16"), (lambda: read(o=offsets.float()), "offsets must be int32 or int64"), (lambda: read(o=offsets[:3]), "block_tables must be int32"),
+        (lambda: read(n=-1), "num_tokens must be in"), (lambda: read(starts=offsets), "starts must hold 3"), (lambda: read(kc=c16, vc=c16), "4-bit rows are in a uint8 cache"),
+        (lambda: read(kc=c16, vc=c16, bits=8, dtype=torch.float32), "rows come as they are stored"), (lambda: read(vc=u8(4, 2, 16, 40)), "same shape and type"),
+        (lambda: append(bits=8), "rows of 36 do not hold 64"), (lambda: append(key=z(3, 2, 63)), "even number"), (lambda: append(kc=u8(4, 2, 16, 37), vc=u8(4, 2, 16, 37)), "4-byte"),
+        (lambda: append(vc=u8(4, 1, 16, 36).expand(-1, 2, -1, -1)), "rows of a cache must not overlap"),
+        (lambda: attend(bits=8), "rows of 36 do not hold 64"), (lambda: attend(query=z(3, 4, 64, t=torch.float32)), "FP16 or BF16|float16 or bfloat16"), (lambda: attend(kc=c16, vc=c16), "4-bit rows are in a uint8 cache"),
+    ]
+    for i, (call, word) in enumerate(refused):
+        with pytest.raises((RuntimeError, ValueError), match=word):
+            call()
+            print("not refused:", i)
+    # heads of which there are none, and no tokens
+    none = rotate(key=k[:, :0])
+    assert none[1].shape == (5, 0, 64) and torch.equal(none[0], q)
+    assert rotate(query=q[:0], key=k[:0], positions=p[:0])[0].shape == (0, 8, 64)
