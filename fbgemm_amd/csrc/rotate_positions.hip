@@ -6,7 +6,8 @@
 // and the rest of the head as it is. In fp32, rounded once.
 //
 // Angles are taken in fp64, as quarters of a turn: what is left of a far position's angle behind its whole
-// quarters is off by 2^-53 of the angle, in fp32 it would be 2^-24 of it (262 143 radians: 0.02). Sine and
+// quarters is off by three roundings of 2^-53 of the angle (2 / pi, its product with the frequency, that with the position), less than
+// 2^-51; in fp32 it would be 2^-24 of it (262 143 radians: 0.02). Sine and
 // cosine of the rest, at most pi/4, are their series.
 //
 // Bound by memory: every element is read once and written once. 16 384 tokens of 40 heads of 128, bf16: 52 us, 6.4 TB/s; 64 of them:

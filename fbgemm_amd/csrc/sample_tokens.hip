@@ -13,7 +13,8 @@
 // A large vocabulary has a border of two tokens within 1e-6 of almost every u, so sums in fp32 would often draw a
 // neighbour. w is a whole number here, 2^fraction times larger and rounded (fraction: 45 bits for
 // 131 071 tokens): sums of whole numbers are the same in any order, so lanes, waves and LDS atomics add them as they come,
-// and a running sum is off by no more than the w's own roundings, some 2^-46 of the largest each. exp is made in fp64 (2^-48).
+// and a running sum is off by no more than the w's own roundings, 2^-46 of the largest each (2^-29 if all of them went one way; u has 24 bits).
+// exp is made in fp64 (2^-48).
 //
 // A workgroup has a row. It reads it once to keep the largest logit of every few pieces of 16 bytes, in LDS. Few of these groups
 // hold a token that can matter: with top-k those whose largest is above the k-th largest of the groups' largest, without those with a

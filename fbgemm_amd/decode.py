@@ -187,6 +187,7 @@ def sample_tokens(logits, uniform, temperature=None, top_k=None, top_p=None, min
     are none too, and a ``temperature`` or ``top_p`` that is not above 0 is the first of the largest logits, of probability 1.
 
     NaN and -inf are never drawn, +inf counts as the largest finite number; a row with nothing else gives -1 and -inf. Sums
-    are of whole numbers (``w`` in units of 2 ** -42 of the largest and finer), the same on every run. Returns ``Samples``: ``tokens``
+    are of whole numbers, the same on every run: ``w`` rounded to units of ``2 ** -min(50, 62 - vocab.bit_length())`` of the largest (2 ** -45
+    for 131 071 tokens, 2 ** -41 for 2 ** 20), half a unit a token. No gradient goes through it. Returns ``Samples``: ``tokens``
     (int64) and ``log_probabilities`` (fp32), the logarithm of the probability a token was drawn with."""
     return Samples._make(_sample(logits, uniform, temperature, top_k, top_p, min_p))

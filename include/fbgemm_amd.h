@@ -726,9 +726,12 @@ int fbgemm_amd_penalize_logits(
  * >= 1: those of the largest logit); with a temperature or top_p that is not above 0 it
  * is the first of the largest ones, of probability 1. NaN and -inf are never drawn,
  * +inf counts as the largest finite fp32 number; a row with nothing else gives -1 and
- * -inf. Sums are of whole numbers, w in units of 2^-(62 - bits of vocab) at most: a draw
- * is that of exact sums but within some 2^-40 of a border of two tokens. vocab: 1..2^20,
- * rows up to 2^24; a row stride of 0 shares the logits. */
+ * -inf. Sums are of whole numbers, w rounded to units of 2^-f of the largest, f the
+ * smaller of 50 and 62 - bits of vocab (45 for 131 071 tokens, 41 for 2^20): the same in
+ * any order, and off by little more than half a unit a token. A draw is that of exact
+ * sums but within some vocab / 2 units of a border of two tokens (2^-29 of the largest w
+ * for 131 071 tokens, 2^-22 for 2^20). vocab: 1..2^20, rows up to 2^24; a row stride of 0 shares the
+ * logits. */
 int fbgemm_amd_sample_tokens(
     const void* d_logits, int32_t logits_ty, int64_t rows, int64_t vocab, int64_t logits_stride, const float* d_uniform,
     const float* d_temperature, const int32_t* d_top_k, const float* d_top_p, const float* d_min_p, int64_t* d_tokens,
