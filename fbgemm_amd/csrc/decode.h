@@ -124,8 +124,8 @@ struct AttentionArgs {
 };
 constexpr int ATTENTION_STEP = 128; // tokens of a unit of work
 // Workgroups of the attention kernel that a compute unit holds at once: what its registers leave room for. bits: of an element of the
-// rows; pages: whole tiles of 16 tokens. 4-bit rows in such pages, 256 requests of 16 to 8 192 tokens, us: three with one tile on its way 252, two
-// with two tiles 268, with three 279; three with two tiles do not fit the registers, 352.
+// rows; pages: whole tiles of 16 tokens. 4-bit rows in such pages, 256 requests of 16 to 8 192 tokens, times three with one tile on its way: two
+// with two tiles 1.06, with three 1.11; three with two tiles do not fit the registers, 1.40.
 constexpr int attention_residents(int dim, int bits, bool pages) {
   if (dim > 128) return 1;
   if (bits == 4) return pages ? 3 : 2;

@@ -192,11 +192,15 @@ unsigned grid_for(int64_t tokens, int run) {
   return (unsigned)(runs < (1 << 20) ? runs : 1 << 20);
 }
 // f(tokens of a workgroup, whether results are beyond the caches): enough tokens that a thread has a few, where there are some for all of the device.
-// us with 1, 4 and 16 of them, 4-bit rows of 8 heads of 128 to bf16, then 16-bit rows of 2 heads of 64:
+// us with 1, 4 and 16 of them, of the same caches again and again, 4-bit rows of 8 heads of 128 to bf16, then 16-bit rows of 2 heads of 64:
 //    1 024     3.6  3.7  4.7     3.0  2.9  3.1
 //    2 048     5.2  4.4  5.2     4.0  3.1  3.1
 //    8 192    13.5  9.4  8.7     8.7  4.7  3.9
-//   65 536    77.7 43.3 49.0    64.8 23.2 12.8    (the former past the caches; 8-bit rows 80.0 53.0 48.6)
+// With 4 and 16, of other caches in every call, the result of all but the last past the caches from 65 536 on:
+//              4 bits, 8 x 128   8 bits, 8 x 128   16 bits, 8 x 128   16 bits, 2 x 64
+//    8 192          12.4  11.5        14.2  12.5         14.5  15.7        7.3   7.4
+//   65 536          64.8  68.4        81.1  78.2         97.7 104.3       28.5  18.0
+// One rule for them all: what 16 lose with long rows, 4 would lose several times over with short ones.
 template <typename F>
 void by_tokens(const ReadArgs& a, int64_t row_bytes, F&& f) {
   if (2 * a.tokens * a.heads * row_bytes >= (128 << 20)) f(std::integral_constant<int, 16>(), std::true_type());

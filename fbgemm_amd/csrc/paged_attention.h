@@ -35,9 +35,10 @@
 // no instruction converts them. s_t = a_t (q . k4_t) + b_t sum(q) as above, and values by weights p_t a_t for v4, less 8 times the sum of those
 // weights, beside p_t (b_t + 8 a_t); weights are bf16 pairs 2^72 times larger for both types of queries, so that products with 2^-133 are normal
 // numbers. What bounds them is instructions, not bytes: some 330 vector instructions a wave for 32 tokens of 128 (two thirds of the cycles, with
-// three workgroups a compute unit and what is left their waits). The 256 requests above, 1.15 GB of rows: 252 us, 4.55 TB/s, 2.7 times less than in 16
-// bits; 64 requests of 1 to 4 096: 50 us; one of 500: 10.4 us. (Two tiles at once where 8 queries or fewer share a head, which the other
-// half of the product's columns has room for, take 18 % fewer instructions, but registers and LDS banks run short: 271, 57 and 12.6 us.)
+// three workgroups a compute unit and what is left their waits). The 256 requests above, 1.15 GB of rows: 262 us, 4.4 TB/s, 2.6 times less than in 16
+// bits; 64 requests of 1 to 4 096: 50 us; one of 500: 10.4 us. Scores of any size, which cost 1 to 2 % of that: units that are no larger than 2^100, and
+// weights of far maxima by differences. (Two tiles at once where 8 queries or fewer share a head, which the other half of the product's
+// columns has room for, take 18 % fewer instructions, but registers and LDS banks run short: 8, 14 and 20 % longer.)
 //
 // Work: steps of 128 tokens of a (request, key head, 16 queries), 32 for each of a worker's (workgroup's) four waves, numbered in
 // that order. Each of W workers takes a W-th of them in a row, whatever requests they are of, so that all end together
@@ -256,8 +257,9 @@ __device__ __forceinline__ uint32_t inclusive_sum(uint32_t v, int lane) {
 // columns behind read the row's first ones in their place, which meet zeros in the queries or make outputs that nobody wants.
 // PAGE16: pages are whole 16-token tiles, whose addresses are then the same for the wave. PACKED (FULL rows of codes, PAGE16): the
 // rows of a page's tokens follow each other without gaps. 16 of them are then read as one run of bytes, every line by one
-// load and marked as read once, and go through LDS, where a lane finds its pieces: 262 143 tokens 103 us, 118 with a gap
-// of 4 bytes behind each row (two tiles ahead instead of one: 2 % more); 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, 400 us, 459 with gaps.
+// load and marked as read once, and go through LDS, where a lane finds its pieces: 262 143 tokens 103 us, 115 with a gap
+// of 4 bytes behind each row (two tiles ahead instead of one: 2 % more); 256 requests of 16 to 8 192 tokens, 64 queries on 8 heads of 128, 400 us, 443 with gaps
+// (4-bit rows 262 and 283).
 template <bool BF16, int ROWS, int DP, bool FULL, bool PAGE16, bool PACKED>
 struct Attention {
   static constexpr bool ROWS8 = ROWS == 8, ROWS4 = ROWS == 4, CODES = ROWS8 || ROWS4;

@@ -10,9 +10,10 @@
 // 2^-51; in fp32 it would be 2^-24 of it (262 143 radians: 0.02). Sine and
 // cosine of the rest, at most pi/4, are their series.
 //
-// Bound by memory: every element is read once and written once. 16 384 tokens of 40 heads of 128, bf16: 52 us, 6.4 TB/s; 64 of them:
-// 3.0 us. A workgroup has a token: it makes its sines once, in LDS, and turns all heads of queries and keys by them, 16 bytes (two of them,
-// where a pair's elements are apart) a thread at a time. (Four tokens a workgroup, for longer ones: 57.5 us; 8 192 tokens 29.4 instead of 27.2.)
+// Bound by memory: every element is read once and written once. 16 384 tokens of 40 heads of 128, bf16: 54.5 us, 6.2 TB/s; 64 of them:
+// 2.9 us. A workgroup has a token: it makes its sines once, in LDS, and turns all heads of queries and keys by them, 16 bytes (two of them,
+// where a pair's elements are apart) a thread at a time. (Four tokens a workgroup take 8 to 10 % longer.) Pairs that do not fill 16 bytes go
+// element by element: those tokens with heads of 96, 24 of it turned, 156 us, 1.6 TB/s.
 #include "decode.h"
 
 namespace fbgemm_amd {
@@ -20,8 +21,15 @@ namespace fbgemm_amd {
 namespace {
 
 constexpr int THREADS = 256;
-// Bytes of the results from which on they are marked as not read again soon: 168 MB (16 384 tokens of 40 heads of 128, four a workgroup) 65.9 -> 60.5 us,
-// 31 MB (4 095 tokens of 24 heads of 80 fp32 numbers), which the last cache holds, 12.4 -> 16.0
+// Bytes of the results from which on they are marked as not read again soon. us without the mark and with it, on other tensors in every call, and
+// on the same ones, which the last cache may hold (heads of 128 in bf16, the first row heads of 80 in fp32):
+//    31 MB   16.1  17.3   12.3  16.9
+//    61 MB   23.4  22.9   19.8  21.9
+//    84 MB   29.2  29.4   26.1  28.5
+//   123 MB   39.4  41.2   37.4  40.2
+//   168 MB   61.8  55.1   60.8  54.2
+//   336 MB  120.2 106.3  119.6 105.6
+// Between the border and some 130 MB the mark costs a little and leaves the cache to others.
 constexpr int64_t STREAM_FROM = 64 << 20;
 typedef __attribute__((ext_vector_type(4))) uint32_t piece16;
 

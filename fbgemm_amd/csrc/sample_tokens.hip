@@ -959,6 +959,7 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
   //   300 rows of 32 000        11.7 25.9 37.1 65.0    8.9 13.9 39.1 60.8
   //   1 024 rows of 32 000      26.8 54.4 77.0 132     19.0 27.9 70.3 112
   //   300 rows of 65 536        14.5 31.8 51.8 88.9   12.4 17.9 67.6 104
+  // (The last, with 16: which rows have a filter is known on the device alone, and those without one take longest.)
   if (a.vocab <= 8192 || (a.rows > a.compute_units && a.vocab <= 32768)) return launch_shape<TY, 256>(a, stream);
   return launch_shape<TY, 1024>(a, stream);
 }

@@ -22,7 +22,7 @@ and ``t.lengths`` and ``t.free_start`` are the next step's. Everything stays on 
 nothing waits, and a step can be captured into a graph. ``examples/paged_decode.py`` runs one.
 
 All tensors are device tensors; everything runs in the HIP library (the operators ``torch.ops.fbgemm_amd.*``, which these
-functions call), nothing here computes.
+functions call), nothing here computes. It is for inference: of them ``rotate_positions`` alone has a gradient.
 """
 import collections
 import math
