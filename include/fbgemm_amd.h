@@ -723,8 +723,9 @@ int fbgemm_amd_penalize_logits(
  * (or the last one), d_log_probability[row] the logarithm of its w over the whole. Of
  * the four lists, one number per row, each may be NULL: temperature 1, top_k and min_p
  * 0, top_p 1. top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 leave every token (min_p
- * >= 1: those of the largest logit); with a temperature or top_p that is not above 0 it
- * is the first of the largest ones, of probability 1. NaN and -inf are never drawn,
+ * >= 1: those of the largest logit, and any so near it by the temperature that its w is
+ * rounded to the same); with a temperature or top_p that is not above 0 it is the first
+ * of the largest ones, of probability 1. NaN and -inf are never drawn,
  * +inf counts as the largest finite fp32 number; a row with nothing else gives -1 and
  * -inf. Sums are of whole numbers, w rounded to units of 2^-f of the largest, f the
  * smaller of 50 and 62 - bits of vocab (45 for 131 071 tokens, 41 for 2^20): the same in
